@@ -22,6 +22,7 @@
 #include "rx_common.h"
 
 #include <algorithm>
+#include <cstring>
 #include <deque>
 #include <mutex>
 #include <vector>
@@ -306,6 +307,62 @@ struct PinnedArena {
 };
 std::vector<PinnedArena> g_arenas;
 long long g_pin_calls = 0, g_pin_bytes = 0;
+bool g_pin_refused = false;  // the system does not register existing memory: bounce instead
+
+// Where registration is refused, host ranges go through two halves of one pinned allocation: a
+// half is filled by memcpy and drained by DMA on the copy stream while the other one fills. The
+// memory lives as long as the process (copies may be in flight at any time).
+struct Bounce {
+  static constexpr size_t kHalf = 4u << 20;
+  uint8_t* mem = nullptr;
+  hipEvent_t drained[2] = {nullptr, nullptr};
+  bool busy[2] = {false, false};
+  int half = 0;
+  size_t fill = 0;
+};
+Bounce g_bounce;
+
+// Close the half that is being filled: its copies are all enqueued on `copy`.
+int rx_bounce_close(hipStream_t copy) {
+  Bounce& b = g_bounce;
+  if (b.fill == 0) return 0;
+  RX_CHECK(hipEventRecord(b.drained[b.half], copy));
+  b.busy[b.half] = true;
+  b.half ^= 1;
+  b.fill = 0;
+  return 0;
+}
+
+// dst <- [host, host + bytes) through the bounce buffer, in order on `copy`. Caller holds g_mu.
+int rx_bounce_copy(uint8_t* dst, uintptr_t host, size_t bytes, hipStream_t copy, long long* ncopies) {
+  Bounce& b = g_bounce;
+  if (b.mem == nullptr) {
+    RX_CHECK(hipHostMalloc(reinterpret_cast<void**>(&b.mem), 2 * Bounce::kHalf, hipHostMallocPortable));
+    for (auto& e : b.drained) RX_CHECK(hipEventCreateWithFlags(&e, hipEventDisableTiming));
+    ++g_pin_calls;
+    g_pin_bytes += (long long)(2 * Bounce::kHalf);
+  }
+  while (bytes > 0) {
+    if (b.fill == Bounce::kHalf) {
+      const int rc = rx_bounce_close(copy);
+      if (rc) return rc;
+    }
+    if (b.busy[b.half]) {
+      RX_CHECK(hipEventSynchronize(b.drained[b.half]));
+      b.busy[b.half] = false;
+    }
+    const size_t n = std::min(bytes, Bounce::kHalf - b.fill);
+    uint8_t* at = b.mem + (size_t)b.half * Bounce::kHalf + b.fill;
+    memcpy(at, reinterpret_cast<const void*>(host), n);
+    RX_CHECK(hipMemcpyAsync(dst, at, n, hipMemcpyHostToDevice, copy));
+    ++*ncopies;
+    b.fill += n;
+    dst += n;
+    host += n;
+    bytes -= n;
+  }
+  return 0;
+}
 
 // Largest n <= want such that [host, host + n) lies inside one registration run (or `want`
 // when the address is in no registered arena). Caller holds g_mu.
@@ -359,13 +416,15 @@ int rx_arrow_ingest(const IngestArgs* a, void* out, hipStream_t stream) {
   return rx_ingest_launch(*a, out, stream);
 }
 
-// Pin [addr, addr + len) of the arena [base, base + cap) (chunk-granular, idempotent).
-// Returns 0 on success, a HIP error code otherwise.
+// Pin [addr, addr + len) of the arena [base, base + cap) (chunk-granular, idempotent). A system
+// that refuses to register existing memory is asked once: rx_ingest_dma then bounces the range
+// through pinned memory of its own. Returns 0, or -1 for a range outside the arena.
 int rx_pin_range(unsigned long long base, unsigned long long cap, unsigned long long addr,
                  unsigned long long len, unsigned long long chunk) {
   if (len == 0) return 0;
   if (addr < base || addr + len > base + cap || chunk == 0) return -1;
   std::lock_guard<std::mutex> g(g_mu);
+  if (g_pin_refused) return 0;
   PinnedArena* pa = nullptr;
   for (auto& a : g_arenas)
     if (a.base == base && a.cap == cap) pa = &a;
@@ -388,7 +447,8 @@ int rx_pin_range(unsigned long long base, unsigned long long cap, unsigned long 
     const hipError_t rc = hipHostRegister(reinterpret_cast<void*>(s), n, hipHostRegisterDefault);
     if (rc != hipSuccess && rc != hipErrorHostMemoryAlreadyRegistered) {
       (void)hipGetLastError();
-      return (int)rc;
+      g_pin_refused = true;
+      return 0;
     }
     for (size_t k = c; k <= e; ++k) pa->run[k] = (int64_t)c;
     ++g_pin_calls;
@@ -424,7 +484,8 @@ int rx_unpin_arena(unsigned long long base) {
 
 // The whole shard: chunk k's regions are DMA'd on `copy` into the staging ring, the decode of
 // chunk k runs on `compute` after an event; ring space is reused only after the kernel that
-// read it has completed. stats: [pinned bytes, pageable bytes, copies issued, chunks].
+// read it has completed. stats: [pinned bytes, pageable bytes, copies issued, chunks,
+// bytes of the pinned ones that went through the bounce buffer].
 int rx_ingest_dma(const RxDmaChunk* chunks, int nchunks, const RxDmaRegion* regions, const RxDmaCol* cols,
                   int ncols, int out_stride, int out_bf16, void* out, void* stage, long long stage_bytes,
                   hipStream_t compute, hipStream_t copy, long long* stats) {
@@ -443,7 +504,7 @@ int rx_ingest_dma(const RxDmaChunk* chunks, int nchunks, const RxDmaRegion* regi
   };
   std::deque<Busy> busy;
   long long pos = 0;
-  long long pinned = 0, pageable = 0, ncopies = 0;
+  long long pinned = 0, pageable = 0, ncopies = 0, bounced = 0;
   for (int k = 0; k < nchunks; ++k) {
     const RxDmaChunk& ch = chunks[k];
     if (ch.bytes > stage_bytes) return -3;
@@ -468,6 +529,13 @@ int rx_ingest_dma(const RxDmaChunk* chunks, int nchunks, const RxDmaRegion* regi
       const bool pin = hipPointerGetAttributes(&at, reinterpret_cast<void*>(rg.host)) == hipSuccess &&
                        at.type == hipMemoryTypeHost;
       (void)hipGetLastError();
+      if (!pin && g_pin_refused) {
+        const int rc = rx_bounce_copy(ring + s + rg.off, (uintptr_t)rg.host, (size_t)rg.bytes, copy, &ncopies);
+        if (rc) return rc;
+        pinned += rg.bytes;
+        bounced += rg.bytes;
+        continue;
+      }
       (pin ? pinned : pageable) += rg.bytes;
       // one copy per registration run the region touches (usually exactly one)
       size_t done_b = 0;
@@ -511,11 +579,13 @@ int rx_ingest_dma(const RxDmaChunk* chunks, int nchunks, const RxDmaRegion* regi
     busy.push_back(Busy{s, e, ev_done});
     pos = e;
   }
+  if (const int rc = rx_bounce_close(copy)) return rc;
   if (stats != nullptr) {
     stats[0] += pinned;
     stats[1] += pageable;
     stats[2] += ncopies;
     stats[3] += nchunks;
+    stats[4] += bounced;
   }
   return 0;
 }

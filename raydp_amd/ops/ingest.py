@@ -7,7 +7,9 @@ GPU path (``csrc/hip/arrow_ingest.hip``, ``rx_ingest_dma``):
   and hands the list to native code: ranges that are dense in the Arrow IPC body are merged
   into one DMA per block, sparse ones go buffer by buffer;
 * ranges inside a store arena are pinned with ``hipHostRegister`` in 2 MiB chunks, lazily, once
-  per process (``rx_pin_range``), so the copies are true DMAs out of the shared mapping;
+  per process (``rx_pin_range``), so the copies are true DMAs out of the shared mapping; on a
+  system that refuses to register existing memory they go through a pinned buffer of our own
+  (two 4 MiB halves, one filling while the other is copied out);
 * ``hipMemcpyAsync`` runs on a dedicated copy stream into a ring of device staging memory;
   each chunk's decode kernel waits on an event on the compute stream, so chunk k+1's DMA
   overlaps chunk k's decode (column decode, validity -> fill value, dtype cast, transpose to the
@@ -16,7 +18,8 @@ GPU path (``csrc/hip/arrow_ingest.hip``, ``rx_ingest_dma``):
 Counters (``ingest_stats()``): ``host_copy_bytes`` (bytes the host itself copied or converted:
 casts of dictionary / timestamp / string columns, the CPU path), ``dma_pinned_bytes``,
 ``dma_pageable_bytes`` (sources outside any pinned arena: HIP stages those itself), ``dma_copies``,
-``chunks``, plus the native pinning counters.
+``chunks``, ``dma_bounced_bytes`` (those of the pinned ones that the pinned buffer carried), plus
+the native pinning counters.
 
 Reference hot site: ``python/raydp/torch/estimator.py:226-241`` (Ray Data ``to_torch`` per
 batch on the CPU).
@@ -35,7 +38,8 @@ _TYPE_CODES = {
     pa.uint8(): 6, pa.bool_(): 7, pa.uint16(): 8, pa.uint32(): 9,
 }
 
-_STAT_KEYS = ("host_copy_bytes", "dma_pinned_bytes", "dma_pageable_bytes", "dma_copies", "chunks")
+_STAT_KEYS = ("host_copy_bytes", "dma_pinned_bytes", "dma_pageable_bytes", "dma_copies", "chunks",
+              "dma_bounced_bytes")
 _stats: Dict[str, int] = {k: 0 for k in _STAT_KEYS}
 _lock = threading.Lock()
 _copy_streams: Dict[int, "torch.cuda.Stream"] = {}
@@ -214,7 +218,7 @@ def _pin(regions) -> None:
             continue
         rc = lib.rx_pin_range(u64(ar[0]), u64(ar[1]), u64(s), u64(n), u64(PIN_CHUNK))
         if rc != 0:
-            raise RuntimeError(f"hipHostRegister of the object-store arena failed (HIP error {rc})")
+            raise RuntimeError(f"pinning outside the object-store arena (error {rc})")
 
 
 def _reap_inflight():
@@ -305,13 +309,13 @@ def ingest_columns(tables: Sequence[pa.Table], cols: List[str], device, out_bf16
         stage = torch.empty(ring, dtype=torch.uint8, device=device)
         cs = _copy_stream(device)
         compute = torch.cuda.current_stream(device)
-        st = (ctypes.c_longlong * 4)()
+        st = (ctypes.c_longlong * 5)()
         rc = lib.rx_ingest_dma(chunks, len(chunk_l), regs, dcols, len(cols), stride, 2 if out_i64 else int(out_bf16),
                                ctypes.c_void_p(out.data_ptr()), ctypes.c_void_p(stage.data_ptr()), ring,
                                ctypes.c_void_p(compute.cuda_stream), ctypes.c_void_p(cs.cuda_stream), st)
         _hip.check(rc, "rx_ingest_dma")
         stage.record_stream(cs)
-        for key, v in zip(("dma_pinned_bytes", "dma_pageable_bytes", "dma_copies", "chunks"), st):
+        for key, v in zip(("dma_pinned_bytes", "dma_pageable_bytes", "dma_copies", "chunks", "dma_bounced_bytes"), st):
             _stats[key] += int(v)
         ev = torch.cuda.Event()
         ev.record(compute)
