@@ -21,6 +21,9 @@ ROOT = os.path.abspath(os.path.join(HERE, "..", ".."))
 CSRC = os.path.join(ROOT, "csrc")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 ARCH = os.environ.get("RAYDP_GPU_ARCH", "gfx950")
+# no packed fp32 instructions (v_pk_add/mul/fma_f32): the compiler makes them from ordinary float
+# code, and some of their forms give wrong results now and then
+HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hip_sources():
@@ -87,7 +90,7 @@ def _newer(out, srcs):
     if not os.path.exists(out):
         return False
     t = os.path.getmtime(out)
-    deps = list(srcs)
+    deps = list(srcs) + [os.path.abspath(__file__)]     # (flags are set here)
     for d in ("common", "hip", "runtime", "exec", "exec/expr", "comm", "control"):
         p = os.path.join(CSRC, d)
         if os.path.isdir(p):
@@ -124,8 +127,8 @@ def build_one(name: str, force: bool = False) -> str:
         jobs = max(1, min(len(todo), int(os.environ.get("MAX_JOBS", os.cpu_count() or 4)), 16))
         def compile_one(so):
             src, obj = so
-            _run([hipcc, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
-                  "-c", src, "-o", obj + ".tmp"] + inc)
+            _run([hipcc, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics"] + HIP_FLAGS +
+                 ["-c", src, "-o", obj + ".tmp"] + inc)
             os.replace(obj + ".tmp", obj)
 
         with ThreadPoolExecutor(jobs) as ex:

@@ -20,6 +20,7 @@ import subprocess
 import threading
 from typing import Optional
 
+from raydp_amd.native.build import HIP_FLAGS
 from raydp_amd.ops import _hip
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -157,6 +158,7 @@ def _key(src: str) -> str:
             with open(os.path.join(CSRC_HIP, f), "rb") as fh:
                 h.update(fh.read())
         h.update(ARCH.encode())
+        h.update(" ".join(HIP_FLAGS).encode())
         _headers_digest = h.digest()
     h = hashlib.sha256(src.encode())
     h.update(_headers_digest)
@@ -179,8 +181,8 @@ def compile_source(src: str) -> str:
         f.write(src)
     os.replace(cpp + f".{threading.get_ident()}", cpp)
     tmp = path + f".tmp{os.getpid()}.{threading.get_ident()}"   # (precompile_many: same source twice)
-    cmd = [_hipcc(), "--genco", f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-munsafe-fp-atomics",
-           "-I", CSRC_HIP, cpp, "-o", tmp]
+    cmd = [_hipcc(), "--genco", f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-munsafe-fp-atomics"] + HIP_FLAGS + \
+        ["-I", CSRC_HIP, cpp, "-o", tmp]
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"specialised kernel build failed:\n{' '.join(cmd)}\n{r.stdout[-4000:]}")
