@@ -1,0 +1,571 @@
+"""AdamW over many tensors with the moments in 8 or 32 bits, and clipping by the global gradient norm
+(``csrc/hip/adamw.hip``; public names in :mod:`raydp_amd.ops.fused_optim`).
+
+* :class:`FusedAdamW` -- ``torch.optim.AdamW``'s update (decoupled weight decay) as one launch per 48 tensors.
+  Parameters are contiguous fp32 or bf16. ``state_bits=8`` keeps each moment in one byte plus two scale bytes per 256
+  elements (2.01 bytes per parameter where fp32 moments take 8); ``state_bits=32`` keeps them in fp32. fp32 weights
+  that a fused Linear tower reads get their bf16 image in the same pass; bf16 parameters have no master copy and are
+  rounded stochastically. Step counts live on the device, so a step can be captured into a HIP graph once an eager step
+  has made the state.
+* :func:`clip_grad_norm_` -- ``torch.nn.utils.clip_grad_norm_`` (2-norm) in two launches per 128 tensors, without a host
+  read. ``FusedAdamW(max_grad_norm=...)`` applies the same factor inside the step instead, without the pass that
+  rewrites the gradients.
+* :func:`decode_moments` -- the values that 8-bit moments stand for.
+
+On the CPU the same operators are computed by torch expressions with the same codes.
+"""
+import contextlib
+import ctypes
+import math
+from typing import Iterable, Optional, Tuple, Union
+
+import torch
+
+from raydp_amd.ops import _hip
+
+BLOCK = 256                  # elements of a tensor that share a scale
+AW_MAX, PREP_MAX, NORM_MAX = 48, 256, 128
+STEP_CHUNK, NORM_CHUNK = 1024, 4096
+NORM_GRID = 1024             # partial sums of one norm launch at most
+_M_EMIN, _V_EMIN = -14, -30
+_MASK, _PHI, _SQ2, _SQ3 = 0xFFFFFFFF, 0x9E3779B1, 0x6A09E667, 0xBB67AE85
+
+
+class AwPrep(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int), ("maximize", ctypes.c_int), ("npart", ctypes.c_int), ("first", ctypes.c_int),
+                ("lr", ctypes.c_double), ("wd", ctypes.c_double), ("b1", ctypes.c_double), ("b2", ctypes.c_double),
+                ("max_norm", ctypes.c_double), ("lr_dev", ctypes.c_void_p), ("part", ctypes.c_void_p),
+                ("head", ctypes.c_void_p), ("tensors", ctypes.c_void_p), ("norm", ctypes.c_void_p),
+                ("seed", ctypes.c_uint32), ("pad_", ctypes.c_uint32), ("step", ctypes.c_void_p * PREP_MAX),
+                ("ordinal", ctypes.c_int * PREP_MAX)]
+
+
+class AwStep(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int), ("pad_", ctypes.c_int), ("b1", ctypes.c_float), ("omb1", ctypes.c_float),
+                ("b2", ctypes.c_float), ("omb2", ctypes.c_float), ("eps", ctypes.c_float), ("pad2_", ctypes.c_float),
+                ("head", ctypes.c_void_p), ("tensors", ctypes.c_void_p), ("p", ctypes.c_void_p * AW_MAX),
+                ("g", ctypes.c_void_p * AW_MAX), ("m", ctypes.c_void_p * AW_MAX), ("v", ctypes.c_void_p * AW_MAX),
+                ("sc", ctypes.c_void_p * AW_MAX), ("img", ctypes.c_void_p * AW_MAX),
+                ("len", ctypes.c_longlong * AW_MAX), ("start", ctypes.c_uint * (AW_MAX + 1))]
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int), ("pad0_", ctypes.c_int), ("part", ctypes.c_void_p), ("chunks", ctypes.c_uint),
+                ("pad_", ctypes.c_uint), ("g", ctypes.c_void_p * NORM_MAX), ("len", ctypes.c_longlong * NORM_MAX),
+                ("start", ctypes.c_uint * (NORM_MAX + 1)), ("bf16", ctypes.c_ubyte * NORM_MAX)]
+
+
+class ScaleArgs(ctypes.Structure):
+    _fields_ = [("t", NormArgs), ("npart", ctypes.c_int), ("pad_", ctypes.c_int), ("max_norm", ctypes.c_double),
+                ("norm", ctypes.c_void_p)]
+
+
+_bound = None
+
+
+def _lib():
+    global _bound
+    L = _hip.lib()
+    if _bound is not L:
+        vp, i, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+        L.rx_aw_prep.argtypes = [vp, vp]
+        L.rx_aw_step.argtypes = [vp, i, i, vp]
+        L.rx_norm_part.argtypes = [vp, i, vp]
+        L.rx_norm_scale.argtypes = [vp, i, vp]
+        L.rx_aw_decode.argtypes = [vp, vp, vp, vp, vp, ll, i, vp]
+        for n in ("rx_aw_prep", "rx_aw_step", "rx_norm_part", "rx_norm_scale", "rx_aw_decode"):
+            getattr(L, n).restype = i
+        L.rx_aw_sizes.argtypes = [vp]
+        L.rx_aw_sizes.restype = None
+        got = (ctypes.c_int * 9)()
+        L.rx_aw_sizes(got)
+        want = [ctypes.sizeof(c) for c in (AwPrep, AwStep, NormArgs, ScaleArgs)] + \
+            [AW_MAX, PREP_MAX, NORM_MAX, STEP_CHUNK, NORM_CHUNK]
+        if list(got) != want:
+            raise RuntimeError(f"layout mismatch between Python and csrc/hip/adamw.hip: C {list(got)} vs {want}")
+        _bound = L
+    return L
+
+
+def _on(device):
+    """The device whose stream a launch goes to, made current where it is not."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Every element once, without gaps, in whatever order."""
+    if t.is_contiguous():
+        return True
+    need = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda v: v[1]):
+        if stride != need:
+            return False
+        need *= size
+    return True
+
+
+# --------------------------------------------------------------------------------------- moments in 8 bits
+def _mix(x):
+    x = ((x ^ (x >> 16)) * _SQ2) & _MASK
+    x = ((x ^ (x >> 15)) * _SQ3) & _MASK
+    return x ^ (x >> 16)
+
+
+def _dither(n: int, seed: int, ordinal: int, step: int, device):
+    """32 random bits for each of ``n`` elements, as csrc/hip/adamw.hip makes them (in int64)."""
+    key = _mix((_mix((seed + ordinal * _PHI) & _MASK) + step) & _MASK)
+    i = torch.arange(n, device=device)
+    return _mix(((i & _MASK) * _PHI + (i >> 32) * _SQ2 + key) & _MASK)
+
+
+def _pow2(e):
+    return ((e + 1023) << 52).view(torch.float64)
+
+
+def _blocks(x):
+    """[blocks, 256] of a flat tensor, the last block filled up with zeros."""
+    return torch.nn.functional.pad(x, (0, -x.numel() % BLOCK)).view(-1, BLOCK)
+
+
+def _encode(x, rnd16, emin):
+    """(codes, biased scale exponents) of blocks of non-negative fp32 values: 3 mantissa bits, normal from 2^emin."""
+    s = (x.view(torch.int32).long().amax(1) + 0xFFFFF) >> 23
+    y = x.double() * _pow2(127 - s.clamp(min=1))[:, None]
+    f = ((y.view(torch.int64) >> 52) - 1023).clamp(min=emin)
+    code = ((torch.round(y * _pow2(3 - f) * 2.0 ** 20).long() + rnd16 * 16 + 8) >> 20) + 8 * (f - emin)
+    return torch.where((s == 255)[:, None], 0, code), s
+
+
+def _decode(code, s, emin):
+    e, man = code >> 3, code & 7
+    y = torch.where(e > 0, (8 + man).double() * _pow2(e.clamp(min=1) - 1 + emin - 3), man.double() * 2.0 ** (emin - 3))
+    return (y * torch.where(s == 255, math.nan, _pow2(s.clamp(min=1) - 127))[:, None]).float()
+
+
+def _encode_moments(m, v, h):
+    """(exp_avg, exp_avg_sq, scales) in 8 bits from fp32 moments and 32 dither bits per element."""
+    h = _blocks(h)
+    mb, vb = _blocks(m.reshape(-1)), _blocks(v.reshape(-1))
+    mc, ms = _encode(mb.abs(), h & 0xFFFF, _M_EMIN)
+    mc = mc | ((mb.view(torch.int32) < 0) & (ms != 255)[:, None]).long() * 128
+    vc, vs = _encode(vb, h >> 16, _V_EMIN)
+    vc = torch.where((vb > 0) & (vs != 255)[:, None], vc.clamp(min=1), vc)    # it is divided by
+    n, scales = m.numel(), torch.stack([ms, vs], 1).to(torch.uint8)
+    return (mc.to(torch.uint8).view(-1)[:n].view(m.shape), vc.to(torch.uint8).view(-1)[:n].view(v.shape), scales)
+
+
+def _scale_rows(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def decode_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, scales: torch.Tensor,
+                   dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The values of one parameter's 8-bit moments (``state[p]["exp_avg"]``, ``["exp_avg_sq"]``, ``["scales"]``) in
+    ``dtype`` (fp32 or bf16: a code has 4 significant bits, so both hold it exactly). A block that held a value which
+    was not finite decodes to NaN."""
+    n = exp_avg.numel()
+    for t, name in ((exp_avg, "exp_avg"), (exp_avg_sq, "exp_avg_sq"), (scales, "scales")):
+        if t.dtype != torch.uint8 or not t.is_contiguous():
+            raise ValueError(f"decode_moments: {name} must be contiguous uint8 (8-bit moments)")
+        if t.device != exp_avg.device:
+            raise ValueError("decode_moments: moments and scales are on different devices")
+    if exp_avg_sq.shape != exp_avg.shape or scales.numel() != 2 * _scale_rows(n):
+        raise ValueError(f"decode_moments: {n} elements need moments of one shape and {2 * _scale_rows(n)} scale bytes, "
+                         f"got {tuple(exp_avg_sq.shape)} and {scales.numel()}")
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"decode_moments: dtype {dtype} (fp32 or bf16)")
+    if not exp_avg.is_cuda:
+        mc, vc, s = (t.long() for t in (_blocks(exp_avg.view(-1)), _blocks(exp_avg_sq.view(-1)), scales.view(-1, 2)))
+        m = _decode(mc & 127, s[:, 0], _M_EMIN) * (1 - (mc >> 7) * 2)
+        v = _decode(vc, s[:, 1], _V_EMIN)
+        return tuple(t.view(-1)[:n].view(exp_avg.shape).to(dtype) for t in (m, v))
+    if (exp_avg.data_ptr() | exp_avg_sq.data_ptr()) & 3:
+        raise ValueError("decode_moments: moments must start at a multiple of 4 bytes")
+    m, v = torch.empty_like(exp_avg, dtype=dtype), torch.empty_like(exp_avg_sq, dtype=dtype)
+    if n:
+        with _on(m.device):
+            _hip.check(_lib().rx_aw_decode(exp_avg.data_ptr(), exp_avg_sq.data_ptr(), scales.data_ptr(), m.data_ptr(),
+                                           v.data_ptr(), n, int(dtype == torch.bfloat16), _hip.stream_ptr(m.device)),
+                       "rx_aw_decode")
+    return m, v
+
+
+# --------------------------------------------------------------------------------------- norm and clipping
+def _norm_launches(grads):
+    """[(NormArgs, grid)] over ``grads`` (dense fp32 / bf16 tensors), ``part`` still to be filled in."""
+    out = []
+    for k in range(0, len(grads), NORM_MAX):
+        chunk = grads[k:k + NORM_MAX]
+        a, n = NormArgs(), len(chunk)
+        lens = [g.numel() for g in chunk]
+        starts = [0]
+        for ln in lens:
+            starts.append(starts[-1] + -(-ln // NORM_CHUNK))
+        if starts[-1] > _MASK:
+            raise ValueError("gradient norm: too many elements for one launch")
+        a.n, a.chunks = n, starts[-1]
+        a.g[:n] = [g.data_ptr() for g in chunk]
+        a.len[:n], a.start[:n + 1] = lens, starts
+        a.bf16[:n] = [g.dtype == torch.bfloat16 for g in chunk]
+        out.append((a, min(starts[-1], NORM_GRID)))
+    return out
+
+
+def _launch_norm(L, launches, part_ptr, stream):
+    """Partial sums of squares to ``part_ptr`` on; returns how many."""
+    at = 0
+    for a, grid in launches:
+        a.part = part_ptr + 8 * at
+        _hip.check(L.rx_norm_part(ctypes.byref(a), grid, stream), "rx_norm_part")
+        at += grid
+    return at
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float) -> torch.Tensor:
+    """Scale the gradients of ``parameters`` in place by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` their global
+    2-norm (summed in 64 bits), and return the norm (0-dim fp32, on the gradients' device, without a host
+    synchronisation). Gradients are dense (in any dimension order) fp32 or bf16; a parameter that is listed twice
+    counts once. A norm that is not finite is not kept from the gradients (a NaN makes all of them NaN, an infinity 0 and
+    NaN), as in ``torch.nn.utils.clip_grad_norm_``."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm}")
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    seen, grads = set(), []
+    for p in parameters:
+        if p.grad is not None and id(p) not in seen:
+            seen.add(id(p))
+            grads.append(p.grad)
+    if not grads:
+        return torch.zeros(())
+    dev = grads[0].device
+    for g in grads:
+        if g.layout != torch.strided:
+            raise ValueError("clip_grad_norm_: sparse gradients are not supported")
+        if g.device != dev:
+            raise ValueError(f"clip_grad_norm_: gradients on {dev} and {g.device}")
+        if g.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"clip_grad_norm_: gradient dtype {g.dtype} (fp32 or bf16)")
+        if not _dense(g):
+            raise ValueError("clip_grad_norm_: gradients must be dense (no gaps, no broadcast dimensions)")
+    if dev.type != "cuda":
+        norm = torch.sqrt(sum(g.double().square().sum() for g in grads))
+        f = (max_norm / (norm + 1e-6)).clamp(max=1.0).float()
+        for g in grads:
+            g.copy_(g.float() * f)
+        return norm.float()
+    grads = [g for g in grads if g.numel()]
+    if not grads:
+        return torch.zeros((), device=dev)
+    L = _lib()
+    with _on(dev):
+        stream = _hip.stream_ptr(dev)
+        launches = _norm_launches(grads)
+        part = torch.empty(sum(grid for _, grid in launches), dtype=torch.float64, device=dev)
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        npart = _launch_norm(L, launches, part.data_ptr(), stream)
+        for k, (a, grid) in enumerate(launches):
+            s = ScaleArgs()
+            s.t, s.npart, s.max_norm = a, npart, max_norm
+            s.t.part, s.norm = part.data_ptr(), norm.data_ptr() if k == 0 else None
+            _hip.check(L.rx_norm_scale(ctypes.byref(s), min(a.chunks, 8192), stream), "rx_norm_scale")
+    torch.autograd.graph.increment_version(grads)
+    return norm
+
+
+# --------------------------------------------------------------------------------------- the optimizer
+class FusedAdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` on the multi-tensor kernels, with the moments in 8 or 32 bits.
+
+    ``state_bits``      8: one byte per moment and two scale bytes per 256 elements, rounded stochastically (the hash of
+                        ``seed``, the parameter's place, the step and the element's index: the same run gives the same
+                        bits); 32: fp32.
+    ``max_grad_norm``   clip by the global 2-norm of all gradients inside the step (``.grad`` is left as it is; the norm
+                        is ``self.grad_norm``, on the device). A step whose norm is not finite is left out: parameters,
+                        moments and step counts stay as they are. None: no clipping, nothing is left out.
+    ``lr``              a number, or a 0-dim fp32 tensor on the parameters' device (read by the kernel: a captured step
+                        sees what a scheduler fills in).
+
+    State per parameter: ``step`` (0-dim fp32 on the parameter's device), ``exp_avg``, ``exp_avg_sq`` (uint8 codes or
+    fp32) and, for 8 bits, ``scales`` (uint8 ``[ceil(n / 256), 2]``); :func:`decode_moments` gives their values.
+    ``load_state_dict`` also takes the state of a ``torch.optim.AdamW`` and codes its moments.
+
+    Parameters are contiguous fp32 or bf16; gradients are dense and of the parameter's type. Sparse gradients, closures
+    inside a graph capture and a first step inside a capture raise."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 state_bits: int = 8, max_grad_norm: Optional[float] = None, maximize: bool = False, seed: int = 0):
+        if isinstance(lr, torch.Tensor):
+            if lr.numel() != 1:
+                raise ValueError("FusedAdamW: a tensor lr must have one element")
+        elif not 0.0 <= lr:
+            raise ValueError(f"FusedAdamW: invalid learning rate {lr}")
+        if not eps >= 0.0:
+            raise ValueError(f"FusedAdamW: invalid eps {eps}")
+        if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"FusedAdamW: invalid betas {betas}")
+        if not weight_decay >= 0.0:
+            raise ValueError(f"FusedAdamW: invalid weight_decay {weight_decay}")
+        if state_bits not in (8, 32):
+            raise ValueError(f"FusedAdamW: state_bits is 8 or 32, got {state_bits}")
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError(f"FusedAdamW: invalid max_grad_norm {max_grad_norm}")
+        if not 0 <= int(seed) <= _MASK:
+            raise ValueError(f"FusedAdamW: seed must fit 32 bits, got {seed}")
+        super().__init__(params, dict(lr=lr, betas=tuple(float(b) for b in betas), eps=float(eps),
+                                      weight_decay=float(weight_decay), state_bits=int(state_bits),
+                                      max_grad_norm=None if max_grad_norm is None else float(max_grad_norm),
+                                      maximize=bool(maximize), seed=int(seed)))
+        self.grad_norm: Optional[torch.Tensor] = None
+        self._ws = None
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._fill_groups()
+        self.__dict__.setdefault("grad_norm", None)
+        self.__dict__["_ws"] = None
+
+    def _fill_groups(self):
+        for g in self.param_groups:      # (a state dict of torch.optim.AdamW has fewer options)
+            for k, v in self.defaults.items():
+                g.setdefault(k, v)
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        params = self.param_groups[-1]["params"]
+        for p in params:
+            if p.dtype not in (torch.float32, torch.bfloat16):
+                self.param_groups.pop()
+                raise TypeError(f"FusedAdamW: parameter dtype {p.dtype} (fp32 or bf16)")
+        if len({id(p) for p in params}) < len(params):
+            self.param_groups.pop()
+            raise ValueError("FusedAdamW: a parameter is listed twice")
+
+    def load_state_dict(self, state_dict):
+        saved = state_dict["state"]
+        super().load_state_dict(state_dict)
+        self._fill_groups()
+        # torch casts floating state to the parameter's type and codes with it: put the saved bits back
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [(g, p) for g in self.param_groups for p in g["params"]]
+        for k, (i, (g, p)) in enumerate(zip(ids, params)):
+            src = saved.get(i)
+            if not src:
+                continue
+            if any(n not in src for n in ("step", "exp_avg", "exp_avg_sq")):
+                raise ValueError(f"FusedAdamW: state of parameter {k} lacks step, exp_avg or exp_avg_sq")
+            step = src["step"]
+            st = {"step": torch.as_tensor(step, dtype=torch.float32).detach().clone().to(p.device)}
+            m, v = (src[n].detach().to(p.device) for n in ("exp_avg", "exp_avg_sq"))
+            if m.shape != p.shape or v.shape != p.shape:
+                raise ValueError(f"FusedAdamW: moments of parameter {k} are {tuple(m.shape)}, the parameter is {tuple(p.shape)}")
+            coded = m.dtype == torch.uint8
+            if coded:
+                sc = src["scales"].detach().to(p.device, copy=True).contiguous()
+                if v.dtype != torch.uint8 or sc.dtype != torch.uint8 or sc.numel() != 2 * _scale_rows(p.numel()):
+                    raise ValueError(f"FusedAdamW: 8-bit state of parameter {k} is incomplete")
+            m, v = (t.clone(memory_format=torch.contiguous_format) for t in (m, v))
+            if g["state_bits"] == 8:
+                if not coded:
+                    half = torch.full((p.numel(),), (1 << 31) | (1 << 15), dtype=torch.int64, device=p.device)
+                    m, v, sc = _encode_moments(m.float(), v.float(), half)
+                st.update(exp_avg=m, exp_avg_sq=v, scales=sc)
+            else:
+                m, v = decode_moments(m, v, sc) if coded else (m.float(), v.float())
+                st.update(exp_avg=m, exp_avg_sq=v)
+            self.state[p] = st
+
+    def _state_of(self, p, bits):
+        """The parameter's state, made with its first gradient."""
+        st = self.state[p]
+        if not st:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("FusedAdamW: the first step of a parameter cannot be captured into a graph (its state "
+                                   "would be zeroed by every replay): run one eager step first")
+            st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+            kind = torch.uint8 if bits == 8 else torch.float32
+            for n in ("exp_avg", "exp_avg_sq"):
+                st[n] = torch.zeros(p.shape, dtype=kind, device=p.device)
+            if bits == 8:
+                st["scales"] = torch.zeros(_scale_rows(p.numel()), 2, dtype=torch.uint8, device=p.device)
+            return st
+        if st["step"].device != p.device:      # (state loaded before the model was moved)
+            for n, t in st.items():
+                st[n] = t.to(p.device)
+        if (st["exp_avg"].dtype == torch.uint8) != (bits == 8):
+            raise ValueError(f"FusedAdamW: state_bits is {bits}, the moments of a parameter are {st['exp_avg'].dtype}")
+        return st
+
+    def _live(self):
+        """[(group, [(parameter, gradient, place)])] with gradients, checked."""
+        out, place, dev = [], 0, None
+        for group in self.param_groups:
+            live = []
+            for p in group["params"]:
+                g = p.grad
+                if g is not None:
+                    if g.layout != torch.strided:
+                        raise RuntimeError("FusedAdamW does not support sparse gradients")
+                    if dev is None:
+                        dev = p.device
+                    if p.device != dev:
+                        raise ValueError(f"FusedAdamW: parameters with gradients on {dev} and {p.device}")
+                    if p.dtype not in (torch.float32, torch.bfloat16) or g.dtype != p.dtype:
+                        raise TypeError(f"FusedAdamW: parameter {p.dtype} with gradient {g.dtype} (both fp32 or both bf16)")
+                    if not p.is_contiguous():
+                        raise ValueError("FusedAdamW: parameters must be contiguous")
+                    if p.numel():
+                        live.append((p, g if g.is_contiguous() else g.contiguous(), place))
+                place += 1
+            if live:
+                out.append((group, live))
+        if out and any(g["max_grad_norm"] != out[0][0]["max_grad_norm"] or g["seed"] != out[0][0]["seed"] for g, _ in out):
+            raise ValueError("FusedAdamW: max_grad_norm and seed are the optimizer's, not a group's")
+        return out, dev
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        groups, dev = self._live()
+        if groups:
+            if dev.type == "cuda":
+                with _on(dev):
+                    self._gpu_step(groups, dev)
+            else:
+                self._cpu_step(groups)
+        return loss
+
+    # ------------------------------------------------------------------ GPU
+    def _workspace(self, dev, ngroups, ntensors, npart):
+        """Device scratch of this optimizer's steps: heads, per-tensor constants, partial sums."""
+        ws = self._ws
+        if ws is None or ws["dev"] != dev or ws["groups"] < ngroups or ws["tensors"] < ntensors or ws["part"] < npart:
+            ws = dict(dev=dev, groups=ngroups, tensors=ntensors, part=npart)
+            ws["buf"] = torch.empty(16 * ntensors + 8 * ngroups + 8 * npart, dtype=torch.uint8, device=dev)
+            at = ws["buf"].data_ptr()
+            ws["tensors_at"], ws["heads_at"], ws["part_at"] = at, at + 16 * ntensors, at + 16 * ntensors + 8 * ngroups
+            self._ws = ws
+        return ws
+
+    def _gpu_step(self, groups, dev):
+        from raydp_amd.ops.fused_optim import _image_of
+        L, stream = _lib(), _hip.stream_ptr(dev)
+        clip = groups[0][0]["max_grad_norm"]
+        # fp32 parameters first (stable): a launch takes one type
+        groups = [(group, sorted(live, key=lambda e: e[0].dtype == torch.bfloat16)) for group, live in groups]
+        all_states = [[self._state_of(p, group["state_bits"]) for p, _, _ in live] for group, live in groups]
+        launches = _norm_launches([g for _, live in groups for _, g, _ in live]) if clip is not None else []
+        ws = self._workspace(dev, len(groups), sum(len(live) for _, live in groups), sum(grid for _, grid in launches))
+        npart = _launch_norm(L, launches, ws["part_at"], stream) if launches else 0
+        if clip is not None:
+            self.grad_norm = torch.empty((), dtype=torch.float32, device=dev)
+        done, owners, first = [], [], 0
+        for k, (group, live) in enumerate(groups):
+            bits, lr = group["state_bits"], group["lr"]
+            lr_dev = None
+            if isinstance(lr, torch.Tensor):
+                if lr.is_cuda:
+                    if lr.device != dev or lr.dtype != torch.float32:
+                        raise TypeError("FusedAdamW: a tensor lr must be fp32 on the parameters' device")
+                    lr_dev, lr = lr.data_ptr(), 0.0
+                else:
+                    lr = float(lr)
+            states = all_states[k]
+            head = ws["heads_at"] + 8 * k
+            for j in range(0, len(live), PREP_MAX):
+                part = live[j:j + PREP_MAX]
+                a = AwPrep()
+                n = a.n = len(part)
+                a.maximize, a.first, a.lr, a.lr_dev, a.wd = int(group["maximize"]), first + j, lr, lr_dev, group["weight_decay"]
+                a.b1, a.b2 = group["betas"]
+                a.max_norm, a.npart, a.part = -1.0 if clip is None else clip, npart, ws["part_at"]
+                a.head, a.tensors, a.seed = head, ws["tensors_at"], group["seed"]
+                a.norm = self.grad_norm.data_ptr() if clip is not None and first + j == 0 else None
+                a.step[:n] = [st["step"].data_ptr() for st in states[j:j + n]]
+                a.ordinal[:n] = [o for _, _, o in part]
+                _hip.check(L.rx_aw_prep(ctypes.byref(a), stream), "rx_aw_prep")
+            b1, b2 = group["betas"]
+            at = 0
+            while at < len(live):
+                low = live[at][0].dtype == torch.bfloat16
+                end = at
+                while end < len(live) and end - at < AW_MAX and (live[end][0].dtype == torch.bfloat16) == low:
+                    end += 1
+                part, sts = live[at:end], states[at:end]
+                a = AwStep()
+                n = a.n = end - at
+                a.b1, a.omb1, a.b2, a.omb2, a.eps = b1, 1.0 - b1, b2, 1.0 - b2, group["eps"]
+                a.head, a.tensors = head, ws["tensors_at"] + 16 * (first + at)
+                a.p[:n] = [p.data_ptr() for p, _, _ in part]
+                a.g[:n] = [g.data_ptr() for _, g, _ in part]
+                a.m[:n] = [st["exp_avg"].data_ptr() for st in sts]
+                a.v[:n] = [st["exp_avg_sq"].data_ptr() for st in sts]
+                lens = [p.numel() for p, _, _ in part]
+                a.len[:n] = lens
+                starts = [0]
+                for ln in lens:
+                    starts.append(starts[-1] + -(-ln // STEP_CHUNK))
+                if starts[-1] > 0x7FFFFFFF:
+                    raise ValueError("FusedAdamW: too many elements for one launch")
+                a.start[:n + 1] = starts
+                if bits == 8:
+                    a.sc[:n] = [st["scales"].data_ptr() for st in sts]
+                if any((x | y) & (3 if bits == 8 else 15) for x, y in zip(a.m[:n], a.v[:n])):
+                    raise ValueError("FusedAdamW: moments must start at a multiple of 4 (8 bits) or 16 bytes")
+                if not low:
+                    for j, (p, _, _) in enumerate(part):
+                        tower, li, img = _image_of(p)
+                        if img is not None:
+                            a.img[j] = img.data_ptr()
+                            owners.append((tower, li))
+                _hip.check(L.rx_aw_step(ctypes.byref(a), bits, int(low), stream), "rx_aw_step")
+                done += [p for p, _, _ in part]
+                at = end
+            first += len(live)
+        torch.autograd.graph.increment_version(done)
+        for tower, li in owners:
+            tower.image_updated(li)
+
+    # ------------------------------------------------------------------ CPU
+    def _cpu_step(self, groups):
+        clip, scale = groups[0][0]["max_grad_norm"], 1.0
+        if clip is not None:
+            norm = torch.sqrt(sum(g.double().square().sum() for _, live in groups for _, g, _ in live))
+            self.grad_norm = norm.float()
+            if not bool(torch.isfinite(norm)):
+                return
+            scale = (clip / (norm + 1e-6)).clamp(max=1.0).float()
+        for group, live in groups:
+            b1, b2 = group["betas"]
+            bits, lr = group["state_bits"], float(group["lr"])
+            for p, g, place in live:
+                st = self._state_of(p, bits)
+                st["step"] += 1
+                t = int(st["step"])
+                g = g.float() * (-scale if group["maximize"] else scale)
+                m, v = (st["exp_avg"], st["exp_avg_sq"]) if bits == 32 else \
+                    decode_moments(st["exp_avg"], st["exp_avg_sq"], st["scales"])
+                m = m * b1 + g * (1 - b1)
+                v = v * b2 + (g * g) * (1 - b2)
+                den = torch.sqrt(v) * (1.0 / math.sqrt(1.0 - b2 ** t)) + group["eps"]
+                new = p.float() * (1.0 - lr * group["weight_decay"]) + m / den * (-lr / (1.0 - b1 ** t))
+                low = p.dtype == torch.bfloat16
+                h = _dither(p.numel(), group["seed"], place, t, p.device) if bits == 8 or low else None
+                if bits == 8:
+                    codes = _encode_moments(m, v, h)
+                    for n, c in zip(("exp_avg", "exp_avg_sq", "scales"), codes):
+                        st[n].copy_(c)
+                else:
+                    st["exp_avg"].copy_(m)
+                    st["exp_avg_sq"].copy_(v)
+                if low:
+                    b = new.view(torch.int32).long() & _MASK
+                    r = (((h * _SQ2) & _MASK) >> 16).view(p.shape)
+                    b = torch.where(torch.isnan(new), b, b + r) >> 16 << 16
+                    new = torch.where(b > 0x7FFFFFFF, b - (1 << 32), b).int().view(torch.float32)
+                p.copy_(new)

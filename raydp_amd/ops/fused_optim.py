@@ -12,6 +12,8 @@
 * :class:`FusedBCEWithLogits` -- ``nn.BCEWithLogitsLoss()`` (mean reduction, no weights): the
   loss is one single-workgroup kernel and its gradient one elementwise kernel computed from the
   saved operands (eager torch: log-sigmoid, mean, sigmoid, sub, mul ... ~6 launches).
+* :class:`FusedAdamW`, :func:`clip_grad_norm_`, :func:`decode_moments` -- AdamW with the moments in 8 or
+  32 bits, and clipping by the global gradient norm (``raydp_amd/ops/adamw.py``, ``csrc/hip/adamw.hip``).
 
 Reference: the DLRM notebook's ``torch.optim.SGD`` + ``nn.BCEWithLogitsLoss``
 (``examples/pytorch_dlrm.ipynb`` cells 9, 14) on the estimator's loop
@@ -290,3 +292,6 @@ def fusable_bce(loss) -> bool:
     """An ``nn.BCEWithLogitsLoss`` with the defaults (mean, no weight / pos_weight)."""
     return (type(loss) is nn.BCEWithLogitsLoss and loss.reduction == "mean" and loss.weight is None
             and loss.pos_weight is None)
+
+
+from raydp_amd.ops.adamw import FusedAdamW, clip_grad_norm_, decode_moments  # noqa: E402,F401 - public names of this module

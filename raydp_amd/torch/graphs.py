@@ -13,9 +13,9 @@ batches with one launch plus one window copy.
 Rules that keep it exact:
 * the first two steps of the first epoch run eagerly on a side stream (lazy optimizer state,
   library workspaces), as graph capture requires;
-* Adam/AdamW switch to ``capturable=True`` (device-side step counters); with an LR scheduler
-  the learning rate becomes a device tensor that the scheduler ``fill_``s, and chunk = 1 so every
-  step sees its own LR;
+* Adam/AdamW switch to ``capturable=True`` (device-side step counters; ``FusedAdamW`` always keeps
+  them there); with an LR scheduler the learning rate becomes a device tensor that the scheduler
+  ``fill_``s, and chunk = 1 so every step sees its own LR;
 * metric state is zeroed in place between epochs (``TorchMetric.zero_``) so the captured
   accumulation keeps pointing at live storage;
 * list indices in user models (``x[:, [1, 7, 8]]`` as in the reference tutorial's NET_Model) are
@@ -34,8 +34,9 @@ from typing import Optional
 import torch
 from torch.overrides import TorchFunctionMode
 
+from raydp_amd.ops.fused_optim import FusedAdamW
 
-_ADAM_LIKE = (torch.optim.Adam, torch.optim.AdamW)
+_ADAM_LIKE = (torch.optim.Adam, torch.optim.AdamW, FusedAdamW)
 _SAFE_OPT = _ADAM_LIKE + (torch.optim.SGD,)
 
 
@@ -105,7 +106,8 @@ class GraphedTrainLoop:
         opt, dev = self.e.optimizer, self.e.device
         if isinstance(opt, _ADAM_LIKE):
             for g in opt.param_groups:
-                g["capturable"] = True   # (the fused kernel ignores it but step() checks it)
+                if not isinstance(opt, FusedAdamW):
+                    g["capturable"] = True   # (the fused kernel ignores it but step() checks it)
                 if self.e.scheduler is not None and not isinstance(g["lr"], torch.Tensor):
                     g["lr"] = torch.tensor(float(g["lr"]), dtype=torch.float32, device=dev)
             for st in opt.state.values():
