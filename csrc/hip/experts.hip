@@ -67,79 +67,160 @@ struct Vec {
 };
 
 // ------------------------------------------------------------------------------------------------ router
+// L lanes hold a row, V consecutive logits each, as keys that order as (logit, lowest index first) do and differ within a
+// row. The next of the k largest keys is then one max per key and no bookkeeping of what was taken:
+//   16-bit logits: (order-preserving 16 bits, 0xFFFF - index) in 32 bits. key - last wraps for every key below the last
+//                  winner and so puts those above the ones taken: max over (key - last), two keys per v_max3.
+//   fp32 logits:   (order-preserving 32 bits, 0xFFFF - index) as a positive double: v_max_f64 runs at the rate of fp32, two
+//                  words a key; a winner is struck out by its low word.
 constexpr int kRouteMaxK = 32;
 
-// L lanes hold a row, V logits each: element i * L + lane
+// order-preserving unsigned images of the logits' bits (not of NaN and -0: the callers replace them)
+__device__ __forceinline__ uint32_t order16(uint32_t b) { return (b & 0x8000u) ? b ^ 0xFFFFu : b | 0x8000u; }
+__device__ __forceinline__ uint32_t order32(uint32_t b) { return (b & 0x80000000u) ? ~b : b | 0x80000000u; }
+
+// LDS written by lanes of a wave is read by its other lanes after this
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// lane ^ d within groups of L lanes
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v, int d) { return (uint32_t)__shfl_xor((int)v, d); }
+template <int L>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+  if constexpr (L >= 2) v = max(v, rx_dppu<RX_DPP_XOR1>(v));
+  if constexpr (L >= 4) v = max(v, rx_dppu<RX_DPP_XOR2>(v));
+  if constexpr (L >= 8) v = max(v, rx_dppu<RX_DPP_HALF_MIRROR>(v));
+  if constexpr (L >= 16) v = max(v, rx_dppu<RX_DPP_MIRROR>(v));
+  if constexpr (L >= 32) v = max(v, lane_xor(v, 16));
+  if constexpr (L >= 64) v = max(v, lane_xor(v, 32));
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+  if constexpr (L >= 2) v += rx_dpp<RX_DPP_XOR1>(v);
+  if constexpr (L >= 4) v += rx_dpp<RX_DPP_XOR2>(v);
+  if constexpr (L >= 8) v += rx_dpp<RX_DPP_HALF_MIRROR>(v);
+  if constexpr (L >= 16) v += rx_dpp<RX_DPP_MIRROR>(v);
+  if constexpr (L >= 32) v += __shfl_xor(v, 16);
+  if constexpr (L >= 64) v += __shfl_xor(v, 32);
+  return v;
+}
+__device__ __forceinline__ double as_key(uint32_t hi, uint32_t lo) {
+  return __longlong_as_double((long long)(((unsigned long long)hi << 31) | lo));   // sign 0, never infinite or NaN
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_key(double v) {
+  const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+  return __longlong_as_double((long long)(((unsigned long long)rx_dppu<CTRL>((uint32_t)(b >> 32)) << 32) | rx_dppu<CTRL>((uint32_t)b)));
+}
+template <int L>
+__device__ __forceinline__ double group_max(double v) {
+  if constexpr (L >= 2) v = fmax(v, dpp_key<RX_DPP_XOR1>(v));
+  if constexpr (L >= 4) v = fmax(v, dpp_key<RX_DPP_XOR2>(v));
+  if constexpr (L >= 8) v = fmax(v, dpp_key<RX_DPP_HALF_MIRROR>(v));
+  if constexpr (L >= 16) v = fmax(v, dpp_key<RX_DPP_MIRROR>(v));
+  if constexpr (L >= 32) v = fmax(v, __shfl_xor(v, 16));
+  if constexpr (L >= 64) v = fmax(v, __shfl_xor(v, 32));
+  return v;
+}
+
+// e^x for x <= 0: relative error |x| 2^-24 and one ulp
+__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+
 template <int DT, int L, int V>
 __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>::type* __restrict__ z, long long ldz,
                                                         long long T, int E, int k, int renorm, float* __restrict__ w,
                                                         int* __restrict__ ids, float* __restrict__ norm) {
-  const int lane = threadIdx.x % L;
+  extern __shared__ float2 taken[];         // [rows of the workgroup][k]: unnormalised weight, expert
+  constexpr int N = Elem<DT>::kVec;
+  const int lane = threadIdx.x % L, first = lane * V;
   const long long t = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
   if (t >= T) return;
   const float kNone = -__builtin_huge_valf();
   float v[V];
   bool bad = false;
+  uint32_t key[V];
+  double wide[DT == 0 ? V : 1];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = i * L + lane;
-    v[i] = e < E ? Elem<DT>::get(z[t * ldz + e]) : kNone;
-    bad |= v[i] != v[i];
-  }
-  constexpr int kSlots = (kRouteMaxK + L - 1) / L;
-  float zs[kSlots];
-  int is[kSlots];
-  float peak = 0.f, total = 0.f;
-  for (int j = 0; j < k; ++j) {
-    float best = kNone;
-    int at = 0x7FFFFFFF;
+  for (int c = 0; c < V / N; ++c) {
+    Vec<DT> x;
+    const int at = first + c * N;
+    x.load(z + t * ldz + (at < E ? at : 0), E - at);
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (v[i] > best) {
-        best = v[i];
-        at = i * L + lane;
+    for (int q = 0; q < N; ++q) {
+      const int i = c * N + q;
+      const bool there = at + q < E;
+      v[i] = there ? Elem<DT>::get(x.e[q]) : kNone;
+      const bool nan = v[i] != v[i];
+      bad |= nan;
+      // a NaN goes with minus infinity, -0 with 0; places past the row are below everything (and E >= k, so never taken)
+      const uint32_t low = 0xFFFFu - (uint32_t)(at + q);
+      if constexpr (DT == 0) {
+        const uint32_t b = nan ? 0xFF800000u : __float_as_uint(v[i] + 0.f);
+        wide[i] = there ? as_key(order32(b), low) : 0.0;
+      } else {
+        const uint32_t b = nan ? (DT == 1 ? 0xFF80u : 0xFC00u) : x.e[q] == 0x8000u ? 0u : (uint32_t)x.e[q];
+        key[i] = there ? (order16(b) << 16) | low : 0u;
       }
+    }
+  }
+  // a key is a chosen logit's if it is above those of minus infinity
+  float peak = 0.f, total = 0.f;
+  uint32_t last = 0;
+  float2* mine = taken + (threadIdx.x / L) * k;
+  for (int j = 0; j < k; ++j) {
+    float zj;
+    int at;
+    bool there;
+    if constexpr (DT == 0) {
+      double best = wide[0];
 #pragma unroll
-    for (int d = 1; d < L; d <<= 1) {
-      const float ob = __shfl_xor(best, d);
-      const int oa = __shfl_xor(at, d);
-      const bool take = ob > best || (ob == best && oa < at);
-      best = take ? ob : best;
-      at = take ? oa : at;
+      for (int i = 1; i < V; ++i) best = fmax(best, wide[i]);
+      best = group_max<L>(best);
+      const unsigned long long b = (unsigned long long)__double_as_longlong(best);
+      const uint32_t o = (uint32_t)(b >> 31), low = (uint32_t)b & 0xFFFFu;
+      there = o > order32(0xFF800000u);
+      at = (int)(0xFFFFu - low);
+      zj = __uint_as_float((o & 0x80000000u) ? o & 0x7FFFFFFFu : ~o);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (at == first + i) wide[i] = 0.0;
+    } else {
+      uint32_t best = key[0] - last;
+#pragma unroll
+      for (int i = 1; i < V; ++i) best = max(best, key[i] - last);
+      best = group_max<L>(best);
+      last += best;
+      const uint32_t o = last >> 16;
+      there = o > order16(DT == 1 ? 0xFF80u : 0xFC00u);
+      at = (int)(0xFFFFu - (last & 0xFFFFu));
+      zj = Elem<DT>::get((u16)((o & 0x8000u) ? o & 0x7FFFu : ~o));
     }
     if (j == 0) {
-      peak = best > kNone ? best : 0.f;
+      peak = there ? zj : 0.f;
       if (!renorm) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) total += expf(v[i] - peak);
-#pragma unroll
-        for (int d = 1; d < L; d <<= 1) total += __shfl_xor(total, d);
+        for (int i = 0; i < V; ++i) total += exp_neg(v[i] - peak);
+        total = group_sum<L>(total);
       }
     }
-    const float ex = best > kNone ? expf(best - peak) : 0.f;
+    const float ex = there ? exp_neg(zj - peak) : 0.f;
     if (renorm) total += ex;
-#pragma unroll
-    for (int s = 0; s < kSlots; ++s)
-      if (j == s * L + lane) {
-        zs[s] = ex;
-        is[s] = best > kNone ? at : -1;
-      }
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (at == i * L + lane) v[i] = kNone;
+    if (lane == 0) mine[j] = make_float2(ex, __int_as_float(there ? at : -1));
   }
   // a NaN in the row shows in all of its weights
   const unsigned long long rows = __ballot(bad);
   const int shift = (threadIdx.x & 63) / L * L;
   const bool any = ((rows >> shift) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1)) != 0;
   const float inv = any ? __uint_as_float(0x7FC00000u) : total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-#pragma unroll
-  for (int s = 0; s < kSlots; ++s) {
-    const int j = s * L + lane;
-    if (j < k) {
-      w[t * k + j] = zs[s] * inv;
-      ids[t * k + j] = is[s];
-    }
+  wave_sync();                             // (a row's lanes are one wave's)
+  for (int j = lane; j < k; j += L) {
+    const float2 e = mine[j];
+    w[t * k + j] = e.x * inv;
+    ids[t * k + j] = __float_as_int(e.y);
   }
   if (norm != nullptr && lane == 0) {
     norm[2 * t] = peak;
@@ -147,37 +228,59 @@ __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>:
   }
 }
 
+// The chosen experts' terms are added through LDS, where a lane can reach any place of its row: in registers every one of
+// the k would cost a comparison with every one of the V.
 template <int DT, int L, int V>
 __global__ __launch_bounds__(256) void route_bwd_kernel(const typename Elem<DT>::type* __restrict__ z, long long ldz,
                                                         const float* __restrict__ norm, const float* __restrict__ w,
                                                         const int* __restrict__ ids, const float* __restrict__ dw,
                                                         long long T, int E, int k,
                                                         typename Elem<DT>::type* __restrict__ dz) {
-  const int lane = threadIdx.x % L;
+  __shared__ f32x4 rows[256 * V / 4 + 256 / L];      // 16 bytes between rows: their lanes then start on different banks
+  constexpr int N = Elem<DT>::kVec;
+  const int lane = threadIdx.x % L, first = lane * V;
   const long long t = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
   if (t >= T) return;
+  f32x4* row = rows + (threadIdx.x / L) * (L * V / 4 + 1);
   float s = 0.f;
-  for (int j = 0; j < k; ++j) s = ids[t * k + j] >= 0 ? fmaf(w[t * k + j], dw[t * k + j], s) : s;
-  float g[V];
+  for (int j = lane; j < k; j += L)
+    if (ids[t * k + j] >= 0) s = fmaf(w[t * k + j], dw[t * k + j], s);
+  s = group_sum<L>(s);
+  const bool full = norm != nullptr;
+  const float peak = full ? norm[2 * t] : 0.f, scale = full ? -s * norm[2 * t + 1] : 0.f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = i * L + lane;
-    g[i] = 0.f;
-    if (norm != nullptr && e < E)
-      g[i] = -s * (expf(Elem<DT>::get(z[t * ldz + e]) - norm[2 * t]) * norm[2 * t + 1]);
+  for (int c = 0; c < V / N; ++c) {
+    const int at = first + c * N;
+    Vec<DT> x;
+    if (full) x.load(z + t * ldz + (at < E ? at : 0), E - at);
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+      f32x4 g = {0.f, 0.f, 0.f, 0.f};
+      if (full) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] = scale * exp_neg(Elem<DT>::get(x.e[q * 4 + i]) - peak);
+      }
+      row[(at >> 2) + q] = g;
+    }
   }
-  for (int j = 0; j < k; ++j) {
+  wave_sync();
+  float* flat = (float*)row;
+  for (int j = lane; j < k; j += L) {
     const int e = ids[t * k + j];
-    if (e < 0) continue;
-    const float add = w[t * k + j] * (norm != nullptr ? dw[t * k + j] : dw[t * k + j] - s);
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (e == i * L + lane) g[i] += add;
+    if (e >= 0) flat[e] += w[t * k + j] * (full ? dw[t * k + j] : dw[t * k + j] - s);
   }
+  wave_sync();
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = i * L + lane;
-    if (e < E) dz[t * E + e] = Elem<DT>::put(g[i]);
+  for (int c = 0; c < V / N; ++c) {
+    const int at = first + c * N;
+    Vec<DT> o;
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+      const f32x4 g = row[(at >> 2) + q];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o.e[q * 4 + i] = Elem<DT>::put(g[i]);
+    }
+    if (at < E) o.store(dz + t * E + at, E - at);
   }
 }
 
@@ -287,7 +390,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_rank_kernel(PlanArgs a) {
   }
   int bits = 0;
   while ((1 << bits) < E) ++bits;
-  volatile int* mynext = next + wave * E;
+  int* mynext = next + wave * E;
   for (int c = 0; c < piece && first + c < a.n; c += 64) {
     const long long i = first + c + lane;
     const bool there = c + lane < piece && i < a.n;
@@ -303,9 +406,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_rank_kernel(PlanArgs a) {
       rank = mynext[e] + below;
       row = a.capacity > 0 && rank >= a.capacity ? -1 : total[e] + rank;
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     if (e >= 0 && (same >> lane) == 1ull) mynext[e] = rank + 1;     // the last of its lanes
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     if (there) {
       a.position[i] = row;
       if (row >= 0) a.source[row] = (int)i;
@@ -326,16 +429,29 @@ struct RowArgs {
   float* dw;                  // scatter with h: [T][k]
 };
 
-template <int DT>
+constexpr int kTogether = 4;   // expert rows of a sample that are in flight together
+constexpr int kLook = 16;      // expert rows that a wave looks at for empty ones
+
+// The sample that a group of lanes works on. A whole wave's sample is uniform, and saying so puts its choices and weights
+// into scalar registers and the row addresses into scalar bases.
+template <bool WAVE>
+__device__ __forceinline__ long long rows_sample(int lg) {
+  if constexpr (WAVE) return (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  return ((long long)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg);
+}
+
+// W: times weights; H: and inner products of the sample's row with h's
+template <int DT, bool W, bool H, bool WAVE>
 __global__ __launch_bounds__(256) void rows_scatter_kernel(RowArgs a, unsigned sample_blocks) {
   typedef typename Elem<DT>::type T;
   constexpr int N = Elem<DT>::kVec;
-  T* out = (T*)a.out;
-  if (blockIdx.x >= sample_blocks) {        // rows that no sample fills: 64 looked at by each wave, zeroed together
+  T* __restrict__ out = (T*)a.out;
+  if (blockIdx.x >= sample_blocks) {        // rows that no sample fills are zeroed by a wave together
     const int lane = threadIdx.x & 63;
-    const long long r0 = ((long long)(blockIdx.x - sample_blocks) * 4 + (threadIdx.x >> 6)) * 64;
+    const long long r0 = ((long long)(blockIdx.x - sample_blocks) * 4 + (threadIdx.x >> 6)) * kLook;
     const long long r = r0 + lane;
-    unsigned long long empty = __ballot(r < a.rows && a.source[r < a.rows ? r : 0] < 0);
+    const bool look = lane < kLook && r < a.rows;
+    unsigned long long empty = __ballot(look && a.source[look ? r : 0] < 0);
     Vec<DT> zero;
     zero.w = (u32x4){0, 0, 0, 0};
     while (empty) {
@@ -345,65 +461,110 @@ __global__ __launch_bounds__(256) void rows_scatter_kernel(RowArgs a, unsigned s
     }
     return;
   }
-  const int L = 1 << a.lg, lane = threadIdx.x & (L - 1);
-  const long long t = ((long long)blockIdx.x << (8 - a.lg)) + (threadIdx.x >> a.lg);
+  const int L = WAVE ? 64 : 1 << a.lg, lane = threadIdx.x & (L - 1);
+  const long long t = rows_sample<WAVE>(a.lg);
   if (t >= a.T) return;
-  const T* x = (const T*)a.x + t * a.ldx;
-  const T* h = (const T*)a.h;
-  for (int j = 0; j < a.k; ++j) {
-    const long long row = a.position[t * a.k + j];
-    float dot = 0.f;
-    if (row >= 0) {
-      const float w = a.w != nullptr ? a.w[t * a.k + j] : 1.f;
-      for (int d = lane * N; d < a.D; d += L * N) {
-        Vec<DT> v;
-        v.load(x + d, a.D - d);
-        if (h != nullptr) {
-          Vec<DT> u;
-          u.load(h + row * a.D + d, a.D - d);
+  const T* __restrict__ x = (const T*)a.x + t * a.ldx;
+  const T* __restrict__ h = (const T*)a.h;
+  for (int j0 = 0; j0 < a.k; j0 += kTogether) {
+    long long row[kTogether];
+    float w[kTogether], dot[kTogether];
 #pragma unroll
-          for (int q = 0; q < N; ++q) dot = fmaf(Elem<DT>::get(v.e[q]), Elem<DT>::get(u.e[q]), dot);
-        }
-        if (a.w != nullptr) {
+    for (int j = 0; j < kTogether; ++j) {
+      const bool there = j0 + j < a.k;
+      row[j] = there ? (long long)a.position[t * a.k + j0 + j] : -1ll;
+      w[j] = W && there ? a.w[t * a.k + j0 + j] : 1.f;
+      dot[j] = 0.f;
+    }
+    for (int d = lane * N; d < a.D; d += L * N) {
+      Vec<DT> v, u[H ? kTogether : 1];
+      v.load(x + d, a.D - d);
+      if constexpr (H) {
 #pragma unroll
-          for (int q = 0; q < N; ++q) v.e[q] = Elem<DT>::put(Elem<DT>::get(v.e[q]) * w);
+        for (int j = 0; j < kTogether; ++j)
+          if (row[j] >= 0) u[j].load(h + row[j] * a.D + d, a.D - d);
+      }
+#pragma unroll
+      for (int j = 0; j < kTogether; ++j) {
+        if (row[j] < 0) continue;
+        Vec<DT> o = v;
+        if constexpr (H) {
+#pragma unroll
+          for (int q = 0; q < N; ++q) dot[j] = fmaf(Elem<DT>::get(v.e[q]), Elem<DT>::get(u[j].e[q]), dot[j]);
         }
-        v.store(out + row * a.D + d, a.D - d);
+        if constexpr (W) {
+#pragma unroll
+          for (int q = 0; q < N; ++q) o.e[q] = Elem<DT>::put(Elem<DT>::get(v.e[q]) * w[j]);
+        }
+        o.store(out + row[j] * a.D + d, a.D - d);
       }
     }
-    if (a.dw != nullptr) {
-      for (int s = 1; s < L; s <<= 1) dot += __shfl_xor(dot, s);
-      if (lane == 0) a.dw[t * a.k + j] = dot;
+    if constexpr (H) {
+#pragma unroll
+      for (int j = 0; j < kTogether; ++j) {
+        if (j0 + j >= a.k) break;
+        for (int s = 1; s < L; s <<= 1) dot[j] += __shfl_xor(dot[j], s);
+        if (lane == 0) a.dw[t * a.k + j0 + j] = dot[j];
+      }
     }
   }
 }
 
-template <int DT>
+// P: vectors of a row in flight per lane
+template <int DT, bool W, bool WAVE, int P>
 __global__ __launch_bounds__(256) void rows_gather_kernel(RowArgs a) {
   typedef typename Elem<DT>::type T;
   constexpr int N = Elem<DT>::kVec;
-  const int L = 1 << a.lg, lane = threadIdx.x & (L - 1);
-  const long long t = ((long long)blockIdx.x << (8 - a.lg)) + (threadIdx.x >> a.lg);
+  const int L = WAVE ? 64 : 1 << a.lg, lane = threadIdx.x & (L - 1);
+  const long long t = rows_sample<WAVE>(a.lg);
   if (t >= a.T) return;
-  const T* h = (const T*)a.h;
-  T* out = (T*)a.out + t * a.D;
-  for (int d = lane * N; d < a.D; d += L * N) {
-    float sum[N];
+  const T* __restrict__ h = (const T*)a.h;
+  T* __restrict__ out = (T*)a.out + t * a.D;
+  const int* __restrict__ position = a.position + t * a.k;
+  const float* __restrict__ weight = W ? a.w + t * a.k : nullptr;
+  for (int d0 = lane * N; d0 < a.D; d0 += L * N * P) {
+    float sum[P][N];
 #pragma unroll
-    for (int q = 0; q < N; ++q) sum[q] = 0.f;
-    for (int j = 0; j < a.k; ++j) {
-      const long long row = a.position[t * a.k + j];
-      if (row < 0) continue;
-      const float w = a.w != nullptr ? a.w[t * a.k + j] : 1.f;
-      Vec<DT> v;
-      v.load(h + row * a.D + d, a.D - d);
+    for (int p = 0; p < P; ++p)
 #pragma unroll
-      for (int q = 0; q < N; ++q) sum[q] = fmaf(w, Elem<DT>::get(v.e[q]), sum[q]);
+      for (int q = 0; q < N; ++q) sum[p][q] = 0.f;
+    for (int j0 = 0; j0 < a.k; j0 += kTogether) {
+      long long row[kTogether];
+      float w[kTogether];
+#pragma unroll
+      for (int j = 0; j < kTogether; ++j) {
+        const bool there = j0 + j < a.k;
+        row[j] = there ? (long long)position[j0 + j] : -1ll;
+        w[j] = W && there ? weight[j0 + j] : 1.f;
+      }
+      Vec<DT> v[kTogether][P];
+#pragma unroll
+      for (int j = 0; j < kTogether; ++j)
+        if (row[j] >= 0) {
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            const int d = d0 + p * L * N;
+            v[j][p].load(h + row[j] * a.D + d, a.D - d);
+          }
+        }
+#pragma unroll
+      for (int j = 0; j < kTogether; ++j) {
+        if (row[j] < 0) continue;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int q = 0; q < N; ++q)
+            sum[p][q] = W ? fmaf(w[j], Elem<DT>::get(v[j][p].e[q]), sum[p][q]) : sum[p][q] + Elem<DT>::get(v[j][p].e[q]);
+      }
     }
-    Vec<DT> o;
 #pragma unroll
-    for (int q = 0; q < N; ++q) o.e[q] = Elem<DT>::put(sum[q]);
-    o.store(out + d, a.D - d);
+    for (int p = 0; p < P; ++p) {
+      const int d = d0 + p * L * N;
+      Vec<DT> o;
+#pragma unroll
+      for (int q = 0; q < N; ++q) o.e[q] = Elem<DT>::put(sum[p][q]);
+      o.store(out + d, a.D - d);
+    }
   }
 }
 
@@ -417,19 +578,23 @@ int route_launch(int bwd, const void* z, long long ldz, const float* norm, float
     hipLaunchKernelGGL((route_bwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), 0, stream, (const S*)z, ldz, norm,
                        w, ids, dw, T, E, k, (S*)dz);
   else
-    hipLaunchKernelGGL((route_fwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), 0, stream, (const S*)z, ldz, T, E,
-                       k, renorm, w, ids, norm_out);
+    hipLaunchKernelGGL((route_fwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), sizeof(float2) * (256 / L) * k,
+                       stream, (const S*)z, ldz, T, E, k, renorm, w, ids, norm_out);
   return (int)hipGetLastError();
 }
 
+// Lanes and logits per lane: the fewest lanes that hold a row in at most 16 logits each, since what crosses lanes is paid
+// per row and a wave then has 64 / L rows to overlap; a lane's logits are whole 16-byte loads.
 template <int DT>
 int route_pick(int bwd, const void* z, long long ldz, const float* norm, float* w, int* ids, const float* dw, long long T,
                int E, int k, int renorm, float* norm_out, void* dz, hipStream_t stream) {
 #define RX_ROUTE(L, V) \
   return route_launch<DT, L, V>(bwd, z, ldz, norm, w, ids, dw, T, E, k, renorm, norm_out, dz, stream)
-  if (E <= 16) RX_ROUTE(4, 4);
-  if (E <= 64) RX_ROUTE(8, 8);
-  if (E <= 128) RX_ROUTE(16, 8);
+  if (E <= 8) RX_ROUTE(1, 8);
+  if (E <= 16) RX_ROUTE(2, 8);
+  if (E <= 32) RX_ROUTE(4, 8);
+  if (E <= 64) RX_ROUTE(4, 16);
+  if (E <= 128) RX_ROUTE(8, 16);
   if (E <= 256) RX_ROUTE(16, 16);
   if (E <= 512) RX_ROUTE(32, 16);
   RX_ROUTE(64, 16);
@@ -493,13 +658,30 @@ int rx_expert_plan(const PlanArgs* a, int* counts, hipStream_t stream) {
 
 int rx_rows_scatter(const RowArgs* a, int dtype, hipStream_t stream) {
   if (a->T < 0 || a->rows < 0 || a->k <= 0 || a->D <= 0 || a->lg < 0 || a->lg > 6 || dtype < 0 || dtype > 2) return -1;
-  const long long sb = (a->T + (256 >> a->lg) - 1) >> (8 - a->lg), grid = sb + (a->rows + 255) / 256;
+  // (without samples only rows are zeroed)
+  const bool weighted = a->T > 0 && a->w != nullptr, products = a->T > 0 && a->h != nullptr;
+  if (products && (a->dw == nullptr || !weighted)) return -1;
+  const long long sb = (a->T + (256 >> a->lg) - 1) >> (8 - a->lg), grid = sb + (a->rows + 4 * kLook - 1) / (4 * kLook);
   if (grid == 0) return 0;
   if (grid > 0x7FFFFFFFll) return -1;
   const dim3 g((unsigned)grid), b(256);
-  if (dtype == 0) hipLaunchKernelGGL((rows_scatter_kernel<0>), g, b, 0, stream, *a, (unsigned)sb);
-  else if (dtype == 1) hipLaunchKernelGGL((rows_scatter_kernel<1>), g, b, 0, stream, *a, (unsigned)sb);
-  else hipLaunchKernelGGL((rows_scatter_kernel<2>), g, b, 0, stream, *a, (unsigned)sb);
+  const bool wave = a->lg == 6;
+#define RX_SCATTER_AS(DT, W, H)                                                                                         \
+  do {                                                                                                               \
+    if (wave) hipLaunchKernelGGL((rows_scatter_kernel<DT, W, H, true>), g, b, 0, stream, *a, (unsigned)sb);          \
+    else hipLaunchKernelGGL((rows_scatter_kernel<DT, W, H, false>), g, b, 0, stream, *a, (unsigned)sb);              \
+  } while (0)
+#define RX_SCATTER(W, H)                       \
+  do {                                         \
+    if (dtype == 0) RX_SCATTER_AS(0, W, H);    \
+    else if (dtype == 1) RX_SCATTER_AS(1, W, H); \
+    else RX_SCATTER_AS(2, W, H);               \
+  } while (0)
+  if (products) RX_SCATTER(true, true);
+  else if (weighted) RX_SCATTER(true, false);
+  else RX_SCATTER(false, false);
+#undef RX_SCATTER
+#undef RX_SCATTER_AS
   return (int)hipGetLastError();
 }
 
@@ -509,9 +691,22 @@ int rx_rows_gather(const RowArgs* a, int dtype, hipStream_t stream) {
   if (grid == 0) return 0;
   if (grid > 0x7FFFFFFFll) return -1;
   const dim3 g((unsigned)grid), b(256);
-  if (dtype == 0) hipLaunchKernelGGL((rows_gather_kernel<0>), g, b, 0, stream, *a);
-  else if (dtype == 1) hipLaunchKernelGGL((rows_gather_kernel<1>), g, b, 0, stream, *a);
-  else hipLaunchKernelGGL((rows_gather_kernel<2>), g, b, 0, stream, *a);
+  const bool wave = a->lg == 6;
+#define RX_GATHER_AS(DT, W)                                                                        \
+  do {                                                                                             \
+    if (wave) hipLaunchKernelGGL((rows_gather_kernel<DT, W, true, 2>), g, b, 0, stream, *a);       \
+    else hipLaunchKernelGGL((rows_gather_kernel<DT, W, false, 1>), g, b, 0, stream, *a);           \
+  } while (0)
+#define RX_GATHER(W)                       \
+  do {                                     \
+    if (dtype == 0) RX_GATHER_AS(0, W);    \
+    else if (dtype == 1) RX_GATHER_AS(1, W); \
+    else RX_GATHER_AS(2, W);               \
+  } while (0)
+  if (a->w != nullptr) RX_GATHER(true);
+  else RX_GATHER(false);
+#undef RX_GATHER
+#undef RX_GATHER_AS
   return (int)hipGetLastError();
 }
 

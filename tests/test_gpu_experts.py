@@ -83,6 +83,13 @@ def test_route_layouts_nan_and_infinity():
         w, ids = route(z, 2, renorm)
         assert torch.isnan(w[1]).all() and torch.isfinite(w[0]).all() and torch.isfinite(w[2]).all()
         assert 2 not in ids[1].tolist()
+    for dtype in DTYPES:      # zeros of either sign are a tie; both ends of the type keep their order
+        big = torch.finfo(dtype).max
+        z = torch.tensor([[-0.0, 0.0, -0.0, 0.0], [0.0, -0.0, 1.0, -1.0], [-big, -math.inf, big, 0.0]], device="cuda").to(dtype)
+        assert route(z, 4)[1].tolist() == [[0, 1, 2, 3], [2, 0, 1, 3], [2, 3, 0, -1]]
+        z = torch.full((1, 7), math.nan, device="cuda").to(dtype)
+        w, ids = route(z, 3)
+        assert ids.tolist() == [[-1, -1, -1]] and torch.isnan(w).all()
     w, ids = route(torch.empty(0, 5, device="cuda"), 2)
     assert w.shape == (0, 2) and ids.shape == (0, 2)
 
