@@ -21,7 +21,7 @@
 
 namespace {
 
-constexpr int kAwMax = 48;      // tensors in one step launch (kernel arguments under 4 KiB)
+constexpr int kAwMax = 64;      // tensors in one step launch (kernel arguments under 4 KiB)
 constexpr int kPrepMax = 256;   // tensors in one preparation launch (one thread each)
 constexpr int kNormMax = 128;   // tensors in one norm / scale launch
 constexpr int kBlk = 256;       // elements that share a scale: 4 per lane of one wave
@@ -115,42 +115,64 @@ __device__ __forceinline__ uint32_t aw_wavemax(uint32_t v) {
   return max(q[0], q[1]);
 }
 
-// biased scale exponent of a block from the largest magnitude's bits (NaN and infinity: 255)
+// biased scale exponent of a block from the largest magnitude's bits (NaN and infinity: 255 or more)
 __device__ __forceinline__ int aw_scale(uint32_t top) { return (int)((top + 0xFFFFFu) >> 23); }
 __device__ __forceinline__ int aw_exp(int s) { return (s > 0 ? s : 1) - 127; }
 
-// code <-> value: a value scaled so that the code's smallest normal lands on fp32's is a code in its top bits
+// code <-> value: a value scaled so that the code's smallest normal lands on fp32's is a code in bits 20 on
 constexpr int kMShift = 112, kVShift = 96;   // 126 - 14, 126 - 30
-__device__ __forceinline__ float aw_dec_m(uint32_t c, int e) {
-  const float a = ldexpf(__uint_as_float((c & 0x7Fu) << 20), e + kMShift);
-  return (c & 0x80u) ? -a : a;
+template <int Q>
+__device__ __forceinline__ float aw_dec_m(uint32_t codes, int e) {   // byte Q: its sign goes to bit 31, the rest to 26..20
+  const int c = (int)(codes << (24 - 8 * Q)) >> 24;
+  return ldexpf(__uint_as_float((uint32_t)(c << 20) & 0x87F00000u), e + kMShift);
 }
-__device__ __forceinline__ float aw_dec_v(uint32_t c, int e) {
-  return ldexpf(__uint_as_float(c << 20), e + kVShift);
+template <int Q>
+__device__ __forceinline__ float aw_dec_v(uint32_t codes, int e) {
+  return ldexpf(__uint_as_float(((codes >> (8 * Q)) & 0xFFu) << 20), e + kVShift);
 }
+// the code in the top byte
 __device__ __forceinline__ uint32_t aw_enc_m(float m, int e, uint32_t rnd16) {
-  const uint32_t a = __float_as_uint(ldexpf(fabsf(m), -e - kMShift));
-  return ((a + (rnd16 * 16u + 8u)) >> 20) | ((__float_as_uint(m) >> 31) << 7);
+  const uint32_t a = __float_as_uint(ldexpf(fabsf(m), -e - kMShift)) + (rnd16 << 4) + 8u;
+  return ((a << 4) & 0x7FFFFFFFu) | (__float_as_uint(m) & 0x80000000u);
 }
 __device__ __forceinline__ uint32_t aw_enc_v(float v, int e, uint32_t rnd16) {
-  const uint32_t a = __float_as_uint(ldexpf(v, -e - kVShift));
-  const uint32_t c = (a + (rnd16 * 16u + 8u)) >> 20;
-  return (v > 0.f && c == 0u) ? 1u : c;      // what is not zero stays so: it is divided by
+  const uint32_t a = __float_as_uint(ldexpf(v, -e - kVShift)) + (rnd16 << 4) + 8u;
+  return (v != 0.f ? max(a, 0x100000u) : a) << 4;      // what is not zero stays so: it is divided by
+}
+// the top bytes of four words
+__device__ __forceinline__ uint32_t aw_pack(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0C0C0703u), hi = __builtin_amdgcn_perm(d, c, 0x07030C0Cu);
+  return lo | hi;
 }
 
-__device__ __forceinline__ u16 aw_dither_bf16(float x, uint32_t rnd16) {
-  const uint32_t b = __float_as_uint(x);
-  return (u16)(((b & 0x7FFFFFFFu) > 0x7F800000u ? b : b + rnd16) >> 16);
+// the upper half of x's bits plus the dither; two of them packed
+__device__ __forceinline__ uint32_t aw_dither_bf16x2(float x, float y, uint32_t rx, uint32_t ry) {
+  // (a NaN is made the plain one: its low bits plus the dither could carry into the sign)
+  const uint32_t a = (x != x ? 0x7FC00000u : __float_as_uint(x)) + rx, b = (y != y ? 0x7FC00000u : __float_as_uint(y)) + ry;
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
 }
 
-// 4 consecutive elements from i on; n: how many there are (<= 4)
-template <bool BF16>
+// Loads and stores of 4 consecutive elements; n: how many there are (<= 4); vec: aligned. NT: streamed past the caches. A
+// step that touches more than the 256 MB of the last-level cache gains by that (24 M fp32 with 32-bit moments, 384 MB:
+// 128 -> 112 us; 48 M with 8 bits: 148 -> 133), one that fits loses (16 M, 256 MB: 68 -> 76), so the host goes by the bytes.
+template <bool NT, class T>
+__device__ __forceinline__ T aw_get(const T* s) {
+  if constexpr (NT) return __builtin_nontemporal_load(s);
+  return *s;
+}
+template <bool NT, class T>
+__device__ __forceinline__ void aw_put(T* s, T v) {
+  if constexpr (NT) __builtin_nontemporal_store(v, s);
+  else *s = v;
+}
+
+template <bool BF16, bool NT = false>
 __device__ __forceinline__ f32x4 aw_load4(const void* base, long long i, int n, bool vec) {
   f32x4 r = {0.f, 0.f, 0.f, 0.f};
   if constexpr (BF16) {
     const u16* s = (const u16*)base + i;
     if (vec && n == 4) {
-      const uint2 w = *(const uint2*)s;
+      const rx_u32x2 w = aw_get<NT>((const rx_u32x2*)s);
       r[0] = rx_bf2f((u16)w.x);
       r[1] = __uint_as_float(w.x & 0xFFFF0000u);
       r[2] = rx_bf2f((u16)w.y);
@@ -163,7 +185,7 @@ __device__ __forceinline__ f32x4 aw_load4(const void* base, long long i, int n, 
   } else {
     const float* s = (const float*)base + i;
     if (vec && n == 4) {
-      r = *(const f32x4*)s;
+      r = aw_get<NT>((const f32x4*)s);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -173,35 +195,39 @@ __device__ __forceinline__ f32x4 aw_load4(const void* base, long long i, int n, 
   return r;
 }
 
+template <bool NT = false>
 __device__ __forceinline__ void aw_store4(float* s, const f32x4& r, int n, bool vec) {
   if (vec && n == 4) {
-    *(f32x4*)s = r;
+    aw_put<NT>((f32x4*)s, r);
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (k < n) s[k] = r[k];
   }
 }
-__device__ __forceinline__ void aw_store4h(u16* s, const u16* r, int n, bool vec) {
+template <bool NT = false>
+__device__ __forceinline__ void aw_store4h(u16* s, uint32_t lo, uint32_t hi, int n, bool vec) {
   if (vec && n == 4) {
-    *(uint2*)s = make_uint2(r[0] | (uint32_t)r[1] << 16, r[2] | (uint32_t)r[3] << 16);
+    aw_put<NT>((rx_u32x2*)s, (rx_u32x2){lo, hi});
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (k < n) s[k] = r[k];
+      if (k < n) s[k] = (u16)((k < 2 ? lo : hi) >> (16 * (k & 1)));
   }
 }
+template <bool NT = false>
 __device__ __forceinline__ uint32_t aw_load4c(const uint8_t* s, int n) {
-  if (n == 4) return *(const uint32_t*)s;
+  if (n == 4) return aw_get<NT>((const uint32_t*)s);
   uint32_t r = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (k < n) r |= (uint32_t)s[k] << (8 * k);
   return r;
 }
+template <bool NT = false>
 __device__ __forceinline__ void aw_store4c(uint8_t* s, uint32_t c, int n) {
   if (n == 4) {
-    *(uint32_t*)s = c;
+    aw_put<NT>((uint32_t*)s, c);
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -209,105 +235,141 @@ __device__ __forceinline__ void aw_store4c(uint8_t* s, uint32_t c, int n) {
   }
 }
 
-constexpr int kStepUnroll = 1;                        // scale blocks per wave
+__device__ __forceinline__ void aw_decode4(uint32_t mc, uint32_t vc, int sm, int sv, f32x4& m, f32x4& v) {
+  const int em = aw_exp(sm), ev = aw_exp(sv);
+  m[0] = aw_dec_m<0>(mc, em);
+  m[1] = aw_dec_m<1>(mc, em);
+  m[2] = aw_dec_m<2>(mc, em);
+  m[3] = aw_dec_m<3>(mc, em);
+  v[0] = aw_dec_v<0>(vc, ev);
+  v[1] = aw_dec_v<1>(vc, ev);
+  v[2] = aw_dec_v<2>(vc, ev);
+  v[3] = aw_dec_v<3>(vc, ev);
+}
+
+constexpr int kStepUnroll = 2;                        // scale blocks of a wave that are in flight together
 constexpr int kStepChunk = 4 * kBlk * kStepUnroll;    // elements per workgroup of 4 waves
 
-template <bool BITS8, bool BF16>
-__global__ __launch_bounds__(256) void aw_step_kernel(AwStep a) {
-  const AwHead head = *a.head;
-  if (head.skip) return;
-  const int t = aw_find(a, a.n, blockIdx.x);
-  const AwTensor k = a.tensors[t];
-  const long long n = a.len[t];
-  void* p = a.p[t];
-  const void* g = a.g[t];
-  u16* img = BF16 ? nullptr : a.img[t];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const bool vec = (((uintptr_t)p | (uintptr_t)g | (uintptr_t)img * 2) & 15) == 0;
-#pragma unroll
-  for (int u = 0; u < kStepUnroll; ++u) {
-    const long long blk = (long long)(blockIdx.x - a.start[t]) * (4 * kStepUnroll) + wave * kStepUnroll + u;
-    const long long i = blk * kBlk + lane * 4;
-    const int left = n - i >= 4 ? 4 : n - i > 0 ? (int)(n - i) : 0;
-    if (blk * kBlk >= n) break;                       // (wave-uniform)
-    f32x4 pv = aw_load4<BF16>(p, i, left, vec), gv = aw_load4<BF16>(g, i, left, vec);
-    f32x4 mv, vv;
-    uint8_t* sc = nullptr;
+struct AwPlace {       // where a launch's workgroup works (wave-uniform)
+  void* p;
+  const void* g;
+  void *m, *v;
+  uint8_t* sc;
+  u16* img;
+  long long n;
+};
+
+// One lane's share of a scale block: 4 elements. FULL: the block lies inside the tensor and the vectors are aligned, so
+// loads and stores are whole and nothing branches; otherwise element by element under the tensor's end.
+template <bool BITS8, bool BF16, bool NT, bool FULL>
+struct AwLane {
+  f32x4 p, g, m, v;
+  uint32_t mc, vc;
+  int sm, sv;
+
+  __device__ __forceinline__ void load(const AwPlace& a, long long blk, long long i, int left) {
+    p = aw_load4<BF16, NT>(a.p, i, left, FULL);
+    g = aw_load4<BF16, NT>(a.g, i, left, FULL);
     if constexpr (BITS8) {
-      sc = a.sc[t] + blk * 2;
-      const int sm = sc[0], sv = sc[1];
-      const uint32_t mc = aw_load4c((const uint8_t*)a.m[t] + i, left), vc = aw_load4c((const uint8_t*)a.v[t] + i, left);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        mv[q] = aw_dec_m((mc >> (8 * q)) & 0xFFu, aw_exp(sm));
-        vv[q] = aw_dec_v((vc >> (8 * q)) & 0xFFu, aw_exp(sv));
-      }
-      if (sm == 255 || sv == 255) {
-        const float nan = __uint_as_float(0x7FC00000u);
-        mv = sm == 255 ? (f32x4){nan, nan, nan, nan} : mv;
-        vv = sv == 255 ? (f32x4){nan, nan, nan, nan} : vv;
-      }
+      const u16 s = *(const u16*)(a.sc + blk * 2);
+      sm = s & 0xFF;
+      sv = s >> 8;
+      mc = aw_load4c<NT>((const uint8_t*)a.m + i, left);
+      vc = aw_load4c<NT>((const uint8_t*)a.v + i, left);
     } else {
-      mv = aw_load4<false>(a.m[t], i, left, true);
-      vv = aw_load4<false>(a.v[t], i, left, true);
+      m = aw_load4<false, NT>(a.m, i, left, FULL);
+      v = aw_load4<false, NT>(a.v, i, left, FULL);
+    }
+  }
+
+  __device__ __forceinline__ void step(const AwStep& c, const AwTensor& k, float gscale, const AwPlace& a, long long blk,
+                                       long long i, int left, int lane) {
+    float b1 = c.b1, b2 = c.b2;
+    if constexpr (BITS8) {
+      aw_decode4(mc, vc, sm, sv, m, v);
+      // a block that was not finite: what remains of its moments is NaN
+      b1 = sm == 255 ? __uint_as_float(0x7FC00000u) : b1;
+      b2 = sv == 255 ? __uint_as_float(0x7FC00000u) : b2;
     }
     uint32_t h[4];
     uint32_t mtop = 0, vtop = 0;
+    uint32_t x = 0;
+    if constexpr (BITS8 || BF16) x = (uint32_t)i * kPhi + (uint32_t)((unsigned long long)i >> 32) * kSq2 + k.key;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       {
 #pragma clang fp contract(off)
-        const float gq = gv[q] * head.gscale;
-        mv[q] = a.b1 * mv[q] + a.omb1 * gq;
-        vv[q] = a.b2 * vv[q] + a.omb2 * (gq * gq);
+        const float gq = g[q] * gscale;
+        m[q] = b1 * m[q] + c.omb1 * gq;
+        v[q] = b2 * v[q] + c.omb2 * (gq * gq);
       }
       // square root and quotient to 1 ulp each: the update is about 1e-3 of p
-      const float den = fmaf(__builtin_amdgcn_sqrtf(vv[q]), k.rs_bc2, a.eps);
-      pv[q] = fmaf(k.nlr_bc1, mv[q] * __builtin_amdgcn_rcpf(den), pv[q] * k.decay);
-      if (q < left) {
-        mtop = max(mtop, __float_as_uint(mv[q]) & 0x7FFFFFFFu);
-        vtop = max(vtop, __float_as_uint(vv[q]) & 0x7FFFFFFFu);
+      const float den = fmaf(__builtin_amdgcn_sqrtf(v[q]), k.rs_bc2, c.eps);
+      p[q] = fmaf(k.nlr_bc1, m[q] * __builtin_amdgcn_rcpf(den), p[q] * k.decay);
+      if (FULL || q < left) {
+        mtop = max(mtop, __float_as_uint(m[q]) & 0x7FFFFFFFu);
+        vtop = max(vtop, __float_as_uint(v[q]));       // (not negative, or NaN)
       }
-      if constexpr (BITS8 || BF16) {
-        const unsigned long long j = (unsigned long long)i + q;
-        h[q] = aw_mix((uint32_t)j * kPhi + (uint32_t)(j >> 32) * kSq2 + k.key);
-      }
+      // (a lane's 4 indexes do not cross 2^32)
+      if constexpr (BITS8 || BF16) h[q] = aw_mix(x + q * kPhi);
     }
     if constexpr (BITS8) {
-      const int sm = aw_scale(aw_wavemax(mtop)), sv = aw_scale(aw_wavemax(vtop));
-      uint32_t mc = 0, vc = 0;
+      const int sm1 = aw_scale(aw_wavemax(mtop)), sv1 = aw_scale(aw_wavemax(vtop));
+      const int em = aw_exp(sm1), ev = aw_exp(sv1);
+      uint32_t me[4], ve[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        mc |= aw_enc_m(mv[q], aw_exp(sm), h[q] & 0xFFFFu) << (8 * q);
-        vc |= aw_enc_v(vv[q], aw_exp(sv), h[q] >> 16) << (8 * q);
+        me[q] = aw_enc_m(m[q], em, h[q] & 0xFFFFu);
+        ve[q] = aw_enc_v(v[q], ev, h[q] >> 16);
       }
-      if (sm == 255) mc = 0;
-      if (sv == 255) vc = 0;
-      aw_store4c((uint8_t*)a.m[t] + i, mc, left);
-      aw_store4c((uint8_t*)a.v[t] + i, vc, left);
-      if (lane == 0) {
-        sc[0] = (uint8_t)sm;
-        sc[1] = (uint8_t)sv;
-      }
+      const uint32_t m1 = sm1 >= 255 ? 0u : aw_pack(me[0], me[1], me[2], me[3]);
+      const uint32_t v1 = sv1 >= 255 ? 0u : aw_pack(ve[0], ve[1], ve[2], ve[3]);
+      aw_store4c<NT>((uint8_t*)a.m + i, m1, left);
+      aw_store4c<NT>((uint8_t*)a.v + i, v1, left);
+      if (lane == 0) *(u16*)(a.sc + blk * 2) = (u16)(min(sm1, 255) | min(sv1, 255) << 8);
     } else {
-      aw_store4((float*)a.m[t] + i, mv, left, true);
-      aw_store4((float*)a.v[t] + i, vv, left, true);
+      aw_store4<NT>((float*)a.m + i, m, left, FULL);
+      aw_store4<NT>((float*)a.v + i, v, left, FULL);
     }
     if constexpr (BF16) {
       // no master copy: rounded with the dither, so that updates under half a step of p are not lost
-      u16 o[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) o[q] = aw_dither_bf16(pv[q], (h[q] * kSq2) >> 16);
-      aw_store4h((u16*)p + i, o, left, vec);
+      const uint32_t lo = aw_dither_bf16x2(p[0], p[1], (h[0] * kSq2) >> 16, (h[1] * kSq2) >> 16);
+      const uint32_t hi = aw_dither_bf16x2(p[2], p[3], (h[2] * kSq2) >> 16, (h[3] * kSq2) >> 16);
+      aw_store4h<NT>((u16*)a.p + i, lo, hi, left, FULL);
     } else {
-      aw_store4((float*)p + i, pv, left, vec);
-      if (img != nullptr) {
-        u16 o[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) o[q] = rx_f2bf(pv[q]);
-        aw_store4h(img + i, o, left, vec);
+      aw_store4<NT>((float*)a.p + i, p, left, FULL);
+      if (a.img != nullptr) {
+        aw_store4h(a.img + i, rx_f2bf2(p[0], p[1]), rx_f2bf2(p[2], p[3]), left, FULL);
       }
     }
+  }
+};
+
+template <bool BITS8, bool BF16, bool NT>
+__global__ __launch_bounds__(256) void aw_step_kernel(AwStep c) {
+  const AwHead head = *c.head;
+  if (head.skip) return;
+  const int t = aw_find(c, c.n, blockIdx.x);
+  const AwTensor k = c.tensors[t];
+  const AwPlace a = {c.p[t], c.g[t], c.m[t], c.v[t], BITS8 ? c.sc[t] : nullptr, BF16 ? nullptr : c.img[t], c.len[t]};
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long blk = ((long long)(blockIdx.x - c.start[t]) * 4 + wave) * kStepUnroll;
+  // bf16 vectors are 8 bytes, an image's too
+  const uintptr_t low = BF16 ? ((uintptr_t)a.p | (uintptr_t)a.g) * 2 : (uintptr_t)a.p | (uintptr_t)a.g | (uintptr_t)a.img * 2;
+  if ((low & 15) == 0 && (blk + kStepUnroll) * kBlk <= a.n) {
+    AwLane<BITS8, BF16, NT, true> w[kStepUnroll];
+#pragma unroll
+    for (int u = 0; u < kStepUnroll; ++u) w[u].load(a, blk + u, (blk + u) * kBlk + lane * 4, 4);
+#pragma unroll
+    for (int u = 0; u < kStepUnroll; ++u) w[u].step(c, k, head.gscale, a, blk + u, (blk + u) * kBlk + lane * 4, 4, lane);
+    return;
+  }
+  for (long long b = blk; b < blk + kStepUnroll && b * kBlk < a.n; ++b) {
+    const long long i = b * kBlk + lane * 4;
+    const int left = a.n - i >= 4 ? 4 : a.n - i > 0 ? (int)(a.n - i) : 0;
+    AwLane<BITS8, BF16, NT, false> w;
+    w.load(a, b, i, left);
+    w.step(c, k, head.gscale, a, b, i, left, lane);
   }
 }
 
@@ -360,34 +422,76 @@ __global__ __launch_bounds__(256) void aw_prep_kernel(AwPrep a) {
 }
 
 // Sums of squares in 64 bits: the norm then does not depend on the order of the sum in any of its 32 bits but by chance.
-constexpr int kNormChunk = 4096;
+constexpr int kNormChunk = 8192;
 
-template <bool BF16>
-__device__ __forceinline__ double aw_squares(const void* g, long long i, long long n, bool vec) {
+// 4 x 4 (bf16: 2 x 8) elements of a lane, in flight together
+template <bool BF16, bool FULL>
+__device__ __forceinline__ double aw_squares(const void* g, long long i, long long n) {
   double s = 0.0;
+  if constexpr (BF16 && FULL) {
+    u32x4 w[kNormChunk / 2048];
+#pragma unroll
+    for (int u = 0; u < kNormChunk / 2048; ++u) w[u] = *(const u32x4*)((const u16*)g + i + u * 2048 + threadIdx.x * 8);
+#pragma unroll
+    for (int u = 0; u < kNormChunk / 2048; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float a = __uint_as_float(w[u][q] << 16), b = __uint_as_float(w[u][q] & 0xFFFF0000u);
+        s = fma((double)a, (double)a, s);
+        s = fma((double)b, (double)b, s);
+      }
+    return s;
+  }
+  f32x4 v[kNormChunk / 1024];
 #pragma unroll
   for (int u = 0; u < kNormChunk / 1024; ++u) {
     const long long j = i + u * 1024 + threadIdx.x * 4;
-    const int left = n - j >= 4 ? 4 : n - j > 0 ? (int)(n - j) : 0;
-    const f32x4 v = aw_load4<BF16>(g, j, left, vec);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) s = fma((double)v[q], (double)v[q], s);
+    v[u] = aw_load4<BF16>(g, j, FULL ? 4 : n - j >= 4 ? 4 : n - j > 0 ? (int)(n - j) : 0, FULL);
   }
+#pragma unroll
+  for (int u = 0; u < kNormChunk / 1024; ++u)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) s = fma((double)v[u][q], (double)v[u][q], s);
   return s;
 }
 
+// a workgroup takes consecutive chunks, so that it looks for its tensor once and then walks on
 __global__ __launch_bounds__(256) void norm_part_kernel(NormArgs a) {
   __shared__ double lds[4];
   double s = 0.0;
-  for (unsigned c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-    const int t = aw_find(a, a.n, c);
+  const unsigned per = a.chunks / gridDim.x, more = a.chunks % gridDim.x, b = blockIdx.x;
+  const unsigned first = b * per + min(b, more), last = first + per + (b < more ? 1u : 0u);
+  int t = first < last ? aw_find(a, a.n, first) : 0;
+  for (unsigned c = first; c < last; ++c) {
+    while (c >= a.start[t + 1]) ++t;
     const void* g = a.g[t];
-    const long long i = (long long)(c - a.start[t]) * kNormChunk;
-    const bool vec = ((uintptr_t)g & 15) == 0;
-    s += a.bf16[t] ? aw_squares<true>(g, i, a.len[t], vec) : aw_squares<false>(g, i, a.len[t], vec);
+    const long long i = (long long)(c - a.start[t]) * kNormChunk, n = a.len[t];
+    const bool full = i + kNormChunk <= n && ((uintptr_t)g & 15) == 0;
+    if (a.bf16[t]) s += full ? aw_squares<true, true>(g, i, n) : aw_squares<true, false>(g, i, n);
+    else s += full ? aw_squares<false, true>(g, i, n) : aw_squares<false, false>(g, i, n);
   }
   s = aw_blocksum(s, lds);
   if (threadIdx.x == 0) a.part[blockIdx.x] = s;
+}
+
+template <bool BF16, bool FULL>
+__device__ __forceinline__ void aw_scale_chunk(void* g, long long i, long long n, float f) {
+  constexpr int U = kNormChunk / 1024;
+  f32x4 v[U];
+  int left[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long j = i + u * 1024 + threadIdx.x * 4;
+    left[u] = FULL ? 4 : n - j >= 4 ? 4 : n - j > 0 ? (int)(n - j) : 0;
+    v[u] = aw_load4<BF16>(g, j, left[u], FULL);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long j = i + u * 1024 + threadIdx.x * 4;
+    v[u] *= f;
+    if constexpr (BF16) aw_store4h((u16*)g + j, rx_f2bf2(v[u][0], v[u][1]), rx_f2bf2(v[u][2], v[u][3]), left[u], FULL);
+    else aw_store4((float*)g + j, v[u], left[u], FULL);
+  }
 }
 
 // g *= min(1, max_norm / (norm + 1e-6)); every workgroup finishes the norm itself (a few KB out of L2), which saves a
@@ -398,60 +502,63 @@ __global__ __launch_bounds__(256) void norm_scale_kernel(ScaleArgs a) {
   const float f = aw_clip(norm, a.max_norm);
   if (blockIdx.x == 0 && threadIdx.x == 0 && a.norm != nullptr) *a.norm = (float)norm;
   if (f == 1.f) return;
-  for (unsigned c = blockIdx.x; c < a.t.chunks; c += gridDim.x) {
-    const int t = aw_find(a.t, a.t.n, c);
+  const unsigned per = a.t.chunks / gridDim.x, more = a.t.chunks % gridDim.x, b = blockIdx.x;
+  const unsigned first = b * per + min(b, more), last = first + per + (b < more ? 1u : 0u);
+  int t = first < last ? aw_find(a.t, a.t.n, first) : 0;
+  for (unsigned c = first; c < last; ++c) {
+    while (c >= a.t.start[t + 1]) ++t;
     void* g = const_cast<void*>(a.t.g[t]);
-    const long long n = a.t.len[t];
-    const bool vec = ((uintptr_t)g & 15) == 0;
-#pragma unroll
-    for (int u = 0; u < kNormChunk / 1024; ++u) {
-      const long long j = (long long)(c - a.t.start[t]) * kNormChunk + u * 1024 + threadIdx.x * 4;
-      const int left = n - j >= 4 ? 4 : n - j > 0 ? (int)(n - j) : 0;
-      if (left <= 0) continue;
-      if (a.t.bf16[t]) {
-        const f32x4 v = aw_load4<true>(g, j, left, vec);
-        u16 o[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) o[q] = rx_f2bf(v[q] * f);
-        aw_store4h((u16*)g + j, o, left, vec);
-      } else {
-        f32x4 v = aw_load4<false>(g, j, left, vec);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] *= f;
-        aw_store4((float*)g + j, v, left, vec);
-      }
-    }
+    const long long i = (long long)(c - a.t.start[t]) * kNormChunk, n = a.t.len[t];
+    const bool full = i + kNormChunk <= n && ((uintptr_t)g & 15) == 0;
+    if (a.t.bf16[t]) full ? aw_scale_chunk<true, true>(g, i, n, f) : aw_scale_chunk<true, false>(g, i, n, f);
+    else full ? aw_scale_chunk<false, true>(g, i, n, f) : aw_scale_chunk<false, false>(g, i, n, f);
   }
 }
 
-// codes -> the values they stand for (at most 4 significant bits: exact in bf16 too)
+// codes -> the values they stand for (at most 4 significant bits: exact in bf16 too); a wave takes whole scale blocks
+constexpr int kDecUnroll = 4;
+
+template <bool BF16, bool FULL>
+__device__ __forceinline__ void aw_decode_store(uint32_t mc, uint32_t vc, uint32_t s, void* mo, void* vo, long long i,
+                                                int left) {
+  const int sm = s & 0xFF, sv = s >> 8;
+  f32x4 m, v;
+  aw_decode4(mc, vc, sm, sv, m, v);
+  const float nan = __uint_as_float(0x7FC00000u);
+  if (sm == 255) m = (f32x4){nan, nan, nan, nan};
+  if (sv == 255) v = (f32x4){nan, nan, nan, nan};
+  if constexpr (BF16) {
+    aw_store4h((u16*)mo + i, rx_f2bf2(m[0], m[1]), rx_f2bf2(m[2], m[3]), left, FULL);
+    aw_store4h((u16*)vo + i, rx_f2bf2(v[0], v[1]), rx_f2bf2(v[2], v[3]), left, FULL);
+  } else {
+    aw_store4((float*)mo + i, m, left, FULL);
+    aw_store4((float*)vo + i, v, left, FULL);
+  }
+}
+
 template <bool BF16>
-__global__ __launch_bounds__(256) void aw_decode_kernel(const uint8_t* m, const uint8_t* v, const uint8_t* sc, void* mo,
-                                                        void* vo, long long n) {
-  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
-    const int left = n - i >= 4 ? 4 : (int)(n - i);
-    const int sm = sc[(i / kBlk) * 2], sv = sc[(i / kBlk) * 2 + 1];
-    const uint32_t mc = aw_load4c(m + i, left), vc = aw_load4c(v + i, left);
-    const float nan = __uint_as_float(0x7FC00000u);
-    f32x4 mv, vv;
+__global__ __launch_bounds__(256) void aw_decode_kernel(const uint8_t* __restrict__ m, const uint8_t* __restrict__ v,
+                                                        const uint8_t* __restrict__ sc, void* __restrict__ mo,
+                                                        void* __restrict__ vo, long long n) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long blk = ((long long)blockIdx.x * 4 + wave) * kDecUnroll;
+  if ((blk + kDecUnroll) * kBlk <= n) {
+    uint32_t mc[kDecUnroll], vc[kDecUnroll], s[kDecUnroll];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      mv[q] = sm == 255 ? nan : aw_dec_m((mc >> (8 * q)) & 0xFFu, aw_exp(sm));
-      vv[q] = sv == 255 ? nan : aw_dec_v((vc >> (8 * q)) & 0xFFu, aw_exp(sv));
+    for (int u = 0; u < kDecUnroll; ++u) {
+      s[u] = *(const u16*)(sc + (blk + u) * 2);
+      mc[u] = *(const uint32_t*)(m + (blk + u) * kBlk + lane * 4);
+      vc[u] = *(const uint32_t*)(v + (blk + u) * kBlk + lane * 4);
     }
-    if constexpr (BF16) {
-      u16 a[4], b[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        a[q] = rx_f2bf(mv[q]);
-        b[q] = rx_f2bf(vv[q]);
-      }
-      aw_store4h((u16*)mo + i, a, left, true);
-      aw_store4h((u16*)vo + i, b, left, true);
-    } else {
-      aw_store4((float*)mo + i, mv, left, true);
-      aw_store4((float*)vo + i, vv, left, true);
-    }
+    for (int u = 0; u < kDecUnroll; ++u)
+      aw_decode_store<BF16, true>(mc[u], vc[u], s[u], mo, vo, (blk + u) * kBlk + lane * 4, 4);
+    return;
+  }
+  for (long long b = blk; b < blk + kDecUnroll && b * kBlk < n; ++b) {
+    const long long i = b * kBlk + lane * 4;
+    const int left = n - i >= 4 ? 4 : n - i > 0 ? (int)(n - i) : 0;
+    aw_decode_store<BF16, false>(aw_load4c(m + i, left), aw_load4c(v + i, left), *(const u16*)(sc + b * 2), mo, vo, i, left);
   }
 }
 
@@ -477,15 +584,22 @@ int rx_aw_prep(const AwPrep* a, hipStream_t stream) {
   return (int)hipGetLastError();
 }
 
-int rx_aw_step(const AwStep* a, int bits, int bf16, hipStream_t stream) {
+// stream_past: the step's working set is larger than the last-level cache
+int rx_aw_step(const AwStep* a, int bits, int bf16, int stream_past, hipStream_t stream) {
   if (a->n <= 0 || a->n > kAwMax || (bits != 8 && bits != 32)) return -1;
   const unsigned grid = a->start[a->n];
   if (grid == 0) return 0;
   if (grid > 0x7FFFFFFFu) return -1;
-  if (bits == 8 && bf16) hipLaunchKernelGGL((aw_step_kernel<true, true>), dim3(grid), dim3(256), 0, stream, *a);
-  else if (bits == 8) hipLaunchKernelGGL((aw_step_kernel<true, false>), dim3(grid), dim3(256), 0, stream, *a);
-  else if (bf16) hipLaunchKernelGGL((aw_step_kernel<false, true>), dim3(grid), dim3(256), 0, stream, *a);
-  else hipLaunchKernelGGL((aw_step_kernel<false, false>), dim3(grid), dim3(256), 0, stream, *a);
+#define RX_AW(BITS8, BF16)                                                                                             \
+  do {                                                                                                                 \
+    if (stream_past) hipLaunchKernelGGL((aw_step_kernel<BITS8, BF16, true>), dim3(grid), dim3(256), 0, stream, *a);    \
+    else hipLaunchKernelGGL((aw_step_kernel<BITS8, BF16, false>), dim3(grid), dim3(256), 0, stream, *a);               \
+  } while (0)
+  if (bits == 8 && bf16) RX_AW(true, true);
+  else if (bits == 8) RX_AW(true, false);
+  else if (bf16) RX_AW(false, true);
+  else RX_AW(false, false);
+#undef RX_AW
   return (int)hipGetLastError();
 }
 
@@ -505,8 +619,8 @@ int rx_norm_scale(const ScaleArgs* a, int grid, hipStream_t stream) {
 int rx_aw_decode(const uint8_t* m, const uint8_t* v, const uint8_t* sc, void* mo, void* vo, long long n, int bf16,
                  hipStream_t stream) {
   if (n <= 0) return 0;
-  long long grid = (n + 1023) / 1024;
-  grid = grid > 8192 ? 8192 : grid;
+  const long long grid = (n + 4 * kDecUnroll * kBlk - 1) / (4 * kDecUnroll * kBlk);
+  if (grid > 0x7FFFFFFFll) return -1;
   if (bf16)
     hipLaunchKernelGGL((aw_decode_kernel<true>), dim3((unsigned)grid), dim3(256), 0, stream, m, v, sc, mo, vo, n);
   else

@@ -44,10 +44,12 @@ struct Vec {
     u32x4 w;
     T e[Elem<DT>::kVec];
   };
-  // n: elements there (a row's last vector may be short)
+  // n: elements there (a row's last vector may be short); NT: streamed past the caches
+  template <bool NT = false>
   __device__ __forceinline__ void load(const T* p, int n) {
     if (n >= Elem<DT>::kVec) {
-      w = *(const u32x4_u*)p;
+      if constexpr (NT) w = __builtin_nontemporal_load((const u32x4_u*)p);
+      else w = *(const u32x4_u*)p;
     } else {
       w = (u32x4){0, 0, 0, 0};
 #pragma unroll
@@ -55,9 +57,11 @@ struct Vec {
         if (i < n) e[i] = p[i];
     }
   }
+  template <bool NT = false>
   __device__ __forceinline__ void store(T* p, int n) const {
     if (n >= Elem<DT>::kVec) {
-      *(u32x4_u*)p = w;
+      if constexpr (NT) __builtin_nontemporal_store(w, (u32x4_u*)p);
+      else *(u32x4_u*)p = w;
     } else {
 #pragma unroll
       for (int i = 0; i < Elem<DT>::kVec - 1; ++i)
@@ -419,7 +423,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_rank_kernel(PlanArgs a) {
 // ------------------------------------------------------------------------------------------------ rows
 struct RowArgs {
   long long T, rows, ldx;     // samples, expert rows, elements between samples' rows (x)
-  int k, D, lg, pad_;         // lg: log2 of the lanes that work on a sample
+  int k, D, lg, stream;       // lg: log2 of the lanes that work on a sample; stream: rows go past the caches
   const int* position;        // [T][k]
   const int* source;          // [rows]
   const void* x;              // scatter: samples' rows in; gather: not used
@@ -441,7 +445,7 @@ __device__ __forceinline__ long long rows_sample(int lg) {
 }
 
 // W: times weights; H: and inner products of the sample's row with h's
-template <int DT, bool W, bool H, bool WAVE>
+template <int DT, bool W, bool H, bool WAVE, bool NT>
 __global__ __launch_bounds__(256) void rows_scatter_kernel(RowArgs a, unsigned sample_blocks) {
   typedef typename Elem<DT>::type T;
   constexpr int N = Elem<DT>::kVec;
@@ -457,7 +461,7 @@ __global__ __launch_bounds__(256) void rows_scatter_kernel(RowArgs a, unsigned s
     while (empty) {
       const int b = __ffsll((unsigned long long)empty) - 1;
       empty &= empty - 1;
-      for (int d = lane * N; d < a.D; d += 64 * N) zero.store(out + (r0 + b) * a.D + d, a.D - d);
+      for (int d = lane * N; d < a.D; d += 64 * N) zero.template store<NT>(out + (r0 + b) * a.D + d, a.D - d);
     }
     return;
   }
@@ -478,11 +482,11 @@ __global__ __launch_bounds__(256) void rows_scatter_kernel(RowArgs a, unsigned s
     }
     for (int d = lane * N; d < a.D; d += L * N) {
       Vec<DT> v, u[H ? kTogether : 1];
-      v.load(x + d, a.D - d);
+      v.template load<NT>(x + d, a.D - d);
       if constexpr (H) {
 #pragma unroll
         for (int j = 0; j < kTogether; ++j)
-          if (row[j] >= 0) u[j].load(h + row[j] * a.D + d, a.D - d);
+          if (row[j] >= 0) u[j].template load<NT>(h + row[j] * a.D + d, a.D - d);
       }
 #pragma unroll
       for (int j = 0; j < kTogether; ++j) {
@@ -496,7 +500,7 @@ __global__ __launch_bounds__(256) void rows_scatter_kernel(RowArgs a, unsigned s
 #pragma unroll
           for (int q = 0; q < N; ++q) o.e[q] = Elem<DT>::put(Elem<DT>::get(v.e[q]) * w[j]);
         }
-        o.store(out + row[j] * a.D + d, a.D - d);
+        o.template store<NT>(out + row[j] * a.D + d, a.D - d);
       }
     }
     if constexpr (H) {
@@ -511,7 +515,7 @@ __global__ __launch_bounds__(256) void rows_scatter_kernel(RowArgs a, unsigned s
 }
 
 // P: vectors of a row in flight per lane
-template <int DT, bool W, bool WAVE, int P>
+template <int DT, bool W, bool WAVE, int P, bool NT>
 __global__ __launch_bounds__(256) void rows_gather_kernel(RowArgs a) {
   typedef typename Elem<DT>::type T;
   constexpr int N = Elem<DT>::kVec;
@@ -544,7 +548,7 @@ __global__ __launch_bounds__(256) void rows_gather_kernel(RowArgs a) {
 #pragma unroll
           for (int p = 0; p < P; ++p) {
             const int d = d0 + p * L * N;
-            v[j][p].load(h + row[j] * a.D + d, a.D - d);
+            v[j][p].template load<NT>(h + row[j] * a.D + d, a.D - d);
           }
         }
 #pragma unroll
@@ -563,7 +567,7 @@ __global__ __launch_bounds__(256) void rows_gather_kernel(RowArgs a) {
       Vec<DT> o;
 #pragma unroll
       for (int q = 0; q < N; ++q) o.e[q] = Elem<DT>::put(sum[p][q]);
-      o.store(out + d, a.D - d);
+      o.template store<NT>(out + d, a.D - d);
     }
   }
 }
@@ -666,10 +670,14 @@ int rx_rows_scatter(const RowArgs* a, int dtype, hipStream_t stream) {
   if (grid > 0x7FFFFFFFll) return -1;
   const dim3 g((unsigned)grid), b(256);
   const bool wave = a->lg == 6;
-#define RX_SCATTER_AS(DT, W, H)                                                                                         \
-  do {                                                                                                               \
-    if (wave) hipLaunchKernelGGL((rows_scatter_kernel<DT, W, H, true>), g, b, 0, stream, *a, (unsigned)sb);          \
-    else hipLaunchKernelGGL((rows_scatter_kernel<DT, W, H, false>), g, b, 0, stream, *a, (unsigned)sb);              \
+#define RX_SCATTER_TO(DT, W, H, WAVE, NT) \
+  hipLaunchKernelGGL((rows_scatter_kernel<DT, W, H, WAVE, NT>), g, b, 0, stream, *a, (unsigned)sb)
+#define RX_SCATTER_AS(DT, W, H)                                   \
+  do {                                                            \
+    if (wave && a->stream) RX_SCATTER_TO(DT, W, H, true, true);   \
+    else if (wave) RX_SCATTER_TO(DT, W, H, true, false);          \
+    else if (a->stream) RX_SCATTER_TO(DT, W, H, false, true);     \
+    else RX_SCATTER_TO(DT, W, H, false, false);                   \
   } while (0)
 #define RX_SCATTER(W, H)                       \
   do {                                         \
@@ -682,6 +690,7 @@ int rx_rows_scatter(const RowArgs* a, int dtype, hipStream_t stream) {
   else RX_SCATTER(false, false);
 #undef RX_SCATTER
 #undef RX_SCATTER_AS
+#undef RX_SCATTER_TO
   return (int)hipGetLastError();
 }
 
@@ -692,10 +701,19 @@ int rx_rows_gather(const RowArgs* a, int dtype, hipStream_t stream) {
   if (grid > 0x7FFFFFFFll) return -1;
   const dim3 g((unsigned)grid), b(256);
   const bool wave = a->lg == 6;
-#define RX_GATHER_AS(DT, W)                                                                        \
-  do {                                                                                             \
-    if (wave) hipLaunchKernelGGL((rows_gather_kernel<DT, W, true, 2>), g, b, 0, stream, *a);       \
-    else hipLaunchKernelGGL((rows_gather_kernel<DT, W, false, 1>), g, b, 0, stream, *a);           \
+#define RX_GATHER_TO(DT, W, WAVE, P, NT) hipLaunchKernelGGL((rows_gather_kernel<DT, W, WAVE, P, NT>), g, b, 0, stream, *a)
+#define RX_GATHER_AS(DT, W)                                                        \
+  do {                                                                             \
+    if (wave && a->D > 64 * Elem<DT>::kVec) {                                      \
+      if (a->stream) RX_GATHER_TO(DT, W, true, 2, true);                           \
+      else RX_GATHER_TO(DT, W, true, 2, false);                                    \
+    } else if (wave) {                                                             \
+      if (a->stream) RX_GATHER_TO(DT, W, true, 1, true);                           \
+      else RX_GATHER_TO(DT, W, true, 1, false);                                    \
+    } else {                                                                       \
+      if (a->stream) RX_GATHER_TO(DT, W, false, 1, true);                          \
+      else RX_GATHER_TO(DT, W, false, 1, false);                                   \
+    }                                                                              \
   } while (0)
 #define RX_GATHER(W)                       \
   do {                                     \
@@ -707,6 +725,7 @@ int rx_rows_gather(const RowArgs* a, int dtype, hipStream_t stream) {
   else RX_GATHER(false);
 #undef RX_GATHER
 #undef RX_GATHER_AS
+#undef RX_GATHER_TO
   return (int)hipGetLastError();
 }
 

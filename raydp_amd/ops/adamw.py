@@ -1,7 +1,7 @@
 """AdamW over many tensors with the moments in 8 or 32 bits, and clipping by the global gradient norm
 (``csrc/hip/adamw.hip``; public names in :mod:`raydp_amd.ops.fused_optim`).
 
-* :class:`FusedAdamW` -- ``torch.optim.AdamW``'s update (decoupled weight decay) as one launch per 48 tensors.
+* :class:`FusedAdamW` -- ``torch.optim.AdamW``'s update (decoupled weight decay) as one launch per 64 tensors.
   Parameters are contiguous fp32 or bf16. ``state_bits=8`` keeps each moment in one byte plus two scale bytes per 256
   elements (2.01 bytes per parameter where fp32 moments take 8); ``state_bits=32`` keeps them in fp32. fp32 weights
   that a fused Linear tower reads get their bf16 image in the same pass; bf16 parameters have no master copy and are
@@ -24,9 +24,10 @@ import torch
 from raydp_amd.ops import _hip
 
 BLOCK = 256                  # elements of a tensor that share a scale
-AW_MAX, PREP_MAX, NORM_MAX = 48, 256, 128
-STEP_CHUNK, NORM_CHUNK = 1024, 4096
+AW_MAX, PREP_MAX, NORM_MAX = 64, 256, 128
+STEP_CHUNK, NORM_CHUNK = 2048, 8192
 NORM_GRID = 1024             # partial sums of one norm launch at most
+LAST_LEVEL = 256 << 20       # bytes of the last-level cache: steps that touch more are streamed past it
 _M_EMIN, _V_EMIN = -14, -30
 _MASK, _PHI, _SQ2, _SQ3 = 0xFFFFFFFF, 0x9E3779B1, 0x6A09E667, 0xBB67AE85
 
@@ -69,7 +70,7 @@ def _lib():
     if _bound is not L:
         vp, i, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
         L.rx_aw_prep.argtypes = [vp, vp]
-        L.rx_aw_step.argtypes = [vp, i, i, vp]
+        L.rx_aw_step.argtypes = [vp, i, i, i, vp]
         L.rx_norm_part.argtypes = [vp, i, vp]
         L.rx_norm_scale.argtypes = [vp, i, vp]
         L.rx_aw_decode.argtypes = [vp, vp, vp, vp, vp, ll, i, vp]
@@ -270,7 +271,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
             s = ScaleArgs()
             s.t, s.npart, s.max_norm = a, npart, max_norm
             s.t.part, s.norm = part.data_ptr(), norm.data_ptr() if k == 0 else None
-            _hip.check(L.rx_norm_scale(ctypes.byref(s), min(a.chunks, 8192), stream), "rx_norm_scale")
+            _hip.check(L.rx_norm_scale(ctypes.byref(s), min(a.chunks, 2 * NORM_GRID), stream), "rx_norm_scale")
     torch.autograd.graph.increment_version(grads)
     return norm
 
@@ -464,6 +465,8 @@ class FusedAdamW(torch.optim.Optimizer):
         npart = _launch_norm(L, launches, ws["part_at"], stream) if launches else 0
         if clip is not None:
             self.grad_norm = torch.empty((), dtype=torch.float32, device=dev)
+        # parameter, gradient and two moments
+        touched = sum(p.numel() * (2 * p.element_size() + group["state_bits"] // 4) for group, live in groups for p, _, _ in live)
         done, owners, first = [], [], 0
         for k, (group, live) in enumerate(groups):
             bits, lr = group["state_bits"], group["lr"]
@@ -523,7 +526,7 @@ class FusedAdamW(torch.optim.Optimizer):
                         if img is not None:
                             a.img[j] = img.data_ptr()
                             owners.append((tower, li))
-                _hip.check(L.rx_aw_step(ctypes.byref(a), bits, int(low), stream), "rx_aw_step")
+                _hip.check(L.rx_aw_step(ctypes.byref(a), bits, int(low), int(touched > LAST_LEVEL), stream), "rx_aw_step")
                 done += [p for p, _, _ in part]
                 at = end
             first += len(live)

@@ -25,6 +25,7 @@ MAX_EXPERTS, MAX_TOPK = 1024, 32
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _VEC = {0: 4, 1: 8, 2: 8}          # elements of a 16-byte vector
 _INT32 = 0x7FFFFFFF
+LAST_LEVEL = 256 << 20          # bytes of the last-level cache
 
 
 class PlanArgs(ctypes.Structure):
@@ -36,7 +37,7 @@ class PlanArgs(ctypes.Structure):
 
 class RowArgs(ctypes.Structure):
     _fields_ = [("T", ctypes.c_longlong), ("rows", ctypes.c_longlong), ("ldx", ctypes.c_longlong), ("k", ctypes.c_int),
-                ("D", ctypes.c_int), ("lg", ctypes.c_int), ("pad_", ctypes.c_int), ("position", ctypes.c_void_p),
+                ("D", ctypes.c_int), ("lg", ctypes.c_int), ("stream", ctypes.c_int), ("position", ctypes.c_void_p),
                 ("source", ctypes.c_void_p), ("x", ctypes.c_void_p), ("w", ctypes.c_void_p), ("h", ctypes.c_void_p),
                 ("out", ctypes.c_void_p), ("dw", ctypes.c_void_p)]
 
@@ -241,8 +242,10 @@ def _plan_cpu(experts, E, C, rows):
 def _row_args(plan, D, dtype, x=None, ldx=0, w=None, h=None, out=None, dw=None):
     code = _DTYPES[dtype]
     units = -(-D // _VEC[code])
-    a = RowArgs(plan.tokens, plan.rows, ldx, plan.k, D, min(6, (units - 1).bit_length()), 0, plan.position.data_ptr(),
-                plan.source.data_ptr())
+    # samples' rows and expert rows, these twice where products are taken: more than the last-level cache is streamed past it
+    touched = (plan.tokens + plan.rows * (2 if dw is not None else 1)) * D * dtype.itemsize
+    a = RowArgs(plan.tokens, plan.rows, ldx, plan.k, D, min(6, (units - 1).bit_length()), int(touched > LAST_LEVEL),
+                plan.position.data_ptr(), plan.source.data_ptr())
     a.x, a.w, a.h, a.out, a.dw = (t.data_ptr() if t is not None else None for t in (x, w, h, out, dw))
     return a, code
 
