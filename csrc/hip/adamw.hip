@@ -17,14 +17,12 @@
 // e is the exponent of the block's maximum once that is rounded up to 3 mantissa bits, so no rounding overflows. A byte
 // of 255 marks a block whose values are not finite: it decodes to NaN, as fp32 moments would show it.
 // m and v are computed as separately rounded products and sums: any IEEE fp32 implementation gets the same codes.
+#include "adamw.h"
 #include "rx_common.h"
 
 namespace {
 
-constexpr int kAwMax = 64;      // tensors in one step launch (kernel arguments under 4 KiB)
-constexpr int kPrepMax = 256;   // tensors in one preparation launch (one thread each)
-constexpr int kNormMax = 128;   // tensors in one norm / scale launch
-constexpr int kBlk = 256;       // elements that share a scale: 4 per lane of one wave
+constexpr int kBlk = kAwBlock;
 
 // dither: 2^32 / golden ratio and the fractional bits of sqrt(2), sqrt(3) as odd multipliers
 constexpr uint32_t kPhi = 0x9E3779B1u, kSq2 = 0x6A09E667u, kSq3 = 0xBB67AE85u;
@@ -34,63 +32,6 @@ __device__ __forceinline__ uint32_t aw_mix(uint32_t x) {
   x = (x ^ (x >> 15)) * kSq3;
   return x ^ (x >> 16);
 }
-
-struct AwHead {      // one per launch group of a step
-  float gscale;      // what gradients are multiplied with (clip factor, -1 to maximize)
-  int skip;          // 1: the norm is not finite, the step is left out
-};
-
-struct AwTensor {    // what one step has in common for a tensor
-  float nlr_bc1;     // -lr / (1 - b1^t)
-  float decay;       // 1 - lr wd
-  float rs_bc2;      // 1 / sqrt(1 - b2^t)
-  uint32_t key;      // of its dither in this step
-};
-
-struct AwPrep {
-  int n, maximize, npart, first;   // first: index of this launch's first tensor in tensors[]
-  double lr, wd, b1, b2, max_norm; // max_norm < 0: no clipping
-  const float* lr_dev;             // not null: the learning rate, on the device
-  const double* part;              // npart partial sums of squared gradients
-  AwHead* head;
-  AwTensor* tensors;
-  float* norm;                     // not null: where the norm goes
-  uint32_t seed, pad_;
-  float* step[kPrepMax];           // the tensors' step words
-  int ordinal[kPrepMax];           // their places in the optimizer
-};
-
-struct AwStep {
-  int n, pad_;
-  float b1, omb1, b2, omb2, eps, pad2_;
-  const AwHead* head;
-  const AwTensor* tensors;         // of this launch's first tensor
-  void* p[kAwMax];
-  const void* g[kAwMax];
-  void* m[kAwMax];
-  void* v[kAwMax];
-  uint8_t* sc[kAwMax];             // [blocks][2] scale bytes (8-bit moments)
-  u16* img[kAwMax];                // bf16 image of an fp32 p (null: none)
-  long long len[kAwMax];
-  unsigned start[kAwMax + 1];      // first chunk of each tensor
-};
-
-struct NormArgs {
-  int n, bf16_mask_;
-  double* part;                    // one partial sum per workgroup
-  unsigned chunks, pad_;
-  const void* g[kNormMax];
-  long long len[kNormMax];
-  unsigned start[kNormMax + 1];
-  unsigned char bf16[kNormMax];
-};
-
-struct ScaleArgs {
-  NormArgs t;                      // t.part: the partial sums to finish
-  int npart, pad_;
-  double max_norm;
-  float* norm;
-};
 
 // the tensor that a chunk belongs to: start[] is ascending, wave-uniform
 template <class A>
@@ -247,8 +188,7 @@ __device__ __forceinline__ void aw_decode4(uint32_t mc, uint32_t vc, int sm, int
   v[3] = aw_dec_v<3>(vc, ev);
 }
 
-constexpr int kStepUnroll = 2;                        // scale blocks of a wave that are in flight together
-constexpr int kStepChunk = 4 * kBlk * kStepUnroll;    // elements per workgroup of 4 waves
+constexpr int kStepUnroll = kAwChunk / (4 * kBlk);    // scale blocks of a wave that are in flight together
 
 struct AwPlace {       // where a launch's workgroup works (wave-uniform)
   void* p;
@@ -422,8 +362,6 @@ __global__ __launch_bounds__(256) void aw_prep_kernel(AwPrep a) {
 }
 
 // Sums of squares in 64 bits: the norm then does not depend on the order of the sum in any of its 32 bits but by chance.
-constexpr int kNormChunk = 8192;
-
 // 4 x 4 (bf16: 2 x 8) elements of a lane, in flight together
 template <bool BF16, bool FULL>
 __device__ __forceinline__ double aw_squares(const void* g, long long i, long long n) {
@@ -566,26 +504,15 @@ __global__ __launch_bounds__(256) void aw_decode_kernel(const uint8_t* __restric
 
 extern "C" {
 
-void rx_aw_sizes(int* out) {   // struct sizes and limits that raydp_amd/ops/fused_optim.py mirrors
-  out[0] = (int)sizeof(AwPrep);
-  out[1] = (int)sizeof(AwStep);
-  out[2] = (int)sizeof(NormArgs);
-  out[3] = (int)sizeof(ScaleArgs);
-  out[4] = kAwMax;
-  out[5] = kPrepMax;
-  out[6] = kNormMax;
-  out[7] = kStepChunk;
-  out[8] = kNormChunk;
-}
-
-int rx_aw_prep(const AwPrep* a, hipStream_t stream) {
-  if (a->n < 0 || a->n > kPrepMax) return -1;
+int rx_aw_prep(const AwPrep* a, void* on) {
+  hipStream_t stream = static_cast<hipStream_t>(on);
+  if (a->n < 0 || a->n > kAwPrepMax) return -1;
   hipLaunchKernelGGL(aw_prep_kernel, dim3(1), dim3(256), 0, stream, *a);
   return (int)hipGetLastError();
 }
 
-// stream_past: the step's working set is larger than the last-level cache
-int rx_aw_step(const AwStep* a, int bits, int bf16, int stream_past, hipStream_t stream) {
+int rx_aw_step(const AwStep* a, int bits, int bf16, int stream_past, void* on) {
+  hipStream_t stream = static_cast<hipStream_t>(on);
   if (a->n <= 0 || a->n > kAwMax || (bits != 8 && bits != 32)) return -1;
   const unsigned grid = a->start[a->n];
   if (grid == 0) return 0;
@@ -603,21 +530,23 @@ int rx_aw_step(const AwStep* a, int bits, int bf16, int stream_past, hipStream_t
   return (int)hipGetLastError();
 }
 
-// grid: workgroups, one partial sum each
-int rx_norm_part(const NormArgs* a, int grid, hipStream_t stream) {
+int rx_norm_part(const NormArgs* a, int grid, void* on) {
+  hipStream_t stream = static_cast<hipStream_t>(on);
   if (a->n <= 0 || a->n > kNormMax || grid <= 0) return -1;
   hipLaunchKernelGGL(norm_part_kernel, dim3((unsigned)grid), dim3(256), 0, stream, *a);
   return (int)hipGetLastError();
 }
 
-int rx_norm_scale(const ScaleArgs* a, int grid, hipStream_t stream) {
+int rx_norm_scale(const ScaleArgs* a, int grid, void* on) {
+  hipStream_t stream = static_cast<hipStream_t>(on);
   if (a->t.n <= 0 || a->t.n > kNormMax || grid <= 0) return -1;
   hipLaunchKernelGGL(norm_scale_kernel, dim3((unsigned)grid), dim3(256), 0, stream, *a);
   return (int)hipGetLastError();
 }
 
 int rx_aw_decode(const uint8_t* m, const uint8_t* v, const uint8_t* sc, void* mo, void* vo, long long n, int bf16,
-                 hipStream_t stream) {
+                 void* on) {
+  hipStream_t stream = static_cast<hipStream_t>(on);
   if (n <= 0) return 0;
   const long long grid = (n + 4 * kDecUnroll * kBlk - 1) / (4 * kDecUnroll * kBlk);
   if (grid > 0x7FFFFFFFll) return -1;

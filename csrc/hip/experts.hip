@@ -10,6 +10,7 @@
 //
 // scatter and gather are each other's gradients; every kernel works sample by sample, so that x, dy and y cross memory
 // once, the sums of a sample are one lane group's in a fixed order, and nothing needs atomics on floats.
+#include "experts.h"
 #include "rx_common.h"
 
 namespace {
@@ -77,8 +78,6 @@ struct Vec {
 //                  winner and so puts those above the ones taken: max over (key - last), two keys per v_max3.
 //   fp32 logits:   (order-preserving 32 bits, 0xFFFF - index) as a positive double: v_max_f64 runs at the rate of fp32, two
 //                  words a key; a winner is struck out by its low word.
-constexpr int kRouteMaxK = 32;
-
 // order-preserving unsigned images of the logits' bits (not of NaN and -0: the callers replace them)
 __device__ __forceinline__ uint32_t order16(uint32_t b) { return (b & 0x8000u) ? b ^ 0xFFFFu : b | 0x8000u; }
 __device__ __forceinline__ uint32_t order32(uint32_t b) { return (b & 0x80000000u) ? ~b : b | 0x80000000u; }
@@ -289,8 +288,7 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(const typename Elem<DT>:
 }
 
 // ------------------------------------------------------------------------------------------------ plan
-constexpr int kPlanWaves = 16, kPlanThreads = 64 * kPlanWaves;
-constexpr int kMaxExperts = 1024;
+constexpr int kPlanWaves = kPlanThreads / 64;
 
 __device__ __forceinline__ int plan_expert(const void* ids, int wide, long long i, int E) {
   const long long e = wide ? ((const long long*)ids)[i] : (long long)((const int*)ids)[i];
@@ -311,16 +309,6 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const void* __
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += kPlanThreads) counts[(long long)blockIdx.x * E + e] = hist[e];
 }
-
-struct PlanArgs {
-  const void* ids;
-  int wide, n, E, chunk, blocks, capacity, rows, pad_;
-  const int* counts;    // [blocks][E] (null with one block)
-  int* position;        // [n]
-  int* source;          // [rows]
-  int* load;            // [E]
-  int* offsets;         // [E + 1]
-};
 
 // Stable ranks. A workgroup's waves own consecutive pieces of its chunk; a wave takes 64 choices at a time, finds the
 // lanes with the same expert by one ballot per bit of the expert's number, and counts on in LDS.
@@ -421,18 +409,6 @@ __global__ __launch_bounds__(kPlanThreads) void plan_rank_kernel(PlanArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ rows
-struct RowArgs {
-  long long T, rows, ldx;     // samples, expert rows, elements between samples' rows (x)
-  int k, D, lg, stream;       // lg: log2 of the lanes that work on a sample; stream: rows go past the caches
-  const int* position;        // [T][k]
-  const int* source;          // [rows]
-  const void* x;              // scatter: samples' rows in; gather: not used
-  const float* w;             // [T][k] or null
-  const void* h;              // scatter: expert rows to take products with, or null; gather: expert rows in
-  void* out;                  // scatter: expert rows out; gather: samples' rows out
-  float* dw;                  // scatter with h: [T][k]
-};
-
 constexpr int kTogether = 4;   // expert rows of a sample that are in flight together
 constexpr int kLook = 16;      // expert rows that a wave looks at for empty ones
 
@@ -609,16 +585,9 @@ int route_pick(int bwd, const void* z, long long ldz, const float* norm, float* 
 
 extern "C" {
 
-void rx_expert_sizes(int* out) {   // mirrored by raydp_amd/ops/expert_ops.py
-  out[0] = (int)sizeof(PlanArgs);
-  out[1] = (int)sizeof(RowArgs);
-  out[2] = kMaxExperts;
-  out[3] = kRouteMaxK;
-}
-
-// dtype: 0 fp32, 1 bf16, 2 fp16. norm: [T][2] peak and 1 / sum, written when not null
 int rx_route_fwd(const void* z, long long ldz, int dtype, long long T, int E, int k, int renorm, float* w, int* ids,
-                 float* norm, hipStream_t stream) {
+                 float* norm, void* on) {
+  hipStream_t stream = static_cast<hipStream_t>(on);
   if (T < 0 || E <= 0 || E > kMaxExperts || k <= 0 || k > kRouteMaxK || k > E) return -1;
   if (T == 0) return 0;
   if (dtype == 0) return route_pick<0>(0, z, ldz, nullptr, w, ids, nullptr, T, E, k, renorm, norm, nullptr, stream);
@@ -627,9 +596,9 @@ int rx_route_fwd(const void* z, long long ldz, int dtype, long long T, int E, in
   return -1;
 }
 
-// norm null: softmax over the chosen ones (z is not read)
 int rx_route_bwd(const void* z, long long ldz, int dtype, const float* norm, const float* w, const int* ids,
-                 const float* dw, long long T, int E, int k, void* dz, hipStream_t stream) {
+                 const float* dw, long long T, int E, int k, void* dz, void* on) {
+  hipStream_t stream = static_cast<hipStream_t>(on);
   if (T < 0 || E <= 0 || E > kMaxExperts || k <= 0 || k > kRouteMaxK || k > E) return -1;
   if (T == 0) return 0;
   float* wm = const_cast<float*>(w);
@@ -640,8 +609,8 @@ int rx_route_bwd(const void* z, long long ldz, int dtype, const float* norm, con
   return -1;
 }
 
-// counts: blocks * E ints of scratch (not read or written with one block)
-int rx_expert_plan(const PlanArgs* a, int* counts, hipStream_t stream) {
+int rx_expert_plan(const PlanArgs* a, int* counts, void* on) {
+  hipStream_t stream = static_cast<hipStream_t>(on);
   if (a->E <= 0 || a->E > kMaxExperts || a->n < 0 || a->blocks < 1 || a->chunk <= 0 || a->chunk % kPlanThreads ||
       (long long)a->blocks * a->chunk < a->n || (a->blocks > 1 && counts == nullptr))
     return -1;
@@ -660,7 +629,8 @@ int rx_expert_plan(const PlanArgs* a, int* counts, hipStream_t stream) {
   return (int)hipGetLastError();
 }
 
-int rx_rows_scatter(const RowArgs* a, int dtype, hipStream_t stream) {
+int rx_rows_scatter(const RowArgs* a, int dtype, void* on) {
+  hipStream_t stream = static_cast<hipStream_t>(on);
   if (a->T < 0 || a->rows < 0 || a->k <= 0 || a->D <= 0 || a->lg < 0 || a->lg > 6 || dtype < 0 || dtype > 2) return -1;
   // (without samples only rows are zeroed)
   const bool weighted = a->T > 0 && a->w != nullptr, products = a->T > 0 && a->h != nullptr;
@@ -694,7 +664,8 @@ int rx_rows_scatter(const RowArgs* a, int dtype, hipStream_t stream) {
   return (int)hipGetLastError();
 }
 
-int rx_rows_gather(const RowArgs* a, int dtype, hipStream_t stream) {
+int rx_rows_gather(const RowArgs* a, int dtype, void* on) {
+  hipStream_t stream = static_cast<hipStream_t>(on);
   if (a->T < 0 || a->k <= 0 || a->D <= 0 || a->lg < 0 || a->lg > 6 || dtype < 0 || dtype > 2) return -1;
   const long long grid = (a->T + (256 >> a->lg) - 1) >> (8 - a->lg);
   if (grid == 0) return 0;

@@ -3,6 +3,7 @@
 * ``libexec_kernels.so``  — CPU shuffle/hash kernels (g++).
 * ``libraydp_runtime.so`` — shared-memory object store + actor supervisor + framed IPC (g++).
 * ``libhipkernels.so``    — CDNA4 HIP kernels for gfx950 (hipcc ``--offload-arch=gfx950``).
+* ``raydp_torch.so``      — extension module over torch's C++ API: autograd nodes and tensor lists of some of them (g++).
 * ``raydp_supervisor`` / ``raydp_appmaster`` / ``raydp_shuffle_service`` — native services (g++).
 
 ``build_sanitized("asan"|"tsan", dir)`` builds the host-side services and the runtime stress
@@ -55,6 +56,8 @@ LIBS = {
                                             os.path.join(CSRC, "exec", "expr", "expr_vm.cc")],
                            libs=["-L", HERE, "-lraydp_runtime", "-Wl,-rpath,$ORIGIN", "-lpthread"]),
     "hipkernels": dict(kind="hip", sources=_hip_sources),
+    # torch front end (autograd nodes, tensor lists) of the optimizer and expert kernels
+    "raydp_torch": dict(kind="torch", sources=lambda: [os.path.join(CSRC, "torch", "raydp_torch.cc")]),
     # executables: the per-node actor supervisor, the application master (native control
     # plane) and the per-node external shuffle-block service
     "raydp_supervisor": dict(kind="exe", sources=lambda: [os.path.join(CSRC, "runtime", "supervisor.cc")]),
@@ -75,8 +78,23 @@ def _arrow_flags():
     return ["-I", pa.get_include(), "-L", libdir, f"-l:{so[0]}", f"-Wl,-rpath,{libdir}"]
 
 
+def _torch_flags():
+    """Compile/link flags for an extension module against this interpreter's torch and libhipkernels."""
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_path("include"), os.path.join(ROCM, "include")]
+    lib = os.path.join(root, "lib")
+    return [f"-I{d}" for d in inc] + [
+        "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        "-L", lib, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python", f"-Wl,-rpath,{lib}",
+        "-L", HERE, "-lhipkernels", "-Wl,-rpath,$ORIGIN"]
+
+
 def out_path(name: str) -> str:
-    return os.path.join(HERE, name if LIBS[name]["kind"] == "exe" else f"lib{name}.so")
+    kind = LIBS[name]["kind"]
+    return os.path.join(HERE, name if kind == "exe" else f"{name}.so" if kind == "torch" else f"lib{name}.so")
 
 
 def _run(cmd):
@@ -109,6 +127,9 @@ def build_one(name: str, force: bool = False) -> str:
     if spec["kind"] == "exe":
         cxx = shutil.which("g++") or "c++"
         _run([cxx, "-O2", "-std=c++17", "-Wall"] + inc + srcs + ["-o", tmp])
+    elif spec["kind"] == "torch":
+        cxx = shutil.which("g++") or "c++"
+        _run([cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden"] + inc + srcs + ["-o", tmp] + _torch_flags())
     elif spec["kind"] == "cpu":
         cxx = shutil.which("g++") or "c++"
         extra = _arrow_flags() if spec.get("arrow") else []

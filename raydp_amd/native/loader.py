@@ -36,6 +36,27 @@ def load(name: str, build_if_missing: bool = True):
         return lib
 
 
+def load_torch():
+    """The extension module over torch's C++ API (``raydp_torch.so``); the HIP kernels it calls are loaded first."""
+    mod = _loaded.get("raydp_torch")
+    if mod is not None:
+        return mod
+    from raydp_amd.ops import _hip
+    _hip.lib()
+    path = os.path.join(HERE, "raydp_torch.so")
+    with _lock:
+        if "raydp_torch" not in _loaded:
+            if not os.path.exists(path):
+                from raydp_amd.native import build
+                build.build_one("raydp_torch")
+            import importlib.util
+            spec = importlib.util.spec_from_file_location("raydp_torch", path)
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+            _loaded["raydp_torch"] = mod
+        return _loaded["raydp_torch"]
+
+
 def executable(name: str, build_if_missing: bool = True) -> str:
     """Path of an in-tree native executable (built on first use).
 

@@ -14,95 +14,25 @@
 
 On the CPU the same operators are computed by torch expressions with the same codes.
 """
-import contextlib
-import ctypes
 import math
 from typing import Iterable, Optional, Tuple, Union
 
 import torch
 
-from raydp_amd.ops import _hip
-
 BLOCK = 256                  # elements of a tensor that share a scale
-AW_MAX, PREP_MAX, NORM_MAX = 64, 256, 128
-STEP_CHUNK, NORM_CHUNK = 2048, 8192
-NORM_GRID = 1024             # partial sums of one norm launch at most
-LAST_LEVEL = 256 << 20       # bytes of the last-level cache: steps that touch more are streamed past it
 _M_EMIN, _V_EMIN = -14, -30
 _MASK, _PHI, _SQ2, _SQ3 = 0xFFFFFFFF, 0x9E3779B1, 0x6A09E667, 0xBB67AE85
 
 
-class AwPrep(ctypes.Structure):
-    _fields_ = [("n", ctypes.c_int), ("maximize", ctypes.c_int), ("npart", ctypes.c_int), ("first", ctypes.c_int),
-                ("lr", ctypes.c_double), ("wd", ctypes.c_double), ("b1", ctypes.c_double), ("b2", ctypes.c_double),
-                ("max_norm", ctypes.c_double), ("lr_dev", ctypes.c_void_p), ("part", ctypes.c_void_p),
-                ("head", ctypes.c_void_p), ("tensors", ctypes.c_void_p), ("norm", ctypes.c_void_p),
-                ("seed", ctypes.c_uint32), ("pad_", ctypes.c_uint32), ("step", ctypes.c_void_p * PREP_MAX),
-                ("ordinal", ctypes.c_int * PREP_MAX)]
+_module = None
 
 
-class AwStep(ctypes.Structure):
-    _fields_ = [("n", ctypes.c_int), ("pad_", ctypes.c_int), ("b1", ctypes.c_float), ("omb1", ctypes.c_float),
-                ("b2", ctypes.c_float), ("omb2", ctypes.c_float), ("eps", ctypes.c_float), ("pad2_", ctypes.c_float),
-                ("head", ctypes.c_void_p), ("tensors", ctypes.c_void_p), ("p", ctypes.c_void_p * AW_MAX),
-                ("g", ctypes.c_void_p * AW_MAX), ("m", ctypes.c_void_p * AW_MAX), ("v", ctypes.c_void_p * AW_MAX),
-                ("sc", ctypes.c_void_p * AW_MAX), ("img", ctypes.c_void_p * AW_MAX),
-                ("len", ctypes.c_longlong * AW_MAX), ("start", ctypes.c_uint * (AW_MAX + 1))]
-
-
-class NormArgs(ctypes.Structure):
-    _fields_ = [("n", ctypes.c_int), ("pad0_", ctypes.c_int), ("part", ctypes.c_void_p), ("chunks", ctypes.c_uint),
-                ("pad_", ctypes.c_uint), ("g", ctypes.c_void_p * NORM_MAX), ("len", ctypes.c_longlong * NORM_MAX),
-                ("start", ctypes.c_uint * (NORM_MAX + 1)), ("bf16", ctypes.c_ubyte * NORM_MAX)]
-
-
-class ScaleArgs(ctypes.Structure):
-    _fields_ = [("t", NormArgs), ("npart", ctypes.c_int), ("pad_", ctypes.c_int), ("max_norm", ctypes.c_double),
-                ("norm", ctypes.c_void_p)]
-
-
-_bound = None
-
-
-def _lib():
-    global _bound
-    L = _hip.lib()
-    if _bound is not L:
-        vp, i, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
-        L.rx_aw_prep.argtypes = [vp, vp]
-        L.rx_aw_step.argtypes = [vp, i, i, i, vp]
-        L.rx_norm_part.argtypes = [vp, i, vp]
-        L.rx_norm_scale.argtypes = [vp, i, vp]
-        L.rx_aw_decode.argtypes = [vp, vp, vp, vp, vp, ll, i, vp]
-        for n in ("rx_aw_prep", "rx_aw_step", "rx_norm_part", "rx_norm_scale", "rx_aw_decode"):
-            getattr(L, n).restype = i
-        L.rx_aw_sizes.argtypes = [vp]
-        L.rx_aw_sizes.restype = None
-        got = (ctypes.c_int * 9)()
-        L.rx_aw_sizes(got)
-        want = [ctypes.sizeof(c) for c in (AwPrep, AwStep, NormArgs, ScaleArgs)] + \
-            [AW_MAX, PREP_MAX, NORM_MAX, STEP_CHUNK, NORM_CHUNK]
-        if list(got) != want:
-            raise RuntimeError(f"layout mismatch between Python and csrc/hip/adamw.hip: C {list(got)} vs {want}")
-        _bound = L
-    return L
-
-
-def _on(device):
-    """The device whose stream a launch goes to, made current where it is not."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _dense(t: torch.Tensor) -> bool:
-    """Every element once, without gaps, in whatever order."""
-    if t.is_contiguous():
-        return True
-    need = 1
-    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda v: v[1]):
-        if stride != need:
-            return False
-        need *= size
-    return True
+def _ext():
+    global _module
+    if _module is None:
+        from raydp_amd.native import loader
+        _module = loader.load_torch()
+    return _module
 
 
 # --------------------------------------------------------------------------------------- moments in 8 bits
@@ -180,48 +110,12 @@ def decode_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, scales: torc
         m = _decode(mc & 127, s[:, 0], _M_EMIN) * (1 - (mc >> 7) * 2)
         v = _decode(vc, s[:, 1], _V_EMIN)
         return tuple(t.view(-1)[:n].view(exp_avg.shape).to(dtype) for t in (m, v))
-    if (exp_avg.data_ptr() | exp_avg_sq.data_ptr()) & 3:
-        raise ValueError("decode_moments: moments must start at a multiple of 4 bytes")
-    m, v = torch.empty_like(exp_avg, dtype=dtype), torch.empty_like(exp_avg_sq, dtype=dtype)
-    if n:
-        with _on(m.device):
-            _hip.check(_lib().rx_aw_decode(exp_avg.data_ptr(), exp_avg_sq.data_ptr(), scales.data_ptr(), m.data_ptr(),
-                                           v.data_ptr(), n, int(dtype == torch.bfloat16), _hip.stream_ptr(m.device)),
-                       "rx_aw_decode")
-    return m, v
+    if (exp_avg.data_ptr() | exp_avg_sq.data_ptr()) & 3 or scales.data_ptr() & 1:
+        raise ValueError("decode_moments: moments must start at a multiple of 4 bytes, scales at an even address")
+    return tuple(_ext().decode_moments(exp_avg, exp_avg_sq, scales, dtype == torch.bfloat16))
 
 
 # --------------------------------------------------------------------------------------- norm and clipping
-def _norm_launches(grads):
-    """[(NormArgs, grid)] over ``grads`` (dense fp32 / bf16 tensors), ``part`` still to be filled in."""
-    out = []
-    for k in range(0, len(grads), NORM_MAX):
-        chunk = grads[k:k + NORM_MAX]
-        a, n = NormArgs(), len(chunk)
-        lens = [g.numel() for g in chunk]
-        starts = [0]
-        for ln in lens:
-            starts.append(starts[-1] + -(-ln // NORM_CHUNK))
-        if starts[-1] > _MASK:
-            raise ValueError("gradient norm: too many elements for one launch")
-        a.n, a.chunks = n, starts[-1]
-        a.g[:n] = [g.data_ptr() for g in chunk]
-        a.len[:n], a.start[:n + 1] = lens, starts
-        a.bf16[:n] = [g.dtype == torch.bfloat16 for g in chunk]
-        out.append((a, min(starts[-1], NORM_GRID)))
-    return out
-
-
-def _launch_norm(L, launches, part_ptr, stream):
-    """Partial sums of squares to ``part_ptr`` on; returns how many."""
-    at = 0
-    for a, grid in launches:
-        a.part = part_ptr + 8 * at
-        _hip.check(L.rx_norm_part(ctypes.byref(a), grid, stream), "rx_norm_part")
-        at += grid
-    return at
-
-
 @torch.no_grad()
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float) -> torch.Tensor:
     """Scale the gradients of ``parameters`` in place by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` their global
@@ -234,46 +128,35 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
         raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm}")
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    seen, grads = set(), []
-    for p in parameters:
-        if p.grad is not None and id(p) not in seen:
-            seen.add(id(p))
-            grads.append(p.grad)
+    grads = [g for g in (p.grad for p in {id(p): p for p in parameters}.values()) if g is not None]
     if not grads:
         return torch.zeros(())
-    dev = grads[0].device
+    if grads[0].is_cuda:
+        return _ext().clip_grad_norm(grads, max_norm)
     for g in grads:
         if g.layout != torch.strided:
             raise ValueError("clip_grad_norm_: sparse gradients are not supported")
-        if g.device != dev:
-            raise ValueError(f"clip_grad_norm_: gradients on {dev} and {g.device}")
+        if g.device != grads[0].device:
+            raise ValueError(f"clip_grad_norm_: gradients on {grads[0].device} and {g.device}")
         if g.dtype not in (torch.float32, torch.bfloat16):
             raise TypeError(f"clip_grad_norm_: gradient dtype {g.dtype} (fp32 or bf16)")
         if not _dense(g):
             raise ValueError("clip_grad_norm_: gradients must be dense (no gaps, no broadcast dimensions)")
-    if dev.type != "cuda":
-        norm = torch.sqrt(sum(g.double().square().sum() for g in grads))
-        f = (max_norm / (norm + 1e-6)).clamp(max=1.0).float()
-        for g in grads:
-            g.copy_(g.float() * f)
-        return norm.float()
-    grads = [g for g in grads if g.numel()]
-    if not grads:
-        return torch.zeros((), device=dev)
-    L = _lib()
-    with _on(dev):
-        stream = _hip.stream_ptr(dev)
-        launches = _norm_launches(grads)
-        part = torch.empty(sum(grid for _, grid in launches), dtype=torch.float64, device=dev)
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        npart = _launch_norm(L, launches, part.data_ptr(), stream)
-        for k, (a, grid) in enumerate(launches):
-            s = ScaleArgs()
-            s.t, s.npart, s.max_norm = a, npart, max_norm
-            s.t.part, s.norm = part.data_ptr(), norm.data_ptr() if k == 0 else None
-            _hip.check(L.rx_norm_scale(ctypes.byref(s), min(a.chunks, 2 * NORM_GRID), stream), "rx_norm_scale")
-    torch.autograd.graph.increment_version(grads)
-    return norm
+    norm = torch.sqrt(sum(g.double().square().sum() for g in grads))
+    f = (max_norm / (norm + 1e-6)).clamp(max=1.0).float()
+    for g in grads:
+        g.copy_(g.float() * f)
+    return norm.float()
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Every element once, without gaps, in whatever order."""
+    need = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda v: v[1]):
+        if stride != need:
+            return False
+        need *= size
+    return True
 
 
 # --------------------------------------------------------------------------------------- the optimizer
@@ -293,8 +176,8 @@ class FusedAdamW(torch.optim.Optimizer):
     fp32) and, for 8 bits, ``scales`` (uint8 ``[ceil(n / 256), 2]``); :func:`decode_moments` gives their values.
     ``load_state_dict`` also takes the state of a ``torch.optim.AdamW`` and codes its moments.
 
-    Parameters are contiguous fp32 or bf16; gradients are dense and of the parameter's type. Sparse gradients, closures
-    inside a graph capture and a first step inside a capture raise."""
+    Parameters are contiguous fp32 or bf16; gradients are dense and of the parameter's type. Sparse gradients, a first
+    step inside a graph capture raise."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                  state_bits: int = 8, max_grad_norm: Optional[float] = None, maximize: bool = False, seed: int = 0):
@@ -320,13 +203,11 @@ class FusedAdamW(torch.optim.Optimizer):
                                       max_grad_norm=None if max_grad_norm is None else float(max_grad_norm),
                                       maximize=bool(maximize), seed=int(seed)))
         self.grad_norm: Optional[torch.Tensor] = None
-        self._ws = None
 
     def __setstate__(self, state):
         super().__setstate__(state)
         self._fill_groups()
         self.__dict__.setdefault("grad_norm", None)
-        self.__dict__["_ws"] = None
 
     def _fill_groups(self):
         for g in self.param_groups:      # (a state dict of torch.optim.AdamW has fewer options)
@@ -378,176 +259,98 @@ class FusedAdamW(torch.optim.Optimizer):
                 st.update(exp_avg=m, exp_avg_sq=v)
             self.state[p] = st
 
-    def _state_of(self, p, bits):
+    def _new_state(self, p, bits):
         """The parameter's state, made with its first gradient."""
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW: the first step of a parameter cannot be captured into a graph (its state "
+                               "would be zeroed by every replay): run one eager step first")
+        if not p.is_contiguous():
+            raise ValueError("FusedAdamW: parameters must be contiguous")
         st = self.state[p]
-        if not st:
-            if p.is_cuda and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("FusedAdamW: the first step of a parameter cannot be captured into a graph (its state "
-                                   "would be zeroed by every replay): run one eager step first")
-            st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
-            kind = torch.uint8 if bits == 8 else torch.float32
-            for n in ("exp_avg", "exp_avg_sq"):
-                st[n] = torch.zeros(p.shape, dtype=kind, device=p.device)
-            if bits == 8:
-                st["scales"] = torch.zeros(_scale_rows(p.numel()), 2, dtype=torch.uint8, device=p.device)
-            return st
-        if st["step"].device != p.device:      # (state loaded before the model was moved)
-            for n, t in st.items():
-                st[n] = t.to(p.device)
-        if (st["exp_avg"].dtype == torch.uint8) != (bits == 8):
-            raise ValueError(f"FusedAdamW: state_bits is {bits}, the moments of a parameter are {st['exp_avg'].dtype}")
+        st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+        kind = torch.uint8 if bits == 8 else torch.float32
+        for n in ("exp_avg", "exp_avg_sq"):
+            st[n] = torch.zeros(p.shape, dtype=kind, device=p.device)
+        if bits == 8:
+            st["scales"] = torch.zeros(_scale_rows(p.numel()), 2, dtype=torch.uint8, device=p.device)
         return st
-
-    def _live(self):
-        """[(group, [(parameter, gradient, place)])] with gradients, checked."""
-        out, place, dev = [], 0, None
-        for group in self.param_groups:
-            live = []
-            for p in group["params"]:
-                g = p.grad
-                if g is not None:
-                    if g.layout != torch.strided:
-                        raise RuntimeError("FusedAdamW does not support sparse gradients")
-                    if dev is None:
-                        dev = p.device
-                    if p.device != dev:
-                        raise ValueError(f"FusedAdamW: parameters with gradients on {dev} and {p.device}")
-                    if p.dtype not in (torch.float32, torch.bfloat16) or g.dtype != p.dtype:
-                        raise TypeError(f"FusedAdamW: parameter {p.dtype} with gradient {g.dtype} (both fp32 or both bf16)")
-                    if not p.is_contiguous():
-                        raise ValueError("FusedAdamW: parameters must be contiguous")
-                    if p.numel():
-                        live.append((p, g if g.is_contiguous() else g.contiguous(), place))
-                place += 1
-            if live:
-                out.append((group, live))
-        if out and any(g["max_grad_norm"] != out[0][0]["max_grad_norm"] or g["seed"] != out[0][0]["seed"] for g, _ in out):
-            raise ValueError("FusedAdamW: max_grad_norm and seed are the optimizer's, not a group's")
-        return out, dev
 
     @torch.no_grad()
     def step(self, closure=None):
+        from raydp_amd.ops.fused_optim import _image_of
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        groups, dev = self._live()
-        if groups:
-            if dev.type == "cuda":
-                with _on(dev):
-                    self._gpu_step(groups, dev)
-            else:
-                self._cpu_step(groups)
+        groups, owners, place, first = [], [], 0, None
+        for group in self.param_groups:
+            params, grads, places, images = [], [], [], {}
+            for o, p in enumerate(group["params"], place):
+                g = p.grad
+                if g is None:
+                    continue
+                if getattr(p, "_raydp_image_owner", None) is not None and p.is_cuda:
+                    tower, li, img = _image_of(p)
+                    if img is not None:
+                        images[len(params)] = img
+                        owners.append((tower, li))
+                params.append(p)
+                grads.append(g)
+                places.append(o)
+            place += len(group["params"])
+            if params:
+                if first is None:
+                    first = group
+                elif group["max_grad_norm"] != first["max_grad_norm"] or group["seed"] != first["seed"]:
+                    raise ValueError("FusedAdamW: max_grad_norm and seed are the optimizer's, not a group's")
+                groups.append((params, grads, places, images, group))
+        if not groups:
+            return loss
+        for _, grads, _, _, _ in groups:
+            if any(g.layout is not torch.strided for g in grads):
+                raise RuntimeError("FusedAdamW does not support sparse gradients")
+        state, clip = self.state, first["max_grad_norm"]
+        steps = []
+        for params, grads, places, images, group in groups:
+            bits = group["state_bits"]
+            states = [state[p] or self._new_state(p, bits) for p in params]
+            steps.append((params, grads, states, places, images, group))
+        if groups[0][0][0].is_cuda:
+            norm = _ext().adamw_step(steps, -1.0 if clip is None else clip, first["seed"])
+            if clip is not None:
+                self.grad_norm = norm
+            for tower, li in owners:
+                tower.image_updated(li)
+        else:
+            self._cpu_step(steps, clip)
         return loss
 
-    # ------------------------------------------------------------------ GPU
-    def _workspace(self, dev, ngroups, ntensors, npart):
-        """Device scratch of this optimizer's steps: heads, per-tensor constants, partial sums."""
-        ws = self._ws
-        if ws is None or ws["dev"] != dev or ws["groups"] < ngroups or ws["tensors"] < ntensors or ws["part"] < npart:
-            ws = dict(dev=dev, groups=ngroups, tensors=ntensors, part=npart)
-            ws["buf"] = torch.empty(16 * ntensors + 8 * ngroups + 8 * npart, dtype=torch.uint8, device=dev)
-            at = ws["buf"].data_ptr()
-            ws["tensors_at"], ws["heads_at"], ws["part_at"] = at, at + 16 * ntensors, at + 16 * ntensors + 8 * ngroups
-            self._ws = ws
-        return ws
-
-    def _gpu_step(self, groups, dev):
-        from raydp_amd.ops.fused_optim import _image_of
-        L, stream = _lib(), _hip.stream_ptr(dev)
-        clip = groups[0][0]["max_grad_norm"]
-        # fp32 parameters first (stable): a launch takes one type
-        groups = [(group, sorted(live, key=lambda e: e[0].dtype == torch.bfloat16)) for group, live in groups]
-        all_states = [[self._state_of(p, group["state_bits"]) for p, _, _ in live] for group, live in groups]
-        launches = _norm_launches([g for _, live in groups for _, g, _ in live]) if clip is not None else []
-        ws = self._workspace(dev, len(groups), sum(len(live) for _, live in groups), sum(grid for _, grid in launches))
-        npart = _launch_norm(L, launches, ws["part_at"], stream) if launches else 0
-        if clip is not None:
-            self.grad_norm = torch.empty((), dtype=torch.float32, device=dev)
-        # parameter, gradient and two moments
-        touched = sum(p.numel() * (2 * p.element_size() + group["state_bits"] // 4) for group, live in groups for p, _, _ in live)
-        done, owners, first = [], [], 0
-        for k, (group, live) in enumerate(groups):
-            bits, lr = group["state_bits"], group["lr"]
-            lr_dev = None
-            if isinstance(lr, torch.Tensor):
-                if lr.is_cuda:
-                    if lr.device != dev or lr.dtype != torch.float32:
-                        raise TypeError("FusedAdamW: a tensor lr must be fp32 on the parameters' device")
-                    lr_dev, lr = lr.data_ptr(), 0.0
-                else:
-                    lr = float(lr)
-            states = all_states[k]
-            head = ws["heads_at"] + 8 * k
-            for j in range(0, len(live), PREP_MAX):
-                part = live[j:j + PREP_MAX]
-                a = AwPrep()
-                n = a.n = len(part)
-                a.maximize, a.first, a.lr, a.lr_dev, a.wd = int(group["maximize"]), first + j, lr, lr_dev, group["weight_decay"]
-                a.b1, a.b2 = group["betas"]
-                a.max_norm, a.npart, a.part = -1.0 if clip is None else clip, npart, ws["part_at"]
-                a.head, a.tensors, a.seed = head, ws["tensors_at"], group["seed"]
-                a.norm = self.grad_norm.data_ptr() if clip is not None and first + j == 0 else None
-                a.step[:n] = [st["step"].data_ptr() for st in states[j:j + n]]
-                a.ordinal[:n] = [o for _, _, o in part]
-                _hip.check(L.rx_aw_prep(ctypes.byref(a), stream), "rx_aw_prep")
-            b1, b2 = group["betas"]
-            at = 0
-            while at < len(live):
-                low = live[at][0].dtype == torch.bfloat16
-                end = at
-                while end < len(live) and end - at < AW_MAX and (live[end][0].dtype == torch.bfloat16) == low:
-                    end += 1
-                part, sts = live[at:end], states[at:end]
-                a = AwStep()
-                n = a.n = end - at
-                a.b1, a.omb1, a.b2, a.omb2, a.eps = b1, 1.0 - b1, b2, 1.0 - b2, group["eps"]
-                a.head, a.tensors = head, ws["tensors_at"] + 16 * (first + at)
-                a.p[:n] = [p.data_ptr() for p, _, _ in part]
-                a.g[:n] = [g.data_ptr() for _, g, _ in part]
-                a.m[:n] = [st["exp_avg"].data_ptr() for st in sts]
-                a.v[:n] = [st["exp_avg_sq"].data_ptr() for st in sts]
-                lens = [p.numel() for p, _, _ in part]
-                a.len[:n] = lens
-                starts = [0]
-                for ln in lens:
-                    starts.append(starts[-1] + -(-ln // STEP_CHUNK))
-                if starts[-1] > 0x7FFFFFFF:
-                    raise ValueError("FusedAdamW: too many elements for one launch")
-                a.start[:n + 1] = starts
-                if bits == 8:
-                    a.sc[:n] = [st["scales"].data_ptr() for st in sts]
-                if any((x | y) & (3 if bits == 8 else 15) for x, y in zip(a.m[:n], a.v[:n])):
-                    raise ValueError("FusedAdamW: moments must start at a multiple of 4 (8 bits) or 16 bytes")
-                if not low:
-                    for j, (p, _, _) in enumerate(part):
-                        tower, li, img = _image_of(p)
-                        if img is not None:
-                            a.img[j] = img.data_ptr()
-                            owners.append((tower, li))
-                _hip.check(L.rx_aw_step(ctypes.byref(a), bits, int(low), int(touched > LAST_LEVEL), stream), "rx_aw_step")
-                done += [p for p, _, _ in part]
-                at = end
-            first += len(live)
-        torch.autograd.graph.increment_version(done)
-        for tower, li in owners:
-            tower.image_updated(li)
-
     # ------------------------------------------------------------------ CPU
-    def _cpu_step(self, groups):
-        clip, scale = groups[0][0]["max_grad_norm"], 1.0
+    def _cpu_step(self, groups, clip):
+        scale, dev = 1.0, groups[0][0][0].device
+        for params, grads, states, _, _, group in groups:
+            for p, g, st in zip(params, grads, states):
+                if p.device != dev or g.device != dev:
+                    raise ValueError(f"FusedAdamW: parameters with gradients on {dev} and {p.device}")
+                if p.dtype not in (torch.float32, torch.bfloat16) or g.dtype != p.dtype:
+                    raise TypeError(f"FusedAdamW: parameter {p.dtype} with gradient {g.dtype} (both fp32 or both bf16)")
+                if not p.is_contiguous():
+                    raise ValueError("FusedAdamW: parameters must be contiguous")
+                if (st["exp_avg"].dtype == torch.uint8) != (group["state_bits"] == 8):
+                    raise ValueError(f"FusedAdamW: state_bits is {group['state_bits']}, the moments of a parameter are "
+                                     f"{st['exp_avg'].dtype}")
         if clip is not None:
-            norm = torch.sqrt(sum(g.double().square().sum() for _, live in groups for _, g, _ in live))
+            norm = torch.sqrt(sum(g.double().square().sum() for _, grads, _, _, _, _ in groups for g in grads))
             self.grad_norm = norm.float()
             if not bool(torch.isfinite(norm)):
                 return
             scale = (clip / (norm + 1e-6)).clamp(max=1.0).float()
-        for group, live in groups:
+        for params, grads, states, places, _, group in groups:
             b1, b2 = group["betas"]
             bits, lr = group["state_bits"], float(group["lr"])
-            for p, g, place in live:
-                st = self._state_of(p, bits)
+            for p, g, st, place in zip(params, grads, states, places):
+                if not p.numel():
+                    continue
                 st["step"] += 1
                 t = int(st["step"])
                 g = g.float() * (-scale if group["maximize"] else scale)

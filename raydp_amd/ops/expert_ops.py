@@ -8,118 +8,31 @@
 Nothing is read back to the host, so a step with them can be captured into a HIP graph; with a ``capacity`` every expert's
 rows are a slice of fixed size (``rows.view(num_experts, capacity, D)``) that a ``FusedLinearTower`` takes as it is.
 
-``route``, ``dispatch`` and ``combine`` are differentiable (once). On the GPU all run on the HIP kernels and fail loudly if
-the library is missing; on the CPU they are the equivalent PyTorch expressions (any floating type, for tests and CPU-only
+``route``, ``dispatch`` and ``combine`` are differentiable (once). On the GPU all run on the HIP kernels (through
+``csrc/torch/raydp_torch.cc``) and fail loudly if these are missing; on the CPU they are the equivalent PyTorch expressions (any floating type, for tests and CPU-only
 hosts).
 """
-import contextlib
-import ctypes
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
-
-from raydp_amd.ops import _hip
 
 MAX_EXPERTS, MAX_TOPK = 1024, 32
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_VEC = {0: 4, 1: 8, 2: 8}          # elements of a 16-byte vector
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _INT32 = 0x7FFFFFFF
-LAST_LEVEL = 256 << 20          # bytes of the last-level cache
 
 
-class PlanArgs(ctypes.Structure):
-    _fields_ = [("ids", ctypes.c_void_p), ("wide", ctypes.c_int), ("n", ctypes.c_int), ("E", ctypes.c_int),
-                ("chunk", ctypes.c_int), ("blocks", ctypes.c_int), ("capacity", ctypes.c_int), ("rows", ctypes.c_int),
-                ("pad_", ctypes.c_int), ("counts", ctypes.c_void_p), ("position", ctypes.c_void_p),
-                ("source", ctypes.c_void_p), ("load", ctypes.c_void_p), ("offsets", ctypes.c_void_p)]
+_module = None
 
 
-class RowArgs(ctypes.Structure):
-    _fields_ = [("T", ctypes.c_longlong), ("rows", ctypes.c_longlong), ("ldx", ctypes.c_longlong), ("k", ctypes.c_int),
-                ("D", ctypes.c_int), ("lg", ctypes.c_int), ("stream", ctypes.c_int), ("position", ctypes.c_void_p),
-                ("source", ctypes.c_void_p), ("x", ctypes.c_void_p), ("w", ctypes.c_void_p), ("h", ctypes.c_void_p),
-                ("out", ctypes.c_void_p), ("dw", ctypes.c_void_p)]
-
-
-_bound = None
-
-
-def _lib():
-    global _bound
-    L = _hip.lib()
-    if _bound is not L:
-        vp, i, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
-        L.rx_route_fwd.argtypes = [vp, ll, i, ll, i, i, i, vp, vp, vp, vp]
-        L.rx_route_bwd.argtypes = [vp, ll, i, vp, vp, vp, vp, ll, i, i, vp, vp]
-        L.rx_expert_plan.argtypes = [vp, vp, vp]
-        L.rx_rows_scatter.argtypes = [vp, i, vp]
-        L.rx_rows_gather.argtypes = [vp, i, vp]
-        for n in ("rx_route_fwd", "rx_route_bwd", "rx_expert_plan", "rx_rows_scatter", "rx_rows_gather"):
-            getattr(L, n).restype = i
-        L.rx_expert_sizes.argtypes = [vp]
-        L.rx_expert_sizes.restype = None
-        got = (ctypes.c_int * 4)()
-        L.rx_expert_sizes(got)
-        want = [ctypes.sizeof(PlanArgs), ctypes.sizeof(RowArgs), MAX_EXPERTS, MAX_TOPK]
-        if list(got) != want:
-            raise RuntimeError(f"layout mismatch between Python and csrc/hip/experts.hip: C {list(got)} vs {want}")
-        _bound = L
-    return L
-
-
-def _on(device):
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _rows_of(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with contiguous rows (any distance between them)."""
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+def _ext():
+    global _module
+    if _module is None:
+        from raydp_amd.native import loader
+        _module = loader.load_torch()
+    return _module
 
 
 # ------------------------------------------------------------------------------------------------ router
-def _route_gpu(z, k, renormalize, keep):
-    T, E = z.shape
-    w = torch.empty(T, k, dtype=torch.float32, device=z.device)
-    ids = torch.empty(T, k, dtype=torch.int32, device=z.device)
-    norm = torch.empty(T, 2, dtype=torch.float32, device=z.device) if keep else None
-    with _on(z.device):
-        _hip.check(_lib().rx_route_fwd(z.data_ptr(), z.stride(0), _DTYPES[z.dtype], T, E, k, int(renormalize),
-                                       w.data_ptr(), ids.data_ptr(), norm.data_ptr() if keep else None,
-                                       _hip.stream_ptr(z.device)), "rx_route_fwd")
-    return w, ids, norm
-
-
-class _Route(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, k, renormalize):
-        z = _rows_of(logits)
-        w, ids, norm = _route_gpu(z, k, renormalize, not renormalize)
-        # the gradient of the renormalised weights needs no logits
-        ctx.save_for_backward(*((w, ids) if renormalize else (w, ids, norm, z)))
-        ctx.meta = (tuple(logits.shape), logits.dtype)
-        ctx.mark_non_differentiable(ids)
-        ctx.set_materialize_grads(False)
-        return w, ids
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dw, _):
-        if dw is None:
-            return None, None, None
-        w, ids = ctx.saved_tensors[:2]
-        norm, z = ctx.saved_tensors[2:] if len(ctx.saved_tensors) == 4 else (None, None)
-        (T, E), dtype = ctx.meta
-        dw = dw.contiguous()
-        dz = torch.empty(T, E, dtype=dtype, device=w.device)
-        with _on(w.device):
-            _hip.check(_lib().rx_route_bwd(z.data_ptr() if z is not None else None, z.stride(0) if z is not None else 0,
-                                           _DTYPES[dtype], norm.data_ptr() if norm is not None else None, w.data_ptr(),
-                                           ids.data_ptr(), dw.data_ptr(), T, E, w.shape[1], dz.data_ptr(),
-                                           _hip.stream_ptr(w.device)), "rx_route_bwd")
-        return dz, None, None
-
-
 def route(logits: torch.Tensor, k: int, renormalize: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
     """The ``k`` experts of every sample and their weights: ``[T, k]`` fp32 weights (differentiable) and int32 experts, in
     the order of the logits (ties: the lowest expert first).
@@ -143,9 +56,7 @@ def route(logits: torch.Tensor, k: int, renormalize: bool = True) -> Tuple[torch
         return _route_cpu(logits, k, renormalize)
     if logits.dtype not in _DTYPES:
         raise TypeError(f"route: logits dtype {logits.dtype} (fp32, bf16 or fp16)")
-    if logits.requires_grad and torch.is_grad_enabled():
-        return _Route.apply(logits, k, bool(renormalize))
-    return _route_gpu(_rows_of(logits), k, renormalize, False)[:2]
+    return _ext().route(logits, k, bool(renormalize))
 
 
 def _route_cpu(logits, k, renormalize):
@@ -197,28 +108,7 @@ def expert_plan(experts: torch.Tensor, num_experts: int, capacity: Optional[int]
         raise ValueError(f"expert_plan: {max(n, rows)} choices or rows do not fit 32 bits")
     if not experts.is_cuda:
         return _plan_cpu(experts, E, C, rows)
-    dev = experts.device
-    ids = experts if experts.is_contiguous() else experts.contiguous()
-    chunk, blocks = _plan_grid(n)
-    # one allocation: position, source, load, offsets, scratch
-    buf = torch.empty(n + rows + 2 * E + 1 + (blocks * E if blocks > 1 else 0), dtype=torch.int32, device=dev)
-    at = buf.data_ptr()
-    a = PlanArgs(ids.data_ptr(), int(ids.dtype == torch.int64), n, E, chunk, blocks, C, rows, 0, None, at, at + 4 * n,
-                 at + 4 * (n + rows), at + 4 * (n + rows + E))
-    with _on(dev):
-        _hip.check(_lib().rx_expert_plan(ctypes.byref(a), at + 4 * (n + rows + 2 * E + 1) if blocks > 1 else None,
-                                         _hip.stream_ptr(dev)), "rx_expert_plan")
-    return ExpertPlan(buf[:n].view(T, k), buf[n:n + rows], buf[n + rows:n + rows + E],
-                      buf[n + rows + E:n + rows + 2 * E + 1], E, C or None)
-
-
-def _plan_grid(n: int) -> Tuple[int, int]:
-    """(choices per workgroup, workgroups): one workgroup up to 4096 choices, which needs one launch and not two; at most
-    256 workgroups beyond, as each sums the counts of all."""
-    if n <= 4096:
-        return max(1024, -(-n // 1024) * 1024), 1
-    chunk = max(1024, -(-n // (256 * 1024)) * 1024)
-    return chunk, -(-n // chunk)
+    return ExpertPlan(*_ext().expert_plan(experts, E, C), E, C or None)
 
 
 def _plan_cpu(experts, E, C, rows):
@@ -239,69 +129,6 @@ def _plan_cpu(experts, E, C, rows):
 
 
 # ------------------------------------------------------------------------------------------------ rows
-def _row_args(plan, D, dtype, x=None, ldx=0, w=None, h=None, out=None, dw=None):
-    code = _DTYPES[dtype]
-    units = -(-D // _VEC[code])
-    # samples' rows and expert rows, these twice where products are taken: more than the last-level cache is streamed past it
-    touched = (plan.tokens + plan.rows * (2 if dw is not None else 1)) * D * dtype.itemsize
-    a = RowArgs(plan.tokens, plan.rows, ldx, plan.k, D, min(6, (units - 1).bit_length()), int(touched > LAST_LEVEL),
-                plan.position.data_ptr(), plan.source.data_ptr())
-    a.x, a.w, a.h, a.out, a.dw = (t.data_ptr() if t is not None else None for t in (x, w, h, out, dw))
-    return a, code
-
-
-def _scatter(plan, x, w=None, h=None):
-    """(expert rows with ``x`` (times ``w``) in them, inner products with ``h`` or None)."""
-    D = x.shape[1]
-    x = _rows_of(x)
-    out = torch.empty(plan.rows, D, dtype=x.dtype, device=x.device)
-    dw = torch.empty(plan.tokens, plan.k, dtype=torch.float32, device=x.device) if h is not None else None
-    a, code = _row_args(plan, D, x.dtype, x, x.stride(0), w, h, out, dw)
-    with _on(x.device):
-        _hip.check(_lib().rx_rows_scatter(ctypes.byref(a), code, _hip.stream_ptr(x.device)), "rx_rows_scatter")
-    return out, dw
-
-
-def _gather(plan, h, w=None):
-    D = h.shape[1]
-    out = torch.empty(plan.tokens, D, dtype=h.dtype, device=h.device)
-    a, code = _row_args(plan, D, h.dtype, w=w, h=h, out=out)
-    with _on(h.device):
-        _hip.check(_lib().rx_rows_gather(ctypes.byref(a), code, _hip.stream_ptr(h.device)), "rx_rows_gather")
-    return out
-
-
-class _Dispatch(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, plan):
-        ctx.plan = plan
-        return _scatter(plan, x)[0]
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        return _gather(ctx.plan, g.contiguous()), None
-
-
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, rows, weights, plan):
-        ctx.plan = plan
-        ctx.weighted = weights is not None
-        if weights is not None:
-            ctx.save_for_backward(weights, *((rows,) if ctx.needs_input_grad[1] else ()))
-        return _gather(plan, rows, weights)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        if not ctx.weighted:
-            return _scatter(ctx.plan, g)[0], None, None
-        w, rows = ctx.saved_tensors if len(ctx.saved_tensors) == 2 else (ctx.saved_tensors[0], None)
-        drows, dw = _scatter(ctx.plan, g, w, rows)
-        return drows, dw, None
-
-
 def _check_rows(t, plan, want, what):
     if t.dim() != 2 or t.shape[0] != want or t.shape[1] < 1 or not t.is_floating_point():
         raise ValueError(f"{what}: expected floating [{want}, D] for this plan, got {t.dtype} {tuple(t.shape)}")
@@ -320,7 +147,7 @@ def dispatch(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
     if not x.is_cuda:
         rows = x[(plan.source.long().clamp(min=0) // plan.k)] if plan.tokens else x.new_zeros(plan.rows, x.shape[1])
         return torch.where((plan.source >= 0)[:, None], rows, 0.0)
-    return _Dispatch.apply(x, plan) if x.requires_grad and torch.is_grad_enabled() else _scatter(plan, x)[0]
+    return _ext().dispatch(x, plan.position, plan.source)
 
 
 def combine(rows: torch.Tensor, plan: ExpertPlan, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -336,12 +163,7 @@ def combine(rows: torch.Tensor, plan: ExpertPlan, weights: Optional[torch.Tensor
             raise ValueError(f"combine: weights on {weights.device}, rows on {rows.device}")
     if not rows.is_cuda:
         return _combine_cpu(rows, plan, weights)
-    rows = rows.contiguous()
-    if weights is not None:
-        weights = weights.float().contiguous()
-    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
-        return _Combine.apply(rows, weights, plan)
-    return _gather(plan, rows, weights)
+    return _ext().combine(rows, weights, plan.position, plan.source)
 
 
 def _combine_cpu(rows, plan, weights):

@@ -5,7 +5,8 @@ import pytest
 import torch
 
 import expert_oracle as oracle
-from raydp_amd.ops.expert_ops import _plan_grid, combine, dispatch, expert_plan, route
+from raydp_amd.native import loader
+from raydp_amd.ops.expert_ops import combine, dispatch, expert_plan, route
 
 
 @pytest.mark.parametrize("renorm", [True, False])
@@ -88,7 +89,8 @@ def test_refusals():
 
 
 def test_plan_grid_covers_every_choice():
+    plan_grid = loader.load_torch().plan_grid
     for n in list(range(0, 5000, 7)) + [4096, 4097, 262144, 262145, 10 ** 6, 2 ** 31 - 1]:
-        chunk, blocks = _plan_grid(n)
+        chunk, blocks = plan_grid(n)
         assert chunk % 1024 == 0 and blocks >= 1 and chunk * blocks >= n and blocks <= 256
         assert blocks == 1 or chunk * (blocks - 1) < n

@@ -28,12 +28,23 @@ def _make(shapes, dtype, seed, scale=1.0, device="cuda"):
     return ps, grads
 
 
+@pytest.fixture(params=[None, 0], ids=["cached", "streamed"])
+def last_level(request):
+    """Both sides of the bound from which kernels stream past the caches."""
+    from raydp_amd.native import loader
+    ext = loader.load_torch()
+    old = ext.set_last_level(request.param) if request.param is not None else None
+    yield
+    if old is not None:
+        ext.set_last_level(old)
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("cfg", [dict(lr=1e-3), dict(lr=1e-2, betas=(0.0, 0.5), eps=1e-6, weight_decay=0.1),
                                  dict(lr=3e-4, maximize=True, max_grad_norm=0.5, seed=77),
                                  dict(lr=1e-3, betas=(0.95, 0.0), weight_decay=0.0, max_grad_norm=1e9)])
-def test_one_step_from_any_state_matches_the_definition(bits, dtype, cfg):
+def test_one_step_from_any_state_matches_the_definition(bits, dtype, cfg, last_level):
     """One step after another: the oracle takes the kernel's own state before each step, so that a rounding of one step is
     not carried into the next comparison."""
     params, grads = _make(SHAPES, dtype, 3)

@@ -17,6 +17,17 @@ def _half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
 
+@pytest.fixture(params=[None, 0], ids=["cached", "streamed"])
+def last_level(request):
+    """Both sides of the bound from which kernels stream past the caches."""
+    from raydp_amd.native import loader
+    ext = loader.load_torch()
+    old = ext.set_last_level(request.param) if request.param is not None else None
+    yield
+    if old is not None:
+        ext.set_last_level(old)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("renorm", [True, False])
 @pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 16, 2), (7, 3, 3), (65, 8, 1), (130, 17, 5), (33, 64, 2), (40, 65, 8),
@@ -134,7 +145,7 @@ def test_plan_of_many_choices_is_a_stable_sort():
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,k,E,D,capacity", [(1, 2, 16, 384, None), (5, 1, 3, 1, None), (67, 2, 8, 7, 20), (33, 3, 4, 64, None),
                                               (70, 2, 5, 383, 30), (40, 4, 64, 1030, None), (9, 32, 40, 24, 8), (0, 2, 3, 10, 4)])
-def test_dispatch_combine_and_their_gradients(T, k, E, D, capacity, dtype):
+def test_dispatch_combine_and_their_gradients(T, k, E, D, capacity, dtype, last_level):
     g = torch.Generator().manual_seed(T + D)
     ids = torch.randint(-1, E, (T, k), generator=g)
     if T > 1:
@@ -219,6 +230,33 @@ def test_offsets_past_32_bits():
     assert not y[:3].any() and not y[-2].any()
     del rows, y, x
     torch.cuda.empty_cache()
+
+
+def test_differentiating_twice_is_refused():
+    z = torch.randn(4, 5, device="cuda", requires_grad=True)
+    w, ids = route(z, 2)
+    p = expert_plan(ids, 5)
+    y = combine(dispatch(torch.randn(4, 3, device="cuda", requires_grad=True), p), p, w)
+    (dz,) = torch.autograd.grad(y.square().sum(), z, create_graph=True)
+    assert torch.isfinite(dz).all()                      # the first gradient is there
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        dz.sum().backward()
+
+
+def test_gradients_of_some_inputs_only():
+    g = torch.Generator().manual_seed(4)
+    p = expert_plan(torch.randint(0, 3, (20, 2), generator=g).int().cuda(), 3)
+    h, w = torch.randn(40, 7, generator=g).cuda(), torch.rand(20, 2, generator=g).cuda()
+    both = [t.clone().requires_grad_() for t in (h, w)]
+    want = torch.autograd.grad(combine(both[0], p, both[1]).square().sum(), both)
+    hr, wr = h.clone().requires_grad_(), w.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(combine(hr, p, w).square().sum(), hr)[0], want[0])
+    assert torch.equal(torch.autograd.grad(combine(h, p, wr).square().sum(), wr)[0], want[1])
+    with torch.no_grad():
+        assert not combine(hr, p, wr).requires_grad and not dispatch(hr[:20], p).requires_grad
+    leaf = h.clone().requires_grad_()                     # a gradient that is one value for all
+    combine(leaf, p, w).sum().backward()
+    assert torch.equal(leaf.grad, torch.autograd.grad(combine(hr, p, w), hr, torch.ones(20, 7, device="cuda"))[0])
 
 
 def test_same_results_every_time_on_two_streams():
