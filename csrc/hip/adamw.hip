@@ -207,9 +207,9 @@ struct AwLane {
   uint32_t mc, vc;
   int sm, sv;
 
-  __device__ __forceinline__ void load(const AwPlace& a, long long blk, long long i, int left) {
-    p = aw_load4<BF16, NT>(a.p, i, left, FULL);
-    g = aw_load4<BF16, NT>(a.g, i, left, FULL);
+  __device__ __forceinline__ void load(const AwPlace& a, long long blk, long long i, int left, bool vec) {
+    p = aw_load4<BF16, NT>(a.p, i, left, FULL || vec);
+    g = aw_load4<BF16, NT>(a.g, i, left, FULL || vec);
     if constexpr (BITS8) {
       const u16 s = *(const u16*)(a.sc + blk * 2);
       sm = s & 0xFF;
@@ -217,13 +217,13 @@ struct AwLane {
       mc = aw_load4c<NT>((const uint8_t*)a.m + i, left);
       vc = aw_load4c<NT>((const uint8_t*)a.v + i, left);
     } else {
-      m = aw_load4<false, NT>(a.m, i, left, FULL);
-      v = aw_load4<false, NT>(a.v, i, left, FULL);
+      m = aw_load4<false, NT>(a.m, i, left, true);
+      v = aw_load4<false, NT>(a.v, i, left, true);
     }
   }
 
   __device__ __forceinline__ void step(const AwStep& c, const AwTensor& k, float gscale, const AwPlace& a, long long blk,
-                                       long long i, int left, int lane) {
+                                       long long i, int left, bool vec, int lane) {
     float b1 = c.b1, b2 = c.b2;
     if constexpr (BITS8) {
       aw_decode4(mc, vc, sm, sv, m, v);
@@ -268,18 +268,18 @@ struct AwLane {
       aw_store4c<NT>((uint8_t*)a.v + i, v1, left);
       if (lane == 0) *(u16*)(a.sc + blk * 2) = (u16)(min(sm1, 255) | min(sv1, 255) << 8);
     } else {
-      aw_store4<NT>((float*)a.m + i, m, left, FULL);
-      aw_store4<NT>((float*)a.v + i, v, left, FULL);
+      aw_store4<NT>((float*)a.m + i, m, left, true);
+      aw_store4<NT>((float*)a.v + i, v, left, true);
     }
     if constexpr (BF16) {
       // no master copy: rounded with the dither, so that updates under half a step of p are not lost
       const uint32_t lo = aw_dither_bf16x2(p[0], p[1], (h[0] * kSq2) >> 16, (h[1] * kSq2) >> 16);
       const uint32_t hi = aw_dither_bf16x2(p[2], p[3], (h[2] * kSq2) >> 16, (h[3] * kSq2) >> 16);
-      aw_store4h<NT>((u16*)a.p + i, lo, hi, left, FULL);
+      aw_store4h<NT>((u16*)a.p + i, lo, hi, left, FULL || vec);
     } else {
-      aw_store4<NT>((float*)a.p + i, p, left, FULL);
+      aw_store4<NT>((float*)a.p + i, p, left, FULL || vec);
       if (a.img != nullptr) {
-        aw_store4h(a.img + i, rx_f2bf2(p[0], p[1]), rx_f2bf2(p[2], p[3]), left, FULL);
+        aw_store4h(a.img + i, rx_f2bf2(p[0], p[1]), rx_f2bf2(p[2], p[3]), left, FULL || vec);
       }
     }
   }
@@ -296,20 +296,21 @@ __global__ __launch_bounds__(256) void aw_step_kernel(AwStep c) {
   const long long blk = ((long long)(blockIdx.x - c.start[t]) * 4 + wave) * kStepUnroll;
   // bf16 vectors are 8 bytes, an image's too
   const uintptr_t low = BF16 ? ((uintptr_t)a.p | (uintptr_t)a.g) * 2 : (uintptr_t)a.p | (uintptr_t)a.g | (uintptr_t)a.img * 2;
-  if ((low & 15) == 0 && (blk + kStepUnroll) * kBlk <= a.n) {
+  const bool vec = (low & 15) == 0;
+  if (vec && (blk + kStepUnroll) * kBlk <= a.n) {
     AwLane<BITS8, BF16, NT, true> w[kStepUnroll];
 #pragma unroll
-    for (int u = 0; u < kStepUnroll; ++u) w[u].load(a, blk + u, (blk + u) * kBlk + lane * 4, 4);
+    for (int u = 0; u < kStepUnroll; ++u) w[u].load(a, blk + u, (blk + u) * kBlk + lane * 4, 4, true);
 #pragma unroll
-    for (int u = 0; u < kStepUnroll; ++u) w[u].step(c, k, head.gscale, a, blk + u, (blk + u) * kBlk + lane * 4, 4, lane);
+    for (int u = 0; u < kStepUnroll; ++u) w[u].step(c, k, head.gscale, a, blk + u, (blk + u) * kBlk + lane * 4, 4, true, lane);
     return;
   }
   for (long long b = blk; b < blk + kStepUnroll && b * kBlk < a.n; ++b) {
     const long long i = b * kBlk + lane * 4;
     const int left = a.n - i >= 4 ? 4 : a.n - i > 0 ? (int)(a.n - i) : 0;
     AwLane<BITS8, BF16, NT, false> w;
-    w.load(a, b, i, left);
-    w.step(c, k, head.gscale, a, b, i, left, lane);
+    w.load(a, b, i, left, vec);
+    w.step(c, k, head.gscale, a, b, i, left, vec, lane);
   }
 }
 
@@ -363,13 +364,13 @@ __global__ __launch_bounds__(256) void aw_prep_kernel(AwPrep a) {
 
 // Sums of squares in 64 bits: the norm then does not depend on the order of the sum in any of its 32 bits but by chance.
 // 4 x 4 (bf16: 2 x 8) elements of a lane, in flight together
-template <bool BF16, bool FULL>
-__device__ __forceinline__ double aw_squares(const void* g, long long i, long long n) {
+template <bool BF16, bool FULL, bool NT>
+__device__ __forceinline__ double aw_squares(const void* g, long long i, long long n, bool vec) {
   double s = 0.0;
   if constexpr (BF16 && FULL) {
     u32x4 w[kNormChunk / 2048];
 #pragma unroll
-    for (int u = 0; u < kNormChunk / 2048; ++u) w[u] = *(const u32x4*)((const u16*)g + i + u * 2048 + threadIdx.x * 8);
+    for (int u = 0; u < kNormChunk / 2048; ++u) w[u] = aw_get<NT>((const u32x4*)((const u16*)g + i + u * 2048 + threadIdx.x * 8));
 #pragma unroll
     for (int u = 0; u < kNormChunk / 2048; ++u)
 #pragma unroll
@@ -384,7 +385,7 @@ __device__ __forceinline__ double aw_squares(const void* g, long long i, long lo
 #pragma unroll
   for (int u = 0; u < kNormChunk / 1024; ++u) {
     const long long j = i + u * 1024 + threadIdx.x * 4;
-    v[u] = aw_load4<BF16>(g, j, FULL ? 4 : n - j >= 4 ? 4 : n - j > 0 ? (int)(n - j) : 0, FULL);
+    v[u] = aw_load4<BF16, NT>(g, j, FULL ? 4 : n - j >= 4 ? 4 : n - j > 0 ? (int)(n - j) : 0, FULL || vec);
   }
 #pragma unroll
   for (int u = 0; u < kNormChunk / 1024; ++u)
@@ -394,6 +395,7 @@ __device__ __forceinline__ double aw_squares(const void* g, long long i, long lo
 }
 
 // a workgroup takes consecutive chunks, so that it looks for its tensor once and then walks on
+template <bool NT>
 __global__ __launch_bounds__(256) void norm_part_kernel(NormArgs a) {
   __shared__ double lds[4];
   double s = 0.0;
@@ -404,16 +406,16 @@ __global__ __launch_bounds__(256) void norm_part_kernel(NormArgs a) {
     while (c >= a.start[t + 1]) ++t;
     const void* g = a.g[t];
     const long long i = (long long)(c - a.start[t]) * kNormChunk, n = a.len[t];
-    const bool full = i + kNormChunk <= n && ((uintptr_t)g & 15) == 0;
-    if (a.bf16[t]) s += full ? aw_squares<true, true>(g, i, n) : aw_squares<true, false>(g, i, n);
-    else s += full ? aw_squares<false, true>(g, i, n) : aw_squares<false, false>(g, i, n);
+    const bool vec = ((uintptr_t)g & 15) == 0, full = vec && i + kNormChunk <= n;
+    if (a.bf16[t]) s += full ? aw_squares<true, true, NT>(g, i, n, vec) : aw_squares<true, false, NT>(g, i, n, vec);
+    else s += full ? aw_squares<false, true, NT>(g, i, n, vec) : aw_squares<false, false, NT>(g, i, n, vec);
   }
   s = aw_blocksum(s, lds);
   if (threadIdx.x == 0) a.part[blockIdx.x] = s;
 }
 
 template <bool BF16, bool FULL>
-__device__ __forceinline__ void aw_scale_chunk(void* g, long long i, long long n, float f) {
+__device__ __forceinline__ void aw_scale_chunk(void* g, long long i, long long n, float f, bool vec) {
   constexpr int U = kNormChunk / 1024;
   f32x4 v[U];
   int left[U];
@@ -421,14 +423,14 @@ __device__ __forceinline__ void aw_scale_chunk(void* g, long long i, long long n
   for (int u = 0; u < U; ++u) {
     const long long j = i + u * 1024 + threadIdx.x * 4;
     left[u] = FULL ? 4 : n - j >= 4 ? 4 : n - j > 0 ? (int)(n - j) : 0;
-    v[u] = aw_load4<BF16>(g, j, left[u], FULL);
+    v[u] = aw_load4<BF16>(g, j, left[u], FULL || vec);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const long long j = i + u * 1024 + threadIdx.x * 4;
     v[u] *= f;
-    if constexpr (BF16) aw_store4h((u16*)g + j, rx_f2bf2(v[u][0], v[u][1]), rx_f2bf2(v[u][2], v[u][3]), left[u], FULL);
-    else aw_store4((float*)g + j, v[u], left[u], FULL);
+    if constexpr (BF16) aw_store4h((u16*)g + j, rx_f2bf2(v[u][0], v[u][1]), rx_f2bf2(v[u][2], v[u][3]), left[u], FULL || vec);
+    else aw_store4((float*)g + j, v[u], left[u], FULL || vec);
   }
 }
 
@@ -447,16 +449,16 @@ __global__ __launch_bounds__(256) void norm_scale_kernel(ScaleArgs a) {
     while (c >= a.t.start[t + 1]) ++t;
     void* g = const_cast<void*>(a.t.g[t]);
     const long long i = (long long)(c - a.t.start[t]) * kNormChunk, n = a.t.len[t];
-    const bool full = i + kNormChunk <= n && ((uintptr_t)g & 15) == 0;
-    if (a.t.bf16[t]) full ? aw_scale_chunk<true, true>(g, i, n, f) : aw_scale_chunk<true, false>(g, i, n, f);
-    else full ? aw_scale_chunk<false, true>(g, i, n, f) : aw_scale_chunk<false, false>(g, i, n, f);
+    const bool vec = ((uintptr_t)g & 15) == 0, full = vec && i + kNormChunk <= n;
+    if (a.t.bf16[t]) full ? aw_scale_chunk<true, true>(g, i, n, f, vec) : aw_scale_chunk<true, false>(g, i, n, f, vec);
+    else full ? aw_scale_chunk<false, true>(g, i, n, f, vec) : aw_scale_chunk<false, false>(g, i, n, f, vec);
   }
 }
 
 // codes -> the values they stand for (at most 4 significant bits: exact in bf16 too); a wave takes whole scale blocks
 constexpr int kDecUnroll = 4;
 
-template <bool BF16, bool FULL>
+template <bool BF16>
 __device__ __forceinline__ void aw_decode_store(uint32_t mc, uint32_t vc, uint32_t s, void* mo, void* vo, long long i,
                                                 int left) {
   const int sm = s & 0xFF, sv = s >> 8;
@@ -466,11 +468,11 @@ __device__ __forceinline__ void aw_decode_store(uint32_t mc, uint32_t vc, uint32
   if (sm == 255) m = (f32x4){nan, nan, nan, nan};
   if (sv == 255) v = (f32x4){nan, nan, nan, nan};
   if constexpr (BF16) {
-    aw_store4h((u16*)mo + i, rx_f2bf2(m[0], m[1]), rx_f2bf2(m[2], m[3]), left, FULL);
-    aw_store4h((u16*)vo + i, rx_f2bf2(v[0], v[1]), rx_f2bf2(v[2], v[3]), left, FULL);
+    aw_store4h((u16*)mo + i, rx_f2bf2(m[0], m[1]), rx_f2bf2(m[2], m[3]), left, true);
+    aw_store4h((u16*)vo + i, rx_f2bf2(v[0], v[1]), rx_f2bf2(v[2], v[3]), left, true);
   } else {
-    aw_store4((float*)mo + i, m, left, FULL);
-    aw_store4((float*)vo + i, v, left, FULL);
+    aw_store4((float*)mo + i, m, left, true);
+    aw_store4((float*)vo + i, v, left, true);
   }
 }
 
@@ -490,13 +492,13 @@ __global__ __launch_bounds__(256) void aw_decode_kernel(const uint8_t* __restric
     }
 #pragma unroll
     for (int u = 0; u < kDecUnroll; ++u)
-      aw_decode_store<BF16, true>(mc[u], vc[u], s[u], mo, vo, (blk + u) * kBlk + lane * 4, 4);
+      aw_decode_store<BF16>(mc[u], vc[u], s[u], mo, vo, (blk + u) * kBlk + lane * 4, 4);
     return;
   }
   for (long long b = blk; b < blk + kDecUnroll && b * kBlk < n; ++b) {
     const long long i = b * kBlk + lane * 4;
     const int left = n - i >= 4 ? 4 : n - i > 0 ? (int)(n - i) : 0;
-    aw_decode_store<BF16, false>(aw_load4c(m + i, left), aw_load4c(v + i, left), *(const u16*)(sc + b * 2), mo, vo, i, left);
+    aw_decode_store<BF16>(aw_load4c(m + i, left), aw_load4c(v + i, left), *(const u16*)(sc + b * 2), mo, vo, i, left);
   }
 }
 
@@ -530,10 +532,11 @@ int rx_aw_step(const AwStep* a, int bits, int bf16, int stream_past, void* on) {
   return (int)hipGetLastError();
 }
 
-int rx_norm_part(const NormArgs* a, int grid, void* on) {
+int rx_norm_part(const NormArgs* a, int grid, int stream_past, void* on) {
   hipStream_t stream = static_cast<hipStream_t>(on);
   if (a->n <= 0 || a->n > kNormMax || grid <= 0) return -1;
-  hipLaunchKernelGGL(norm_part_kernel, dim3((unsigned)grid), dim3(256), 0, stream, *a);
+  if (stream_past) hipLaunchKernelGGL(norm_part_kernel<true>, dim3((unsigned)grid), dim3(256), 0, stream, *a);
+  else hipLaunchKernelGGL(norm_part_kernel<false>, dim3((unsigned)grid), dim3(256), 0, stream, *a);
   return (int)hipGetLastError();
 }
 

@@ -74,13 +74,50 @@ struct Vec {
 // ------------------------------------------------------------------------------------------------ router
 // L lanes hold a row, V consecutive logits each, as keys that order as (logit, lowest index first) do and differ within a
 // row. The next of the k largest keys is then one max per key and no bookkeeping of what was taken:
-//   16-bit logits: (order-preserving 16 bits, 0xFFFF - index) in 32 bits. key - last wraps for every key below the last
-//                  winner and so puts those above the ones taken: max over (key - last), two keys per v_max3.
-//   fp32 logits:   (order-preserving 32 bits, 0xFFFF - index) as a positive double: v_max_f64 runs at the rate of fp32, two
-//                  words a key; a winner is struck out by its low word.
-// order-preserving unsigned images of the logits' bits (not of NaN and -0: the callers replace them)
-__device__ __forceinline__ uint32_t order16(uint32_t b) { return (b & 0x8000u) ? b ^ 0xFFFFu : b | 0x8000u; }
-__device__ __forceinline__ uint32_t order32(uint32_t b) { return (b & 0x80000000u) ? ~b : b | 0x80000000u; }
+//   16-bit logits: (order-preserving 16 bits, 0xFFFF - index) in 32 bits, made two at a time. key - last wraps for every key
+//                  below the last winner and so puts those above the ones taken: max over (key - last), two per v_max3.
+//   fp32 logits:   (order-preserving 32 bits, 0xFFFF - index) as a positive double: one v_max_f64 for two words; a winner is
+//                  struck out by its low word.
+// The order-preserving bits are the sign and magnitude as a number, shifted so that the magnitudes past infinity (NaN, of
+// either sign) wrap to the bottom: the least key of a chosen logit is the first above minus infinity's, and -0 equals 0.
+// The loop keeps winners as keys in LDS; what they stand for is worked out afterwards, a winner per lane.
+typedef short rx_s16x2 __attribute__((ext_vector_type(2)));
+
+template <int DT> struct Order;
+template <> struct Order<0> {
+  static constexpr uint32_t kInf = 0x7F800000u, kShift = 0x80000000u + 0x7FFFFFu, kLowest = 0xFFFFFFu;   // minus infinity's
+};
+template <> struct Order<1> {
+  static constexpr uint32_t kInf = 0x7F80u, kShift = 0x8000u + 0x7Fu, kLowest = 0xFFu;
+};
+template <> struct Order<2> {
+  static constexpr uint32_t kInf = 0x7C00u, kShift = 0x8000u + 0x3FFu, kLowest = 0x7FFu;
+};
+
+// of two 16-bit logits at once, and of an fp32 one
+template <int DT>
+__device__ __forceinline__ uint32_t order_pair(uint32_t x) {
+  const rx_s16x2 v = __builtin_bit_cast(rx_s16x2, x), sign = v >> 15;
+  const rx_s16x2 mag = v & (rx_s16x2){0x7FFF, 0x7FFF};
+  constexpr short c = (short)Order<DT>::kShift;
+  return __builtin_bit_cast(uint32_t, (rx_s16x2)(((mag ^ sign) - sign) + (rx_s16x2){c, c}));
+}
+__device__ __forceinline__ uint32_t order_one(uint32_t x) {
+  const int sign = (int)x >> 31;
+  return (uint32_t)((((int)(x & 0x7FFFFFFFu)) ^ sign) - sign) + Order<0>::kShift;
+}
+// the logit's bits again
+template <int DT>
+__device__ __forceinline__ float order_back(uint32_t o) {
+  const uint32_t n = o - Order<DT>::kShift;                      // signed: the magnitude with the sign
+  if constexpr (DT == 0) {
+    const int sign = (int)n >> 31;
+    return __uint_as_float((uint32_t)(((int)n ^ sign) - sign) | ((uint32_t)sign & 0x80000000u));
+  } else {
+    const int v = (int)(short)n, sign = v >> 31;
+    return Elem<DT>::get((u16)(((v ^ sign) - sign) | (sign & 0x8000)));
+  }
+}
 
 // LDS written by lanes of a wave is read by its other lanes after this
 __device__ __forceinline__ void wave_sync() {
@@ -111,8 +148,9 @@ __device__ __forceinline__ float group_sum(float v) {
   if constexpr (L >= 64) v += __shfl_xor(v, 32);
   return v;
 }
-__device__ __forceinline__ double as_key(uint32_t hi, uint32_t lo) {
-  return __longlong_as_double((long long)(((unsigned long long)hi << 31) | lo));   // sign 0, never infinite or NaN
+// (order in bits 61 to 30: the sign is 0 and the exponent never all ones)
+__device__ __forceinline__ double as_key(uint32_t o, uint32_t low) {
+  return __longlong_as_double((long long)(((unsigned long long)o << 30) | low));
 }
 template <int CTRL>
 __device__ __forceinline__ double dpp_key(double v) {
@@ -137,93 +175,89 @@ template <int DT, int L, int V>
 __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>::type* __restrict__ z, long long ldz,
                                                         long long T, int E, int k, int renorm, float* __restrict__ w,
                                                         int* __restrict__ ids, float* __restrict__ norm) {
-  extern __shared__ float2 taken[];         // [rows of the workgroup][k]: unnormalised weight, expert
+  extern __shared__ uint2 taken[];          // [rows of the workgroup][k]: order, 0xFFFF - index
   constexpr int N = Elem<DT>::kVec;
   const int lane = threadIdx.x % L, first = lane * V;
   const long long t = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
   if (t >= T) return;
-  const float kNone = -__builtin_huge_valf();
-  float v[V];
-  bool bad = false;
-  uint32_t key[V];
-  double wide[DT == 0 ? V : 1];
+  // places past the row are minus infinity with indexes past the row's: k <= E, so they are never taken
+  Vec<DT> x[V / N];
 #pragma unroll
   for (int c = 0; c < V / N; ++c) {
-    Vec<DT> x;
     const int at = first + c * N;
-    x.load(z + t * ldz + (at < E ? at : 0), E - at);
+    x[c].load(z + t * ldz + (at < E ? at : 0), E - at);
+    if (at + N > E) {
 #pragma unroll
-    for (int q = 0; q < N; ++q) {
-      const int i = c * N + q;
-      const bool there = at + q < E;
-      v[i] = there ? Elem<DT>::get(x.e[q]) : kNone;
-      const bool nan = v[i] != v[i];
-      bad |= nan;
-      // a NaN goes with minus infinity, -0 with 0; places past the row are below everything (and E >= k, so never taken)
-      const uint32_t low = 0xFFFFu - (uint32_t)(at + q);
-      if constexpr (DT == 0) {
-        const uint32_t b = nan ? 0xFF800000u : __float_as_uint(v[i] + 0.f);
-        wide[i] = there ? as_key(order32(b), low) : 0.0;
-      } else {
-        const uint32_t b = nan ? (DT == 1 ? 0xFF80u : 0xFC00u) : x.e[q] == 0x8000u ? 0u : (uint32_t)x.e[q];
-        key[i] = there ? (order16(b) << 16) | low : 0u;
-      }
+      for (int q = 0; q < N; ++q)
+        if (at + q >= E) x[c].e[q] = Elem<DT>::put(-__builtin_huge_valf());
     }
   }
-  // a key is a chosen logit's if it is above those of minus infinity
-  float peak = 0.f, total = 0.f;
-  uint32_t last = 0;
-  float2* mine = taken + (threadIdx.x / L) * k;
-  for (int j = 0; j < k; ++j) {
-    float zj;
-    int at;
-    bool there;
-    if constexpr (DT == 0) {
-      double best = wide[0];
+  uint2* mine = taken + (threadIdx.x / L) * k;
+  uint32_t least = 0xFFFFFFFFu;             // a NaN's order is below minus infinity's
+  if constexpr (DT == 0) {
+    double key[V];
 #pragma unroll
-      for (int i = 1; i < V; ++i) best = fmax(best, wide[i]);
+    for (int i = 0; i < V; ++i) {
+      const uint32_t o = order_one(__float_as_uint(x[i / N].e[i % N]));
+      least = min(least, o);
+      key[i] = as_key(o, 0xFFFFu - (uint32_t)(first + i));
+    }
+    for (int j = 0; j < k; ++j) {
+      double best = key[0];
+#pragma unroll
+      for (int i = 1; i < V; ++i) best = fmax(best, key[i]);
       best = group_max<L>(best);
       const unsigned long long b = (unsigned long long)__double_as_longlong(best);
-      const uint32_t o = (uint32_t)(b >> 31), low = (uint32_t)b & 0xFFFFu;
-      there = o > order32(0xFF800000u);
-      at = (int)(0xFFFFu - low);
-      zj = __uint_as_float((o & 0x80000000u) ? o & 0x7FFFFFFFu : ~o);
+      const uint32_t low = (uint32_t)b & 0xFFFFu;
+      if (lane == 0) mine[j] = make_uint2((uint32_t)(b >> 30), low);
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (at == first + i) wide[i] = 0.0;
-    } else {
+        if (0xFFFFu - (uint32_t)(first + i) == low) key[i] = 0.0;
+    }
+  } else {
+    uint32_t key[V];
+    const uint32_t low0 = 0xFFFFu - (uint32_t)first;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const uint32_t o = order_pair<DT>(x[i / N].w[(i % N) / 2]);
+      key[i] = (o << 16) | (low0 - i);
+      key[i + 1] = (o & 0xFFFF0000u) | (low0 - i - 1);
+      least = min(least, min(o << 16, o & 0xFFFF0000u));
+    }
+    least >>= 16;
+    uint32_t last = 0;
+    for (int j = 0; j < k; ++j) {
       uint32_t best = key[0] - last;
 #pragma unroll
       for (int i = 1; i < V; ++i) best = max(best, key[i] - last);
-      best = group_max<L>(best);
-      last += best;
-      const uint32_t o = last >> 16;
-      there = o > order16(DT == 1 ? 0xFF80u : 0xFC00u);
-      at = (int)(0xFFFFu - (last & 0xFFFFu));
-      zj = Elem<DT>::get((u16)((o & 0x8000u) ? o & 0x7FFFu : ~o));
+      last += group_max<L>(best);
+      if (lane == 0) mine[j] = make_uint2(last >> 16, last & 0xFFFFu);
     }
-    if (j == 0) {
-      peak = there ? zj : 0.f;
-      if (!renorm) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) total += exp_neg(v[i] - peak);
-        total = group_sum<L>(total);
-      }
-    }
-    const float ex = there ? exp_neg(zj - peak) : 0.f;
-    if (renorm) total += ex;
-    if (lane == 0) mine[j] = make_float2(ex, __int_as_float(there ? at : -1));
   }
+  wave_sync();                             // (a row's lanes are one wave's)
+  const uint32_t top = mine[0].x;
+  const float peak = top > Order<DT>::kLowest ? order_back<DT>(top) : 0.f;
+  float total = 0.f;
+  if (renorm) {
+    for (int j = lane; j < k; j += L) {
+      const uint32_t o = mine[j].x;
+      if (o > Order<DT>::kLowest) total += exp_neg(order_back<DT>(o) - peak);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) total += exp_neg(Elem<DT>::get(x[i / N].e[i % N]) - peak);
+  }
+  total = group_sum<L>(total);
   // a NaN in the row shows in all of its weights
-  const unsigned long long rows = __ballot(bad);
+  const unsigned long long rows = __ballot(least < Order<DT>::kLowest);
   const int shift = (threadIdx.x & 63) / L * L;
   const bool any = ((rows >> shift) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1)) != 0;
   const float inv = any ? __uint_as_float(0x7FC00000u) : total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-  wave_sync();                             // (a row's lanes are one wave's)
   for (int j = lane; j < k; j += L) {
-    const float2 e = mine[j];
-    w[t * k + j] = e.x * inv;
-    ids[t * k + j] = __float_as_int(e.y);
+    const uint2 e = mine[j];
+    const bool there = e.x > Order<DT>::kLowest;
+    w[t * k + j] = (there ? exp_neg(order_back<DT>(e.x) - peak) : 0.f) * inv;
+    ids[t * k + j] = there ? (int)(0xFFFFu - e.y) : -1;
   }
   if (norm != nullptr && lane == 0) {
     norm[2 * t] = peak;
@@ -558,7 +592,7 @@ int route_launch(int bwd, const void* z, long long ldz, const float* norm, float
     hipLaunchKernelGGL((route_bwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), 0, stream, (const S*)z, ldz, norm,
                        w, ids, dw, T, E, k, (S*)dz);
   else
-    hipLaunchKernelGGL((route_fwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), sizeof(float2) * (256 / L) * k,
+    hipLaunchKernelGGL((route_fwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), sizeof(uint2) * (256 / L) * k,
                        stream, (const S*)z, ldz, T, E, k, renorm, w, ids, norm_out);
   return (int)hipGetLastError();
 }

@@ -58,6 +58,7 @@ struct NormPlan {
   std::vector<NormArgs> launches;
   std::vector<int> grids;
   int npart = 0;
+  int64_t bytes = 0;
 };
 
 NormPlan norm_plan(const std::vector<Tensor>& grads) {
@@ -72,6 +73,7 @@ NormPlan norm_plan(const std::vector<Tensor>& grads) {
       a.g[j] = g.data_ptr();
       a.len[j] = g.numel();
       a.bf16[j] = bf16(g);
+      plan.bytes += g.numel() * g.element_size();
       a.start[j] = (unsigned)at;
       at += (g.numel() + kNormChunk - 1) / kNormChunk;
     }
@@ -86,7 +88,7 @@ NormPlan norm_plan(const std::vector<Tensor>& grads) {
 void launch_norm(NormPlan& plan, double* part, void* stream) {
   for (size_t k = 0; k < plan.launches.size(); ++k) {
     plan.launches[k].part = part;
-    check(rx_norm_part(&plan.launches[k], plan.grids[k], stream), "rx_norm_part");
+    check(rx_norm_part(&plan.launches[k], plan.grids[k], plan.bytes > g_last_level, stream), "rx_norm_part");
     part += plan.grids[k];
   }
 }

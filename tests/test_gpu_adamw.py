@@ -329,7 +329,7 @@ def test_another_stream_and_a_gradient_in_another_order():
 
 
 @pytest.mark.parametrize("limit", [0.0, 0.01, 1e6, math.inf])
-def test_clip_grad_norm_matches_its_definition(limit):
+def test_clip_grad_norm_matches_its_definition(limit, last_level):
     """Over both types, odd offsets, an order of dimensions that is not C's, and more tensors than one launch takes."""
     gen = torch.Generator().manual_seed(8)
     flat = torch.randn(40000, generator=gen).cuda()

@@ -98,6 +98,10 @@ def test_route_layouts_nan_and_infinity():
         big = torch.finfo(dtype).max
         z = torch.tensor([[-0.0, 0.0, -0.0, 0.0], [0.0, -0.0, 1.0, -1.0], [-big, -math.inf, big, 0.0]], device="cuda").to(dtype)
         assert route(z, 4)[1].tolist() == [[0, 1, 2, 3], [2, 0, 1, 3], [2, 3, 0, -1]]
+        z = torch.tensor([[big, math.inf, big, -big, -math.inf]], device="cuda").to(dtype)
+        assert route(z, 5)[1].tolist() == [[1, 0, 2, 3, -1]]
+        z = torch.tensor([[big, -math.nan, big / 2, math.nan, -big]], device="cuda").to(dtype)
+        assert route(z, 4)[1].tolist() == [[0, 2, 4, -1]] and torch.isnan(route(z, 4)[0]).all()
         z = torch.full((1, 7), math.nan, device="cuda").to(dtype)
         w, ids = route(z, 3)
         assert ids.tolist() == [[-1, -1, -1]] and torch.isnan(w).all()
