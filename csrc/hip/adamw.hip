@@ -93,9 +93,14 @@ __device__ __forceinline__ uint32_t aw_dither_bf16x2(float x, float y, uint32_t 
   return __builtin_amdgcn_perm(b, a, 0x07060302u);
 }
 
-// Loads and stores of 4 consecutive elements; n: how many there are (<= 4); vec: aligned. NT: streamed past the caches. A
-// step that touches more than the 256 MB of the last-level cache gains by that (24 M fp32 with 32-bit moments, 384 MB:
+// Loads and stores of 4 consecutive elements from any address of the type's; n: how many there are (<= 4). Parameters are
+// aligned, but gradients may be slices of a bucket: gfx950 takes vectors at any element. NT: streamed past the caches. A step
+// that touches more than the 256 MB of the last-level cache gains by that (24 M fp32 with 32-bit moments, 384 MB:
 // 128 -> 112 us; 48 M with 8 bits: 148 -> 133), one that fits loses (16 M, 256 MB: 68 -> 76), so the host goes by the bytes.
+typedef f32x4 __attribute__((aligned(4))) f32x4_u;
+typedef rx_u32x2 __attribute__((aligned(2))) u32x2_u;
+typedef u32x4 __attribute__((aligned(2))) u32x4_u;
+
 template <bool NT, class T>
 __device__ __forceinline__ T aw_get(const T* s) {
   if constexpr (NT) return __builtin_nontemporal_load(s);
@@ -108,12 +113,12 @@ __device__ __forceinline__ void aw_put(T* s, T v) {
 }
 
 template <bool BF16, bool NT = false>
-__device__ __forceinline__ f32x4 aw_load4(const void* base, long long i, int n, bool vec) {
+__device__ __forceinline__ f32x4 aw_load4(const void* base, long long i, int n) {
   f32x4 r = {0.f, 0.f, 0.f, 0.f};
   if constexpr (BF16) {
     const u16* s = (const u16*)base + i;
-    if (vec && n == 4) {
-      const rx_u32x2 w = aw_get<NT>((const rx_u32x2*)s);
+    if (n == 4) {
+      const rx_u32x2 w = aw_get<NT>((const u32x2_u*)s);
       r[0] = rx_bf2f((u16)w.x);
       r[1] = __uint_as_float(w.x & 0xFFFF0000u);
       r[2] = rx_bf2f((u16)w.y);
@@ -125,8 +130,8 @@ __device__ __forceinline__ f32x4 aw_load4(const void* base, long long i, int n, 
     }
   } else {
     const float* s = (const float*)base + i;
-    if (vec && n == 4) {
-      r = aw_get<NT>((const f32x4*)s);
+    if (n == 4) {
+      r = aw_get<NT>((const f32x4_u*)s);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -137,9 +142,9 @@ __device__ __forceinline__ f32x4 aw_load4(const void* base, long long i, int n, 
 }
 
 template <bool NT = false>
-__device__ __forceinline__ void aw_store4(float* s, const f32x4& r, int n, bool vec) {
-  if (vec && n == 4) {
-    aw_put<NT>((f32x4*)s, r);
+__device__ __forceinline__ void aw_store4(float* s, const f32x4& r, int n) {
+  if (n == 4) {
+    aw_put<NT>((f32x4_u*)s, (f32x4_u)r);
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -147,9 +152,9 @@ __device__ __forceinline__ void aw_store4(float* s, const f32x4& r, int n, bool 
   }
 }
 template <bool NT = false>
-__device__ __forceinline__ void aw_store4h(u16* s, uint32_t lo, uint32_t hi, int n, bool vec) {
-  if (vec && n == 4) {
-    aw_put<NT>((rx_u32x2*)s, (rx_u32x2){lo, hi});
+__device__ __forceinline__ void aw_store4h(u16* s, uint32_t lo, uint32_t hi, int n) {
+  if (n == 4) {
+    aw_put<NT>((u32x2_u*)s, (u32x2_u){lo, hi});
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -207,9 +212,9 @@ struct AwLane {
   uint32_t mc, vc;
   int sm, sv;
 
-  __device__ __forceinline__ void load(const AwPlace& a, long long blk, long long i, int left, bool vec) {
-    p = aw_load4<BF16, NT>(a.p, i, left, FULL || vec);
-    g = aw_load4<BF16, NT>(a.g, i, left, FULL || vec);
+  __device__ __forceinline__ void load(const AwPlace& a, long long blk, long long i, int left) {
+    p = aw_load4<BF16, NT>(a.p, i, left);
+    g = aw_load4<BF16, NT>(a.g, i, left);
     if constexpr (BITS8) {
       const u16 s = *(const u16*)(a.sc + blk * 2);
       sm = s & 0xFF;
@@ -217,13 +222,13 @@ struct AwLane {
       mc = aw_load4c<NT>((const uint8_t*)a.m + i, left);
       vc = aw_load4c<NT>((const uint8_t*)a.v + i, left);
     } else {
-      m = aw_load4<false, NT>(a.m, i, left, true);
-      v = aw_load4<false, NT>(a.v, i, left, true);
+      m = aw_load4<false, NT>(a.m, i, left);
+      v = aw_load4<false, NT>(a.v, i, left);
     }
   }
 
   __device__ __forceinline__ void step(const AwStep& c, const AwTensor& k, float gscale, const AwPlace& a, long long blk,
-                                       long long i, int left, bool vec, int lane) {
+                                       long long i, int left, int lane) {
     float b1 = c.b1, b2 = c.b2;
     if constexpr (BITS8) {
       aw_decode4(mc, vc, sm, sv, m, v);
@@ -268,18 +273,18 @@ struct AwLane {
       aw_store4c<NT>((uint8_t*)a.v + i, v1, left);
       if (lane == 0) *(u16*)(a.sc + blk * 2) = (u16)(min(sm1, 255) | min(sv1, 255) << 8);
     } else {
-      aw_store4<NT>((float*)a.m + i, m, left, true);
-      aw_store4<NT>((float*)a.v + i, v, left, true);
+      aw_store4<NT>((float*)a.m + i, m, left);
+      aw_store4<NT>((float*)a.v + i, v, left);
     }
     if constexpr (BF16) {
       // no master copy: rounded with the dither, so that updates under half a step of p are not lost
       const uint32_t lo = aw_dither_bf16x2(p[0], p[1], (h[0] * kSq2) >> 16, (h[1] * kSq2) >> 16);
       const uint32_t hi = aw_dither_bf16x2(p[2], p[3], (h[2] * kSq2) >> 16, (h[3] * kSq2) >> 16);
-      aw_store4h<NT>((u16*)a.p + i, lo, hi, left, FULL || vec);
+      aw_store4h<NT>((u16*)a.p + i, lo, hi, left);
     } else {
-      aw_store4<NT>((float*)a.p + i, p, left, FULL || vec);
+      aw_store4<NT>((float*)a.p + i, p, left);
       if (a.img != nullptr) {
-        aw_store4h(a.img + i, rx_f2bf2(p[0], p[1]), rx_f2bf2(p[2], p[3]), left, FULL || vec);
+        aw_store4h(a.img + i, rx_f2bf2(p[0], p[1]), rx_f2bf2(p[2], p[3]), left);
       }
     }
   }
@@ -294,23 +299,20 @@ __global__ __launch_bounds__(256) void aw_step_kernel(AwStep c) {
   const AwPlace a = {c.p[t], c.g[t], c.m[t], c.v[t], BITS8 ? c.sc[t] : nullptr, BF16 ? nullptr : c.img[t], c.len[t]};
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long long blk = ((long long)(blockIdx.x - c.start[t]) * 4 + wave) * kStepUnroll;
-  // bf16 vectors are 8 bytes, an image's too
-  const uintptr_t low = BF16 ? ((uintptr_t)a.p | (uintptr_t)a.g) * 2 : (uintptr_t)a.p | (uintptr_t)a.g | (uintptr_t)a.img * 2;
-  const bool vec = (low & 15) == 0;
-  if (vec && (blk + kStepUnroll) * kBlk <= a.n) {
+  if ((blk + kStepUnroll) * kBlk <= a.n) {
     AwLane<BITS8, BF16, NT, true> w[kStepUnroll];
 #pragma unroll
-    for (int u = 0; u < kStepUnroll; ++u) w[u].load(a, blk + u, (blk + u) * kBlk + lane * 4, 4, true);
+    for (int u = 0; u < kStepUnroll; ++u) w[u].load(a, blk + u, (blk + u) * kBlk + lane * 4, 4);
 #pragma unroll
-    for (int u = 0; u < kStepUnroll; ++u) w[u].step(c, k, head.gscale, a, blk + u, (blk + u) * kBlk + lane * 4, 4, true, lane);
+    for (int u = 0; u < kStepUnroll; ++u) w[u].step(c, k, head.gscale, a, blk + u, (blk + u) * kBlk + lane * 4, 4, lane);
     return;
   }
   for (long long b = blk; b < blk + kStepUnroll && b * kBlk < a.n; ++b) {
     const long long i = b * kBlk + lane * 4;
     const int left = a.n - i >= 4 ? 4 : a.n - i > 0 ? (int)(a.n - i) : 0;
     AwLane<BITS8, BF16, NT, false> w;
-    w.load(a, b, i, left, vec);
-    w.step(c, k, head.gscale, a, b, i, left, vec, lane);
+    w.load(a, b, i, left);
+    w.step(c, k, head.gscale, a, b, i, left, lane);
   }
 }
 
@@ -365,12 +367,12 @@ __global__ __launch_bounds__(256) void aw_prep_kernel(AwPrep a) {
 // Sums of squares in 64 bits: the norm then does not depend on the order of the sum in any of its 32 bits but by chance.
 // 4 x 4 (bf16: 2 x 8) elements of a lane, in flight together
 template <bool BF16, bool FULL, bool NT>
-__device__ __forceinline__ double aw_squares(const void* g, long long i, long long n, bool vec) {
+__device__ __forceinline__ double aw_squares(const void* g, long long i, long long n) {
   double s = 0.0;
   if constexpr (BF16 && FULL) {
     u32x4 w[kNormChunk / 2048];
 #pragma unroll
-    for (int u = 0; u < kNormChunk / 2048; ++u) w[u] = aw_get<NT>((const u32x4*)((const u16*)g + i + u * 2048 + threadIdx.x * 8));
+    for (int u = 0; u < kNormChunk / 2048; ++u) w[u] = aw_get<NT>((const u32x4_u*)((const u16*)g + i + u * 2048 + threadIdx.x * 8));
 #pragma unroll
     for (int u = 0; u < kNormChunk / 2048; ++u)
 #pragma unroll
@@ -385,7 +387,7 @@ __device__ __forceinline__ double aw_squares(const void* g, long long i, long lo
 #pragma unroll
   for (int u = 0; u < kNormChunk / 1024; ++u) {
     const long long j = i + u * 1024 + threadIdx.x * 4;
-    v[u] = aw_load4<BF16, NT>(g, j, FULL ? 4 : n - j >= 4 ? 4 : n - j > 0 ? (int)(n - j) : 0, FULL || vec);
+    v[u] = aw_load4<BF16, NT>(g, j, FULL ? 4 : n - j >= 4 ? 4 : n - j > 0 ? (int)(n - j) : 0);
   }
 #pragma unroll
   for (int u = 0; u < kNormChunk / 1024; ++u)
@@ -406,16 +408,16 @@ __global__ __launch_bounds__(256) void norm_part_kernel(NormArgs a) {
     while (c >= a.start[t + 1]) ++t;
     const void* g = a.g[t];
     const long long i = (long long)(c - a.start[t]) * kNormChunk, n = a.len[t];
-    const bool vec = ((uintptr_t)g & 15) == 0, full = vec && i + kNormChunk <= n;
-    if (a.bf16[t]) s += full ? aw_squares<true, true, NT>(g, i, n, vec) : aw_squares<true, false, NT>(g, i, n, vec);
-    else s += full ? aw_squares<false, true, NT>(g, i, n, vec) : aw_squares<false, false, NT>(g, i, n, vec);
+    const bool full = i + kNormChunk <= n;
+    if (a.bf16[t]) s += full ? aw_squares<true, true, NT>(g, i, n) : aw_squares<true, false, NT>(g, i, n);
+    else s += full ? aw_squares<false, true, NT>(g, i, n) : aw_squares<false, false, NT>(g, i, n);
   }
   s = aw_blocksum(s, lds);
   if (threadIdx.x == 0) a.part[blockIdx.x] = s;
 }
 
 template <bool BF16, bool FULL>
-__device__ __forceinline__ void aw_scale_chunk(void* g, long long i, long long n, float f, bool vec) {
+__device__ __forceinline__ void aw_scale_chunk(void* g, long long i, long long n, float f) {
   constexpr int U = kNormChunk / 1024;
   f32x4 v[U];
   int left[U];
@@ -423,14 +425,14 @@ __device__ __forceinline__ void aw_scale_chunk(void* g, long long i, long long n
   for (int u = 0; u < U; ++u) {
     const long long j = i + u * 1024 + threadIdx.x * 4;
     left[u] = FULL ? 4 : n - j >= 4 ? 4 : n - j > 0 ? (int)(n - j) : 0;
-    v[u] = aw_load4<BF16>(g, j, left[u], FULL || vec);
+    v[u] = aw_load4<BF16>(g, j, left[u]);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const long long j = i + u * 1024 + threadIdx.x * 4;
     v[u] *= f;
-    if constexpr (BF16) aw_store4h((u16*)g + j, rx_f2bf2(v[u][0], v[u][1]), rx_f2bf2(v[u][2], v[u][3]), left[u], FULL || vec);
-    else aw_store4((float*)g + j, v[u], left[u], FULL || vec);
+    if constexpr (BF16) aw_store4h((u16*)g + j, rx_f2bf2(v[u][0], v[u][1]), rx_f2bf2(v[u][2], v[u][3]), left[u]);
+    else aw_store4((float*)g + j, v[u], left[u]);
   }
 }
 
@@ -449,9 +451,9 @@ __global__ __launch_bounds__(256) void norm_scale_kernel(ScaleArgs a) {
     while (c >= a.t.start[t + 1]) ++t;
     void* g = const_cast<void*>(a.t.g[t]);
     const long long i = (long long)(c - a.t.start[t]) * kNormChunk, n = a.t.len[t];
-    const bool vec = ((uintptr_t)g & 15) == 0, full = vec && i + kNormChunk <= n;
-    if (a.t.bf16[t]) full ? aw_scale_chunk<true, true>(g, i, n, f, vec) : aw_scale_chunk<true, false>(g, i, n, f, vec);
-    else full ? aw_scale_chunk<false, true>(g, i, n, f, vec) : aw_scale_chunk<false, false>(g, i, n, f, vec);
+    const bool full = i + kNormChunk <= n;
+    if (a.t.bf16[t]) full ? aw_scale_chunk<true, true>(g, i, n, f) : aw_scale_chunk<true, false>(g, i, n, f);
+    else full ? aw_scale_chunk<false, true>(g, i, n, f) : aw_scale_chunk<false, false>(g, i, n, f);
   }
 }
 
@@ -468,11 +470,11 @@ __device__ __forceinline__ void aw_decode_store(uint32_t mc, uint32_t vc, uint32
   if (sm == 255) m = (f32x4){nan, nan, nan, nan};
   if (sv == 255) v = (f32x4){nan, nan, nan, nan};
   if constexpr (BF16) {
-    aw_store4h((u16*)mo + i, rx_f2bf2(m[0], m[1]), rx_f2bf2(m[2], m[3]), left, true);
-    aw_store4h((u16*)vo + i, rx_f2bf2(v[0], v[1]), rx_f2bf2(v[2], v[3]), left, true);
+    aw_store4h((u16*)mo + i, rx_f2bf2(m[0], m[1]), rx_f2bf2(m[2], m[3]), left);
+    aw_store4h((u16*)vo + i, rx_f2bf2(v[0], v[1]), rx_f2bf2(v[2], v[3]), left);
   } else {
-    aw_store4((float*)mo + i, m, left, true);
-    aw_store4((float*)vo + i, v, left, true);
+    aw_store4((float*)mo + i, m, left);
+    aw_store4((float*)vo + i, v, left);
   }
 }
 

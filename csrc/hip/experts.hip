@@ -410,9 +410,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_rank_kernel(PlanArgs a) {
   __syncthreads();
   if (a.capacity > 0) {
     for (int e = blockIdx.x; e < E; e += gridDim.x)
-      for (int r = before[e] + tid; r < a.capacity; r += kPlanThreads) a.source[e * a.capacity + r] = -1;
+      for (long long r = before[e] + tid; r < a.capacity; r += kPlanThreads) a.source[(long long)e * a.capacity + r] = -1;
   } else {
-    for (int r = all + blockIdx.x * kPlanThreads + tid; r < a.rows; r += gridDim.x * kPlanThreads) a.source[r] = -1;
+    for (long long r = (long long)all + blockIdx.x * kPlanThreads + tid; r < a.rows; r += (long long)gridDim.x * kPlanThreads)
+      a.source[r] = -1;
   }
   int bits = 0;
   while ((1 << bits) < E) ++bits;
@@ -454,6 +455,9 @@ __device__ __forceinline__ long long rows_sample(int lg) {
   return ((long long)blockIdx.x << (8 - lg)) + (threadIdx.x >> lg);
 }
 
+// a choice's row, or -1: a plan that was tampered with does not reach past the rows
+__device__ __forceinline__ long long rows_place(const RowArgs& a, int row) { return row < a.rows ? (long long)row : -1ll; }
+
 // W: times weights; H: and inner products of the sample's row with h's
 template <int DT, bool W, bool H, bool WAVE, bool NT>
 __global__ __launch_bounds__(256) void rows_scatter_kernel(RowArgs a, unsigned sample_blocks) {
@@ -486,7 +490,7 @@ __global__ __launch_bounds__(256) void rows_scatter_kernel(RowArgs a, unsigned s
 #pragma unroll
     for (int j = 0; j < kTogether; ++j) {
       const bool there = j0 + j < a.k;
-      row[j] = there ? (long long)a.position[t * a.k + j0 + j] : -1ll;
+      row[j] = there ? rows_place(a, a.position[t * a.k + j0 + j]) : -1ll;
       w[j] = W && there ? a.w[t * a.k + j0 + j] : 1.f;
       dot[j] = 0.f;
     }
@@ -548,7 +552,7 @@ __global__ __launch_bounds__(256) void rows_gather_kernel(RowArgs a) {
 #pragma unroll
       for (int j = 0; j < kTogether; ++j) {
         const bool there = j0 + j < a.k;
-        row[j] = there ? (long long)position[j0 + j] : -1ll;
+        row[j] = there ? rows_place(a, position[j0 + j]) : -1ll;
         w[j] = W && there ? weight[j0 + j] : 1.f;
       }
       Vec<DT> v[kTogether][P];

@@ -120,7 +120,7 @@ def decode_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, scales: torc
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float) -> torch.Tensor:
     """Scale the gradients of ``parameters`` in place by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` their global
     2-norm (summed in 64 bits), and return the norm (0-dim fp32, on the gradients' device, without a host
-    synchronisation). Gradients are dense (in any dimension order) fp32 or bf16; a parameter that is listed twice
+    synchronisation). Gradients are dense (in any dimension order) fp32 or bf16; a gradient that is listed twice
     counts once. A norm that is not finite is not kept from the gradients (a NaN makes all of them NaN, an infinity 0 and
     NaN), as in ``torch.nn.utils.clip_grad_norm_``."""
     max_norm = float(max_norm)
@@ -128,7 +128,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
         raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm}")
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    grads = [g for g in (p.grad for p in {id(p): p for p in parameters}.values()) if g is not None]
+    grads = list({id(g): g for g in (p.grad for p in parameters) if g is not None}.values())
     if not grads:
         return torch.zeros(())
     if grads[0].is_cuda:

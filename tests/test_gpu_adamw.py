@@ -109,11 +109,12 @@ def test_codes_equal_those_of_the_cpu_bit_for_bit():
 
 
 def test_unaligned_parameters_and_gradients_and_what_lies_between_them():
-    """Parameters that are slices of one buffer at odd offsets: the scalar path, and nothing outside the slices changes."""
+    """Parameters and gradients that are slices of one buffer at odd offsets, as in a gradient bucket: the same bits as on
+    their own, and nothing outside the slices changes."""
     for dtype, bits in ((torch.float32, 8), (torch.bfloat16, 8), (torch.float32, 32)):
-        lens, at = [5, 300, 1, 1027], [1, 9, 311, 315]
-        flat = torch.randn(1400, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
-        gflat = torch.randn(1400, generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
+        lens, at = [5, 300, 1, 1027, 9001], [1, 9, 311, 315, 1345]
+        flat = torch.randn(10400, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+        gflat = torch.randn(10400, generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
         params = [nn.Parameter(flat[a:a + n]) for a, n in zip(at, lens)]
         alone = [nn.Parameter(flat[a:a + n].clone()) for a, n in zip(at, lens)]
         for ps in (params, alone):
@@ -126,7 +127,7 @@ def test_unaligned_parameters_and_gradients_and_what_lies_between_them():
             o2.step()
         for p, q in zip(params, alone):
             assert torch.equal(p.detach(), q.detach())
-        inside = torch.zeros(1400, dtype=torch.bool, device="cuda")
+        inside = torch.zeros(10400, dtype=torch.bool, device="cuda")
         for a, n in zip(at, lens):
             inside[a:a + n] = True
         assert torch.equal(flat[~inside], keep[~inside])

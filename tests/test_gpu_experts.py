@@ -217,6 +217,17 @@ def test_rows_with_strides_shared_rows_and_odd_addresses():
     assert abs(float(one.grad) - float(h.double().sum())) <= 1e-4 * float(h.abs().sum())
 
 
+def test_positions_past_the_rows_reach_nothing():
+    """A plan belongs to its rows; one that was written over is held to them."""
+    p = expert_plan(torch.zeros(4, 2, dtype=torch.int32, device="cuda"), 1)
+    x, h = torch.randn(4, 5, device="cuda"), torch.randn(8, 5, device="cuda")
+    p.position[1, 0] = 8
+    p.position[2, 1] = 2 ** 31 - 1
+    p.position[3] = -7
+    rows, y = dispatch(x, p), combine(h, p)
+    assert torch.equal(rows[p.position[0].long()], x[:1].expand(2, 5)) and torch.equal(y[1], h[3]) and not y[3].any()
+
+
 def test_offsets_past_32_bits():
     """2^31 elements and more on either side; only rows at the far end are looked at."""
     T, k, D = 140000, 2, 8200
