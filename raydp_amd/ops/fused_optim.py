@@ -209,6 +209,8 @@ def adam_step(opt) -> None:
                 a.p[j], a.g[j], a.len[j] = p.data_ptr(), p.grad.data_ptr(), p.numel()
                 a.m[j], a.v[j] = st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()
             _hip.check(L.rx_mt_adam(ctypes.byref(a), _hip.stream_ptr(chunk[0].device)), "rx_mt_adam")
+            # a fused tower re-derives the bf16 image of a weight whose version changed
+            torch.autograd.graph.increment_version(chunk)
 
 
 def _has_step_hooks(opt) -> bool:

@@ -451,3 +451,19 @@ def test_it_steps_behind_the_horovod_wrapper():
         hvd.shutdown()
     for a, b in zip(net.parameters(), ref.parameters()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("cls", [torch.optim.Adam, torch.optim.AdamW])
+def test_a_fused_tower_sees_the_multi_tensor_adam_step(cls):
+    """torch's Adam / AdamW stepped by the kernel (hvd.DistributedOptimizer, GPU train workers): the tower's next forward
+    reads the updated weights, not the bf16 images of the old ones."""
+    from raydp_amd.ops.fused_optim import adam_step
+    from raydp_amd.ops.linear_ops import FusedLinearTower
+    torch.manual_seed(0)
+    lins = [nn.Linear(32, 64).cuda(), nn.Linear(64, 8).cuda()]
+    tower = FusedLinearTower(lins, [True, False])
+    x = torch.randn(40, 32, device="cuda")
+    opt = cls([p for lin in lins for p in lin.parameters()], lr=0.1)
+    tower(x).square().mean().backward()
+    adam_step(opt)
+    assert torch.equal(tower(x), FusedLinearTower(lins, [True, False])(x))
