@@ -325,10 +325,30 @@ __device__ __forceinline__ double aw_blocksum(double s, double* lds) {
   return lds[0] + lds[1] + lds[2] + lds[3];
 }
 
+// (a launch gives up to 1024 partial sums: 4 loads a thread, in flight together)
 __device__ __forceinline__ double aw_partsum(const double* part, int npart, double* lds) {
   double s = 0.0;
-  for (int i = threadIdx.x; i < npart; i += 256) s += part[i];
+  for (int i0 = 0; i0 < npart; i0 += kNormGrid) {
+    double v[kNormGrid / 256];
+#pragma unroll
+    for (int u = 0; u < kNormGrid / 256; ++u) {
+      const int i = i0 + u * 256 + (int)threadIdx.x;
+      v[u] = i < npart ? part[i] : 0.0;
+    }
+#pragma unroll
+    for (int u = 0; u < kNormGrid / 256; ++u) s += v[u];
+  }
   return aw_blocksum(s, lds);
+}
+
+// b^n by squaring: under 50 products, each to half an ulp of 64 bits
+__device__ __forceinline__ double aw_pow(double b, uint32_t n) {
+  double r = 1.0;
+  for (; n != 0; n >>= 1) {
+    if (n & 1) r *= b;
+    b *= b;
+  }
+  return r;
 }
 
 // min(1, max / (norm + 1e-6)): the factor of torch.nn.utils.clip_grad_norm_
@@ -355,12 +375,13 @@ __global__ __launch_bounds__(256) void aw_prep_kernel(AwPrep a) {
   if (i >= a.n || skip) return;
   const float step = *a.step[i] + 1.f;
   *a.step[i] = step;
-  const double t = (double)step, lr = a.lr_dev != nullptr ? (double)*a.lr_dev : a.lr;
+  const uint32_t t = (uint32_t)step;
+  const double lr = a.lr_dev != nullptr ? (double)*a.lr_dev : a.lr;
   AwTensor k;
-  k.nlr_bc1 = (float)(-lr / (1.0 - pow(a.b1, t)));
+  k.nlr_bc1 = (float)(-lr / (1.0 - aw_pow(a.b1, t)));
   k.decay = (float)(1.0 - lr * a.wd);
-  k.rs_bc2 = (float)(1.0 / sqrt(1.0 - pow(a.b2, t)));
-  k.key = aw_mix(aw_mix(a.seed + (uint32_t)a.ordinal[i] * kPhi) + (uint32_t)step);
+  k.rs_bc2 = (float)(1.0 / sqrt(1.0 - aw_pow(a.b2, t)));
+  k.key = aw_mix(aw_mix(a.seed + (uint32_t)a.ordinal[i] * kPhi) + t);
   a.tensors[a.first + i] = k;
 }
 
