@@ -261,11 +261,13 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def _new_state(self, p, bits):
         """The parameter's state, made with its first gradient."""
+        if p.grad.layout != torch.strided:
+            raise RuntimeError("FusedAdamW does not support sparse gradients")
+        if not p.is_contiguous():
+            raise ValueError("FusedAdamW: parameters must be contiguous")
         if p.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("FusedAdamW: the first step of a parameter cannot be captured into a graph (its state "
                                "would be zeroed by every replay): run one eager step first")
-        if not p.is_contiguous():
-            raise ValueError("FusedAdamW: parameters must be contiguous")
         st = self.state[p]
         st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
         kind = torch.uint8 if bits == 8 else torch.float32
@@ -275,61 +277,60 @@ class FusedAdamW(torch.optim.Optimizer):
             st["scales"] = torch.zeros(_scale_rows(p.numel()), 2, dtype=torch.uint8, device=p.device)
         return st
 
-    @torch.no_grad()
     def step(self, closure=None):
-        from raydp_amd.ops.fused_optim import _image_of
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        groups, owners, place, first = [], [], 0, None
+        state, steps, owners, place, clip, seed = self.state, [], [], 0, None, None
         for group in self.param_groups:
             params, grads, places, images = [], [], [], {}
             for o, p in enumerate(group["params"], place):
                 g = p.grad
-                if g is None:
-                    continue
-                if getattr(p, "_raydp_image_owner", None) is not None and p.is_cuda:
-                    tower, li, img = _image_of(p)
-                    if img is not None:
-                        images[len(params)] = img
-                        owners.append((tower, li))
-                params.append(p)
-                grads.append(g)
-                places.append(o)
+                if g is not None:
+                    if getattr(p, "_raydp_image_owner", None) is not None and p.is_cuda:
+                        self._image(p, len(params), images, owners)
+                    params.append(p)
+                    grads.append(g)
+                    places.append(o)
             place += len(group["params"])
-            if params:
-                if first is None:
-                    first = group
-                elif group["max_grad_norm"] != first["max_grad_norm"] or group["seed"] != first["seed"]:
-                    raise ValueError("FusedAdamW: max_grad_norm and seed are the optimizer's, not a group's")
-                groups.append((params, grads, places, images, group))
-        if not groups:
-            return loss
-        for _, grads, _, _, _ in groups:
-            if any(g.layout is not torch.strided for g in grads):
-                raise RuntimeError("FusedAdamW does not support sparse gradients")
-        state, clip = self.state, first["max_grad_norm"]
-        steps = []
-        for params, grads, places, images, group in groups:
+            if not params:
+                continue
+            if seed is None:
+                clip, seed = group["max_grad_norm"], group["seed"]
+            elif group["max_grad_norm"] != clip or group["seed"] != seed:
+                raise ValueError("FusedAdamW: max_grad_norm and seed are the optimizer's, not a group's")
             bits = group["state_bits"]
             states = [state[p] or self._new_state(p, bits) for p in params]
             steps.append((params, grads, states, places, images, group))
-        if groups[0][0][0].is_cuda:
-            norm = _ext().adamw_step(steps, -1.0 if clip is None else clip, first["seed"])
+        if not steps:
+            return loss
+        if steps[0][0][0].is_cuda:
+            norm = _ext().adamw_step(steps, -1.0 if clip is None else clip, seed)
             if clip is not None:
                 self.grad_norm = norm
             for tower, li in owners:
                 tower.image_updated(li)
         else:
-            self._cpu_step(steps, clip)
+            with torch.no_grad():
+                self._cpu_step(steps, clip)
         return loss
+
+    @staticmethod
+    def _image(p, index, images, owners):
+        from raydp_amd.ops.fused_optim import _image_of
+        tower, li, img = _image_of(p)
+        if img is not None:
+            images[index] = img
+            owners.append((tower, li))
 
     # ------------------------------------------------------------------ CPU
     def _cpu_step(self, groups, clip):
         scale, dev = 1.0, groups[0][0][0].device
         for params, grads, states, _, _, group in groups:
             for p, g, st in zip(params, grads, states):
+                if g.layout != torch.strided:
+                    raise RuntimeError("FusedAdamW does not support sparse gradients")
                 if p.device != dev or g.device != dev:
                     raise ValueError(f"FusedAdamW: parameters with gradients on {dev} and {p.device}")
                 if p.dtype not in (torch.float32, torch.bfloat16) or g.dtype != p.dtype:
