@@ -290,6 +290,13 @@ struct AwLane {
   }
 };
 
+// Bound by memory: 16 bytes an element with 8-bit moments and fp32 parameters, 10 with bf16 ones, 28 and 22 with 32-bit
+// moments; one pass, a workgroup per 2048 elements of one tensor (found by bisection over at most 64 starts). A scale block
+// is one wave's 4 elements a lane, so its two maxima are six lane exchanges in registers; two blocks per wave are loaded
+// before the first is worked on (bf16: 104 -> 99 us for 48 M; four give nothing more). Coding, dither and update are about 65
+// issue slots an element, of the 76 that bf16 leaves per element at 5 TB/s: they had to come down from 90 (bytes packed
+// by v_perm, m's code decoded by one sign-extending shift, square root and reciprocal to 1 ulp). 35.4 M fp32 in 17 tensors:
+// 95 us with 8 bits (6.0 TB/s), 160 us with 32 (6.2); 16.8 M bf16 in 64 tensors with 8 bits: 35 us (4.8).
 template <bool BITS8, bool BF16, bool NT>
 __global__ __launch_bounds__(256) void aw_step_kernel(AwStep c) {
   const AwHead head = *c.head;
@@ -357,6 +364,8 @@ __device__ __forceinline__ float aw_clip(double norm, double max_norm) {
   return (float)(c < 1.0 ? c : c >= 1.0 ? 1.0 : c);   // (a NaN stays one)
 }
 
+// One workgroup, a thread per tensor: latency only (3.0 us for 18 tensors, 4.4 for 192 and 1500 partial sums). It could be
+// part of the step's workgroups but for the step words, which all of them would read while one counts them on.
 __global__ __launch_bounds__(256) void aw_prep_kernel(AwPrep a) {
   __shared__ double lds[4];
   float scale = 1.f;
@@ -386,6 +395,9 @@ __global__ __launch_bounds__(256) void aw_prep_kernel(AwPrep a) {
 }
 
 // Sums of squares in 64 bits: the norm then does not depend on the order of the sum in any of its 32 bits but by chance.
+// Bound by memory (a conversion and a 64-bit multiply-add an element fit beside it): 8192 elements are loaded before the
+// first is squared, 1024 workgroups give 16 waves a CU. 50 M fp32 in 36 us (5.6 TB/s; 4096 elements: 38, 512 workgroups: 52),
+// bf16 in 18; 67 M fp32 in 256 tensors, streamed, 48 us for both launches.
 // 4 x 4 (bf16: 2 x 8) elements of a lane, in flight together
 template <bool BF16, bool FULL, bool NT>
 __device__ __forceinline__ double aw_squares(const void* g, long long i, long long n) {
@@ -437,7 +449,7 @@ __global__ __launch_bounds__(256) void norm_part_kernel(NormArgs a) {
   if (threadIdx.x == 0) a.part[blockIdx.x] = s;
 }
 
-template <bool BF16, bool FULL>
+template <bool BF16, bool FULL, bool NT>
 __device__ __forceinline__ void aw_scale_chunk(void* g, long long i, long long n, float f) {
   constexpr int U = kNormChunk / 1024;
   f32x4 v[U];
@@ -446,19 +458,21 @@ __device__ __forceinline__ void aw_scale_chunk(void* g, long long i, long long n
   for (int u = 0; u < U; ++u) {
     const long long j = i + u * 1024 + threadIdx.x * 4;
     left[u] = FULL ? 4 : n - j >= 4 ? 4 : n - j > 0 ? (int)(n - j) : 0;
-    v[u] = aw_load4<BF16>(g, j, left[u]);
+    v[u] = aw_load4<BF16, NT>(g, j, left[u]);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const long long j = i + u * 1024 + threadIdx.x * 4;
     v[u] *= f;
-    if constexpr (BF16) aw_store4h((u16*)g + j, rx_f2bf2(v[u][0], v[u][1]), rx_f2bf2(v[u][2], v[u][3]), left[u]);
-    else aw_store4((float*)g + j, v[u], left[u]);
+    if constexpr (BF16) aw_store4h<NT>((u16*)g + j, rx_f2bf2(v[u][0], v[u][1]), rx_f2bf2(v[u][2], v[u][3]), left[u]);
+    else aw_store4<NT>((float*)g + j, v[u], left[u]);
   }
 }
 
+// 67 M in 64 tensors, norm and scaling: fp32 157 us streamed, 172 through the caches (three passes over 268 MB); bf16 86, 97.
 // g *= min(1, max_norm / (norm + 1e-6)); every workgroup finishes the norm itself (a few KB out of L2), which saves a
 // launch between the two passes; with a factor of 1 nothing is touched
+template <bool NT>
 __global__ __launch_bounds__(256) void norm_scale_kernel(ScaleArgs a) {
   __shared__ double lds[4];
   const double norm = sqrt(aw_partsum(a.t.part, a.npart, lds));
@@ -473,12 +487,13 @@ __global__ __launch_bounds__(256) void norm_scale_kernel(ScaleArgs a) {
     void* g = const_cast<void*>(a.t.g[t]);
     const long long i = (long long)(c - a.t.start[t]) * kNormChunk, n = a.t.len[t];
     const bool full = i + kNormChunk <= n;
-    if (a.t.bf16[t]) full ? aw_scale_chunk<true, true>(g, i, n, f) : aw_scale_chunk<true, false>(g, i, n, f);
-    else full ? aw_scale_chunk<false, true>(g, i, n, f) : aw_scale_chunk<false, false>(g, i, n, f);
+    if (a.t.bf16[t]) full ? aw_scale_chunk<true, true, NT>(g, i, n, f) : aw_scale_chunk<true, false, NT>(g, i, n, f);
+    else full ? aw_scale_chunk<false, true, NT>(g, i, n, f) : aw_scale_chunk<false, false, NT>(g, i, n, f);
   }
 }
 
-// codes -> the values they stand for (at most 4 significant bits: exact in bf16 too); a wave takes whole scale blocks
+// codes -> the values they stand for (at most 4 significant bits: exact in bf16 too); a wave takes whole scale blocks, four
+// of them in flight. Bound by memory: 35.4 M to bf16 in 37 us (5.7 TB/s)
 constexpr int kDecUnroll = 4;
 
 template <bool BF16>
@@ -563,10 +578,11 @@ int rx_norm_part(const NormArgs* a, int grid, int stream_past, void* on) {
   return (int)hipGetLastError();
 }
 
-int rx_norm_scale(const ScaleArgs* a, int grid, void* on) {
+int rx_norm_scale(const ScaleArgs* a, int grid, int stream_past, void* on) {
   hipStream_t stream = static_cast<hipStream_t>(on);
   if (a->t.n <= 0 || a->t.n > kNormMax || grid <= 0) return -1;
-  hipLaunchKernelGGL(norm_scale_kernel, dim3((unsigned)grid), dim3(256), 0, stream, *a);
+  if (stream_past) hipLaunchKernelGGL(norm_scale_kernel<true>, dim3((unsigned)grid), dim3(256), 0, stream, *a);
+  else hipLaunchKernelGGL(norm_scale_kernel<false>, dim3((unsigned)grid), dim3(256), 0, stream, *a);
   return (int)hipGetLastError();
 }
 

@@ -171,6 +171,8 @@ __device__ __forceinline__ double group_max(double v) {
 // e^x for x <= 0: relative error |x| 2^-24 and one ulp
 __device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 
+// Bound by instruction issue where k is large (65536 x 256, k = 8: 18 us in bf16, 32 in fp32, where reading takes 7 and 13),
+// by memory where it is small (262144 x 64, k = 2: 11 us in bf16, 18 in fp32; reading takes 7 and 13).
 template <int DT, int L, int V>
 __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>::type* __restrict__ z, long long ldz,
                                                         long long T, int E, int k, int renorm, float* __restrict__ w,
@@ -266,7 +268,7 @@ __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>:
 }
 
 // The chosen experts' terms are added through LDS, where a lane can reach any place of its row: in registers every one of
-// the k would cost a comparison with every one of the V.
+// the k would cost a comparison with every one of the V (65536 x 256 bf16, k = 8: 96 us that way, 16 this way; the bytes 13).
 template <int DT, int L, int V>
 __global__ __launch_bounds__(256) void route_bwd_kernel(const typename Elem<DT>::type* __restrict__ z, long long ldz,
                                                         const float* __restrict__ norm, const float* __restrict__ w,
@@ -344,6 +346,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const void* __
   for (int e = threadIdx.x; e < E; e += kPlanThreads) counts[(long long)blockIdx.x * E + e] = hist[e];
 }
 
+// Bound by latency: 131072 choices among 64 experts take 4.8 us to count and 8 to rank, 4094 among 8 take 7.6 in one launch.
 // Stable ranks. A workgroup's waves own consecutive pieces of its chunk; a wave takes 64 choices at a time, finds the
 // lanes with the same expert by one ballot per bit of the expert's number, and counts on in LDS.
 __global__ __launch_bounds__(kPlanThreads) void plan_rank_kernel(PlanArgs a) {
@@ -444,6 +447,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_rank_kernel(PlanArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ rows
+// Both row kernels are bound by memory. A sample's row is 16 bytes a lane over as many lanes as it fills, at most a wave, and
+// its expert rows are in flight together. 65536 samples of 1024 bf16 to 2 of 64 experts, streamed: scatter 73 us (403 MB),
+// with weights and inner products 123 (671 MB), gather 66 (403 MB): 5.5 to 6.1 TB/s, where a large copy reaches 5.1.
 constexpr int kTogether = 4;   // expert rows of a sample that are in flight together
 constexpr int kLook = 16;      // expert rows that a wave looks at for empty ones
 

@@ -122,7 +122,8 @@ Tensor clip_grad_norm(const std::vector<Tensor>& all, double max_norm) {
     s.pad_ = 0;
     s.max_norm = max_norm;
     s.norm = k == 0 ? ptr<float>(norm) : nullptr;
-    check(rx_norm_scale(&s, (int)std::min<unsigned>(s.t.chunks, 2 * kNormGrid), stream), "rx_norm_scale");
+    check(rx_norm_scale(&s, (int)std::min<unsigned>(s.t.chunks, 2 * kNormGrid), plan.bytes > g_last_level, stream),
+          "rx_norm_scale");
   }
   for (const Tensor& g : grads) torch::autograd::impl::bump_version(g);
   return norm;
