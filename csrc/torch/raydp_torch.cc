@@ -38,6 +38,11 @@ T* ptr(const Tensor& t) {
   return static_cast<T*>(t.data_ptr());
 }
 
+// a kernel wrote t: autograd, and the towers that keep images of weights, go by its version
+void written(const Tensor& t) {
+  if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
 bool bf16(const Tensor& t) { return t.scalar_type() == at::kBFloat16; }
 
 // A backward of ours is not differentiable itself: under create_graph its results carry a node that says so.
@@ -125,7 +130,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& all, double max_norm) {
     check(rx_norm_scale(&s, (int)std::min<unsigned>(s.t.chunks, 2 * kNormGrid), plan.bytes > g_last_level, stream),
           "rx_norm_scale");
   }
-  for (const Tensor& g : grads) torch::autograd::impl::bump_version(g);
+  for (const Tensor& g : grads) written(g);
   return norm;
 }
 
@@ -322,7 +327,7 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
     first += (int)n;
   }
   for (const Group& grp : all)
-    for (const Slot& s : grp.live) torch::autograd::impl::bump_version(s.p);
+    for (const Slot& s : grp.live) written(s.p);
   if (!norm.defined()) return c10::nullopt;
   return norm;
 }

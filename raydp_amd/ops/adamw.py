@@ -321,6 +321,9 @@ class FusedAdamW(torch.optim.Optimizer):
         from raydp_amd.ops.fused_optim import _image_of
         tower, li, img = _image_of(p)
         if img is not None:
+            # (a step that is left out writes no image: it has to be the weight's before)
+            if tower._versions[li] != (p.data_ptr(), p._version):
+                tower._refresh_images()
             images[index] = img
             owners.append((tower, li))
 

@@ -161,6 +161,70 @@ def test_any_number_of_tensors(count):
             assert float(om.state[p]["step"]) == float(oc.state[q]["step"]) == (1 if i % 7 == 3 else 2)
 
 
+def test_groups_with_their_own_options_share_the_norm():
+    """Groups of other moments' bits, rates, betas and decay; places count on over groups; one norm for all."""
+    g = torch.Generator().manual_seed(12)
+    shapes = [(300,), (5, 7), (2000,), (64,)]
+    gpu = [torch.randn(s, generator=g).cuda().requires_grad_() for s in shapes]
+    cpu = [p.detach().cpu().clone().requires_grad_() for p in gpu]
+
+    def make(ps):
+        return FusedAdamW([dict(params=ps[:2], lr=1e-2, state_bits=32, betas=(0.8, 0.99)),
+                           dict(params=ps[2:], weight_decay=0.3, eps=1e-5, maximize=True)], max_grad_norm=1.5, seed=6)
+    a, b = make(gpu), make(cpu)
+    for _ in range(3):
+        for p, q in zip(gpu, cpu):
+            q.grad = torch.randn(p.shape, generator=g)
+            p.grad = q.grad.cuda()
+        a.step()
+        b.step()
+        assert abs(float(a.grad_norm) - float(b.grad_norm)) <= 2 ** -23 * float(b.grad_norm)
+    for p, q in zip(gpu, cpu):
+        for n in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(a.state[p][n].cpu(), b.state[q][n]), n
+        assert ((p.detach().cpu() - q.detach()).abs() <= 2 ** -21 * (q.detach().abs() + 0.1)).all()
+    extra = torch.ones(9, device="cuda", requires_grad=True)
+    extra.grad = torch.ones(9, device="cuda")
+    a.add_param_group(dict(params=[extra], max_grad_norm=1.5, seed=6))
+    a.step()
+    assert float(a.state[extra]["step"]) == 1 and float(a.state[gpu[0]]["step"]) == 4
+
+
+def test_gradients_made_in_inference_mode_are_clipped():
+    p = nn.Parameter(torch.zeros(700, device="cuda"))
+    with torch.inference_mode():
+        grad = torch.ones(700, device="cuda")
+    with torch.inference_mode():
+        norm = clip_grad_norm_([_With(grad)], 1.0)
+    assert abs(float(norm) - math.sqrt(700)) < 1e-4 and abs(float(grad.norm()) - 1) < 1e-4
+    p.grad = torch.ones(700, device="cuda")
+    opt = FusedAdamW([p])
+    with torch.inference_mode():
+        opt.step()
+    assert float(opt.state[p]["step"]) == 1
+
+
+class _With:
+    def __init__(self, grad):
+        self.grad = grad
+
+
+def test_a_left_out_step_leaves_a_towers_image_right():
+    from raydp_amd.ops.linear_ops import FusedLinearTower
+    lin = nn.Linear(40, 24).cuda()
+    tower = FusedLinearTower([lin], [False])              # no forward yet: no image
+    opt = FusedAdamW(lin.parameters(), max_grad_norm=1.0)
+    for p in lin.parameters():
+        p.grad = torch.full_like(p, math.inf)
+    opt.step()
+    x = torch.randn(9, 40, device="cuda")
+    assert torch.equal(tower(x), FusedLinearTower([lin], [False])(x))
+    with torch.no_grad():
+        lin.weight.mul_(2.0)                              # changed behind the optimizer
+    opt.step()
+    assert torch.equal(tower(x), FusedLinearTower([lin], [False])(x))
+
+
 def test_blocks_of_zeros_tiny_and_huge_values():
     """All-zero blocks stay zero and divide by eps only; magnitudes at both ends of fp32 keep finite, sensible moments; a
     second moment that is not zero is never stored as zero."""

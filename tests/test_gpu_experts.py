@@ -210,6 +210,16 @@ def test_rows_with_strides_shared_rows_and_odd_addresses():
     h = torch.randn(p.rows, 9, generator=g).cuda()
     assert torch.equal(combine(h, p, w), combine(h, p, w.contiguous()))
     assert torch.equal(combine(h, p, w.bfloat16()), combine(h, p, w.bfloat16().float()))
+    for kind in (torch.bfloat16, torch.float64):                  # and their gradient comes back in that type
+        wk = w.to(kind).requires_grad_()
+        (dw,) = torch.autograd.grad(combine(h, p, wk).sum(), wk)
+        w32 = w.to(kind).float().requires_grad_()
+        (want,) = torch.autograd.grad(combine(h, p, w32).sum(), w32)
+        assert dw.dtype == kind and torch.equal(dw, want.to(kind))
+    hs = torch.randn(9, p.rows, generator=g).cuda().requires_grad_()      # rows in another order
+    (dh,) = torch.autograd.grad(combine(hs.t(), p, w).square().sum(), hs)
+    hc = hs.detach().t().contiguous().requires_grad_()
+    assert torch.equal(dh, torch.autograd.grad(combine(hc, p, w).square().sum(), hc)[0].t())
     # one weight for all: the gradient is summed over what it was broadcast to
     one = torch.full((1, 1), 0.5, device="cuda", requires_grad=True)
     y = combine(h, p, one.expand(37, 2))
