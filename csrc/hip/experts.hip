@@ -77,7 +77,7 @@ struct Vec {
 //   16-bit logits: (order-preserving 16 bits, 0xFFFF - index) in 32 bits, made two at a time. key - last wraps for every key
 //                  below the last winner and so puts those above the ones taken: max over (key - last), two per v_max3.
 //   fp32 logits:   (order-preserving 32 bits, 0xFFFF - index) as a positive double: one v_max_f64 for two words; a winner is
-//                  struck out by its low word.
+//                  struck out by its index.
 // The order-preserving bits are the sign and magnitude as a number, shifted so that the magnitudes past infinity (NaN, of
 // either sign) wrap to the bottom: the least key of a chosen logit is the first above minus infinity's, and -0 equals 0.
 // The loop keeps winners as keys in LDS; what they stand for is worked out afterwards, a winner per lane.
@@ -149,8 +149,17 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 // (order in bits 61 to 30: the sign is 0 and the exponent never all ones)
-__device__ __forceinline__ double as_key(uint32_t o, uint32_t low) {
-  return __longlong_as_double((long long)(((unsigned long long)o << 30) | low));
+__device__ __forceinline__ double as_key(uint32_t hi, uint32_t lo) {
+  return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
+}
+// No key is a NaN, which fmax() has to allow for with a second instruction an operand (65536 x 256, k = 8: 29 us with it, 25
+// without). LAST: the result is moved across lanes next, which needs two wait states that the compiler does not see here.
+template <bool LAST>
+__device__ __forceinline__ double key_max(double a, double b) {
+  double r;
+  if constexpr (LAST) asm("v_max_f64 %0, %1, %2\n\ts_nop 1" : "=v"(r) : "v"(a), "v"(b));
+  else asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
 }
 template <int CTRL>
 __device__ __forceinline__ double dpp_key(double v) {
@@ -159,20 +168,20 @@ __device__ __forceinline__ double dpp_key(double v) {
 }
 template <int L>
 __device__ __forceinline__ double group_max(double v) {
-  if constexpr (L >= 2) v = fmax(v, dpp_key<RX_DPP_XOR1>(v));
-  if constexpr (L >= 4) v = fmax(v, dpp_key<RX_DPP_XOR2>(v));
-  if constexpr (L >= 8) v = fmax(v, dpp_key<RX_DPP_HALF_MIRROR>(v));
-  if constexpr (L >= 16) v = fmax(v, dpp_key<RX_DPP_MIRROR>(v));
-  if constexpr (L >= 32) v = fmax(v, __shfl_xor(v, 16));
-  if constexpr (L >= 64) v = fmax(v, __shfl_xor(v, 32));
+  if constexpr (L >= 2) v = key_max<true>(v, dpp_key<RX_DPP_XOR1>(v));
+  if constexpr (L >= 4) v = key_max<true>(v, dpp_key<RX_DPP_XOR2>(v));
+  if constexpr (L >= 8) v = key_max<true>(v, dpp_key<RX_DPP_HALF_MIRROR>(v));
+  if constexpr (L >= 16) v = key_max<true>(v, dpp_key<RX_DPP_MIRROR>(v));
+  if constexpr (L >= 32) v = key_max<true>(v, __shfl_xor(v, 16));
+  if constexpr (L >= 64) v = key_max<true>(v, __shfl_xor(v, 32));
   return v;
 }
 
 // e^x for x <= 0: relative error |x| 2^-24 and one ulp
 __device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 
-// Bound by instruction issue where k is large (65536 x 256, k = 8: 18 us in bf16, 32 in fp32, where reading takes 7 and 13),
-// by memory where it is small (262144 x 64, k = 2: 11 us in bf16, 18 in fp32; reading takes 7 and 13).
+// Bound by instruction issue where k is large (65536 x 256, k = 8: 18 us in bf16, 25 in fp32, where reading takes 7 and 13),
+// by memory where it is small (262144 x 64, k = 2: 11 us in bf16, 15 in fp32; reading takes 7 and 13).
 template <int DT, int L, int V>
 __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>::type* __restrict__ z, long long ldz,
                                                         long long T, int E, int k, int renorm, float* __restrict__ w,
@@ -197,24 +206,27 @@ __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>:
   uint2* mine = taken + (threadIdx.x / L) * k;
   uint32_t least = 0xFFFFFFFFu;             // a NaN's order is below minus infinity's
   if constexpr (DT == 0) {
-    double key[V];
+    uint32_t hi[V], lo[V];
+    const uint32_t low0 = 0xFFFFu - (uint32_t)first;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const uint32_t o = order_one(__float_as_uint(x[i / N].e[i % N]));
       least = min(least, o);
-      key[i] = as_key(o, 0xFFFFu - (uint32_t)(first + i));
+      hi[i] = o >> 2;
+      lo[i] = (o << 30) | (low0 - i);
     }
     for (int j = 0; j < k; ++j) {
-      double best = key[0];
+      double best = as_key(hi[0], lo[0]);
 #pragma unroll
-      for (int i = 1; i < V; ++i) best = fmax(best, key[i]);
-      best = group_max<L>(best);
+      for (int i = 1; i < V - 1; ++i) best = key_max<false>(best, as_key(hi[i], lo[i]));
+      best = group_max<L>(key_max<true>(best, as_key(hi[V - 1], lo[V - 1])));
       const unsigned long long b = (unsigned long long)__double_as_longlong(best);
       const uint32_t low = (uint32_t)b & 0xFFFFu;
       if (lane == 0) mine[j] = make_uint2((uint32_t)(b >> 30), low);
+      // a winner loses its high word: what is left stands for less than minus infinity
+      const uint32_t at = low0 - low;
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (0xFFFFu - (uint32_t)(first + i) == low) key[i] = 0.0;
+      for (int i = 0; i < V; ++i) hi[i] = at == (uint32_t)i ? 0u : hi[i];
     }
   } else {
     uint32_t key[V];
