@@ -7,10 +7,12 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/engine.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <unordered_set>
 #include <vector>
 
 #include "hip/adamw.h"
@@ -58,6 +60,41 @@ variable_list once(variable_list out) {
   return named;
 }
 
+// Called by a backward of ours. A node of an eager call runs on that call's stream, and a leaf's gradient node is one of them
+// as long as anything holds the call's graph. The default stream can have no part in a capture: trying to ends the process.
+// What the pass would reach of that kind is found here first, and the call refused.
+void check_capturable(const Tensor& t) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  const auto on = c10::hip::getCurrentHIPStream(t.get_device());
+  check((int)hipStreamIsCapturing(on.stream(), &status), "hipStreamIsCapturing");
+  if (status == hipStreamCaptureStatusNone) return;
+  using torch::autograd::Node;
+  const auto self = torch::autograd::get_current_node();
+  if (!self) return;
+  // (by number: torch's nodes name the same streams as of device type cuda, these as of type hip)
+  const auto plain = c10::hip::getDefaultHIPStream(t.get_device()).id();
+  const auto* wanted = torch::autograd::get_current_graph_task_exec_info();     // empty: all are
+  std::vector<Node*> todo{self.get()};
+  std::unordered_set<Node*> seen{self.get()};
+  while (!todo.empty()) {
+    Node* node = todo.back();
+    todo.pop_back();
+    for (const auto& edge : node->next_edges()) {
+      Node* next = edge.function.get();
+      if (next == nullptr || !seen.insert(next).second) continue;
+      todo.push_back(next);
+      if (wanted != nullptr && !wanted->empty()) {
+        const auto at = wanted->find(next);
+        if (at == wanted->end() || !at->second.should_execute()) continue;
+      }
+      const auto stream = next->stream();
+      if (stream && stream->id() == plain)
+        throw std::runtime_error("a backward pass cannot be captured when it reaches " + next->name() + " of an eager call on "
+                                 "the default stream: drop what that call returned first, or run it on a side stream");
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ gradient norm
 struct NormPlan {
   std::vector<NormArgs> launches;
@@ -98,10 +135,18 @@ void launch_norm(NormPlan& plan, double* part, void* stream) {
   }
 }
 
+// [first, last) bytes of tensors that a launch writes: two workgroups on the same elements would race
+void check_overlap(std::vector<std::pair<uintptr_t, uintptr_t>>& spans, const char* what) {
+  if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());
+  for (size_t k = 1; k < spans.size(); ++k)
+    if (spans[k].first < spans[k - 1].second) throw py::value_error(std::string(what) + " share memory");
+}
+
 // grads: checked here, dense in any order of dimensions; returns the norm
 Tensor clip_grad_norm(const std::vector<Tensor>& all, double max_norm) {
   std::vector<Tensor> grads;
   const auto dev = all.at(0).device();
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
   for (const Tensor& g : all) {
     if (g.layout() != at::kStrided) throw py::value_error("clip_grad_norm_: sparse gradients are not supported");
     if (g.device() != dev)
@@ -110,8 +155,11 @@ Tensor clip_grad_norm(const std::vector<Tensor>& all, double max_norm) {
       throw py::type_error(std::string("clip_grad_norm_: gradient dtype ") + c10::toString(g.scalar_type()) + " (fp32 or bf16)");
     if (!g.is_non_overlapping_and_dense())
       throw py::value_error("clip_grad_norm_: gradients must be dense (no gaps, no broadcast dimensions)");
-    if (g.numel()) grads.push_back(g);
+    if (g.numel() == 0) continue;
+    grads.push_back(g);
+    spans.emplace_back((uintptr_t)g.data_ptr(), (uintptr_t)g.data_ptr() + g.numel() * g.element_size());
   }
+  check_overlap(spans, "clip_grad_norm_: gradients");
   const auto f32 = all[0].options().dtype(at::kFloat).layout(at::kStrided);
   if (grads.empty()) return at::zeros({}, f32);
   c10::DeviceGuard guard(dev);
@@ -170,6 +218,7 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
   c10::optional<c10::Device> dev;
   int64_t touched = 0;
   size_t count = 0;
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
   for (const auto& item : groups) {
     const py::tuple t = item.cast<py::tuple>();
     const auto params = t[0].cast<std::vector<Tensor>>(), gs = t[1].cast<std::vector<Tensor>>();
@@ -244,6 +293,7 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
       }
       touched += s.p.numel() * (2 * s.p.element_size() + grp.bits / 4);
       grads.push_back(s.g);
+      spans.emplace_back((uintptr_t)s.p.data_ptr(), (uintptr_t)s.p.data_ptr() + s.p.numel() * s.p.element_size());
       grp.live.push_back(std::move(s));
     }
     // fp32 parameters first: a launch takes one type
@@ -252,6 +302,7 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
     all.push_back(std::move(grp));
   }
   if (count == 0) return c10::nullopt;
+  check_overlap(spans, "FusedAdamW: parameters");
   c10::DeviceGuard guard(*dev);
   void* stream = current_stream(grads[0]);
   NormPlan plan;
@@ -384,6 +435,7 @@ struct Route : torch::autograd::Function<Route> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Variable(), Variable(), Variable()};
+    check_capturable(grads[0]);
     const auto saved = ctx->get_saved_variables();
     const Tensor &w = saved[0], &ids = saved[1], dw = grads[0].contiguous();
     const bool full = saved.size() == 4;
@@ -438,7 +490,12 @@ std::vector<Tensor> expert_plan(const Tensor& experts, int64_t E, int64_t capaci
   a.offsets = at_ + n + rows + E;
   c10::DeviceGuard guard(ids.device());
   check(rx_expert_plan(&a, blocks > 1 ? at_ + n + rows + 2 * E + 1 : nullptr, current_stream(ids)), "rx_expert_plan");
-  return {buf.narrow(0, 0, n).view({T, k}), buf.narrow(0, n, rows), buf.narrow(0, n + rows, E), buf.narrow(0, n + rows + E, E + 1)};
+  std::vector<Tensor> out{buf.narrow(0, 0, n).view({T, k}), buf.narrow(0, n, rows), buf.narrow(0, n + rows, E),
+                          buf.narrow(0, n + rows + E, E + 1)};
+  // a version each: what the caller writes into load is no change of the positions that backward keeps
+  for (const Tensor& t : out)
+    if (!t.is_inference()) torch::autograd::impl::set_version_counter(t, c10::VariableVersion(0));
+  return out;
 }
 
 RowArgs row_args(const Tensor& position, const Tensor& source, int64_t D, const Tensor& like, bool twice) {
@@ -498,6 +555,7 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
     return scatter(position, source, x, Tensor(), Tensor()).first;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capturable(grads[0]);
     const auto saved = ctx->get_saved_variables();
     return once({gather(saved[0], saved[1], grads[0].contiguous(), Tensor()), Variable(), Variable()});
   }
@@ -512,6 +570,7 @@ struct Combine : torch::autograd::Function<Combine> {
     return gather(position, source, rows, w);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capturable(grads[0]);
     const auto saved = ctx->get_saved_variables();
     auto [drows, dw] = scatter(saved[0], saved[1], grads[0], saved[2], saved[3]);
     return once({drows, dw, Variable(), Variable()});

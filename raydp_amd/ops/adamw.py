@@ -121,8 +121,8 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     """Scale the gradients of ``parameters`` in place by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` their global
     2-norm (summed in 64 bits), and return the norm (0-dim fp32, on the gradients' device, without a host
     synchronisation). Gradients are dense (in any dimension order) fp32 or bf16; a gradient that is listed twice
-    counts once. A norm that is not finite is not kept from the gradients (a NaN makes all of them NaN, an infinity 0 and
-    NaN), as in ``torch.nn.utils.clip_grad_norm_``."""
+    counts once, and gradients that share memory otherwise raise. A norm that is not finite is not kept from the gradients
+    (a NaN makes all of them NaN, an infinity 0 and NaN), as in ``torch.nn.utils.clip_grad_norm_``."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm}")
@@ -142,11 +142,18 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
             raise TypeError(f"clip_grad_norm_: gradient dtype {g.dtype} (fp32 or bf16)")
         if not _dense(g):
             raise ValueError("clip_grad_norm_: gradients must be dense (no gaps, no broadcast dimensions)")
+    _check_overlap(grads, "clip_grad_norm_: gradients")
     norm = torch.sqrt(sum(g.double().square().sum() for g in grads))
     f = (max_norm / (norm + 1e-6)).clamp(max=1.0).float()
     for g in grads:
         g.copy_(g.float() * f)
     return norm.float()
+
+
+def _check_overlap(tensors, what):
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
+    if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        raise ValueError(f"{what} share memory")
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -176,8 +183,8 @@ class FusedAdamW(torch.optim.Optimizer):
     fp32) and, for 8 bits, ``scales`` (uint8 ``[ceil(n / 256), 2]``); :func:`decode_moments` gives their values.
     ``load_state_dict`` also takes the state of a ``torch.optim.AdamW`` and codes its moments.
 
-    Parameters are contiguous fp32 or bf16; gradients are dense and of the parameter's type. Sparse gradients, a first
-    step inside a graph capture raise."""
+    Parameters are contiguous fp32 or bf16; gradients are dense and of the parameter's type. Sparse gradients, parameters
+    that share memory, a first step inside a graph capture raise."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                  state_bits: int = 8, max_grad_norm: Optional[float] = None, maximize: bool = False, seed: int = 0):
@@ -343,6 +350,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 if (st["exp_avg"].dtype == torch.uint8) != (group["state_bits"] == 8):
                     raise ValueError(f"FusedAdamW: state_bits is {group['state_bits']}, the moments of a parameter are "
                                      f"{st['exp_avg'].dtype}")
+        _check_overlap([p for params, *_ in groups for p in params], "FusedAdamW: parameters")
         if clip is not None:
             norm = torch.sqrt(sum(g.double().square().sum() for _, grads, _, _, _, _ in groups for g in grads))
             self.grad_norm = norm.float()

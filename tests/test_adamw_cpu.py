@@ -141,3 +141,27 @@ def test_refusals():
             decode_moments(*bad)
     with pytest.raises(TypeError):
         decode_moments(c, c, s, torch.float16)
+
+
+@pytest.mark.parametrize("views", [((0, 8), (4, 12)), ((0, 8), (0, 8)), ((3, 4), (0, 12))])
+def test_shared_memory_is_refused(views):
+    flat, (p, q) = torch.ones(12), (nn.Parameter(torch.ones(b - a)) for a, b in views)
+    p.grad, q.grad = (flat[a:b] for a, b in views)
+    with pytest.raises(ValueError, match="share memory"):
+        clip_grad_norm_([p, q], 1.0)
+    assert torch.equal(flat, torch.ones(12))
+    FusedAdamW([p, q]).step()                            # (a step only reads them)
+    p, q = (nn.Parameter(flat[a:b]) for a, b in views)
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    with pytest.raises(ValueError, match="share memory"):
+        FusedAdamW([p, q]).step()
+    assert torch.equal(flat, torch.ones(12))
+
+
+def test_neighbours_in_one_buffer_are_not_shared():
+    flat, p, q = torch.ones(12), nn.Parameter(torch.ones(7)), nn.Parameter(torch.ones(5))
+    p.grad, q.grad = flat[5:], flat[:5]
+    assert float(clip_grad_norm_([p, q], 1e9)) == pytest.approx(math.sqrt(12.0), rel=2 ** -23)
+    p, q = nn.Parameter(flat[5:]), nn.Parameter(flat[:5])
+    p.grad, q.grad = torch.ones(7), torch.ones(5)
+    FusedAdamW([p, q]).step()

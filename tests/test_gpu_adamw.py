@@ -531,3 +531,31 @@ def test_a_fused_tower_sees_the_multi_tensor_adam_step(cls):
     tower(x).square().mean().backward()
     adam_step(opt)
     assert torch.equal(tower(x), FusedLinearTower(lins, [True, False])(x))
+
+
+@pytest.mark.parametrize("views", [((0, 8), (4, 12)), ((0, 8), (0, 8)), ((3, 4), (0, 12))])
+def test_shared_memory_is_refused(views):
+    """Two workgroups of one launch would race there."""
+    flat = torch.ones(12, device="cuda")
+    p, q = (nn.Parameter(torch.ones(b - a, device="cuda")) for a, b in views)
+    p.grad, q.grad = (flat[a:b] for a, b in views)
+    with pytest.raises(ValueError, match="share memory"):
+        clip_grad_norm_([p, q], 1.0)
+    assert torch.equal(flat, torch.ones_like(flat))
+    FusedAdamW([p, q]).step()                            # (a step only reads them)
+    p, q = (nn.Parameter(flat[a:b]) for a, b in views)
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    with pytest.raises(ValueError, match="share memory"):
+        FusedAdamW([p, q]).step()
+    assert torch.equal(flat, torch.ones_like(flat))
+
+
+def test_neighbours_in_one_buffer_are_not_shared():
+    flat = torch.ones(12, device="cuda")
+    p, q = nn.Parameter(torch.ones(7, device="cuda")), nn.Parameter(torch.ones(5, device="cuda"))
+    p.grad, q.grad = flat[5:], flat[:5]
+    assert float(clip_grad_norm_([p, q], 1e9)) == pytest.approx(math.sqrt(12.0), rel=2 ** -23)
+    p, q = nn.Parameter(flat[5:]), nn.Parameter(flat[:5])
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    FusedAdamW([p, q]).step()
+    assert bool((flat < 1).all())

@@ -399,3 +399,57 @@ def test_a_training_step_of_a_routed_tower():
         for a, b in zip(model.parameters(), twin.parameters()):
             assert torch.equal(a, b), k
     del graph
+
+
+def test_parts_of_a_plan_are_tensors_of_their_own():
+    """Writing into the loads between forward and backward is no change of what backward reads."""
+    x = torch.randn(20, 6, device="cuda", requires_grad=True)
+    p = expert_plan(torch.arange(40, device="cuda").view(20, 2) % 3, 3, 10)
+    y = combine(dispatch(x, p), p)
+    p.load.clamp_(max=10)
+    p.offsets.add_(1)
+    (dx,) = torch.autograd.grad(y.sum(), x)
+    assert torch.equal(dx, (p.position >= 0).sum(1, keepdim=True).float().expand(20, 6))
+    y = combine(dispatch(x, p), p)
+    p.position.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), x)
+
+
+@pytest.mark.parametrize("what", ["leaf", "result", "asked"])
+def test_capturing_what_an_eager_call_made_is_refused(what):
+    """Nodes of an eager call on the default stream cannot run in a capture: a leaf's gradient node that the call's result
+    holds, an intermediate result's. Those of a side stream can."""
+    x = torch.randn(20, 6, device="cuda", requires_grad=True)
+    p = expert_plan(torch.arange(40, device="cuda").view(20, 2) % 3, 3)
+
+    def once(leaf):
+        y = combine(dispatch(leaf, p), p)
+        if what == "asked":
+            leaf.grad, = torch.autograd.grad(y.sum(), leaf)
+        else:
+            y.sum().backward()
+        return y
+    held = once(x)
+    x.grad = None
+    start = x * 1 if what == "result" else x
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(graph):
+            once(start)
+    assert x.grad is None
+    z = x.detach().requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        held = once(z)
+    torch.cuda.current_stream().wait_stream(side)
+    z.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = once(z)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(z.grad, torch.full_like(z, 2.0)) and torch.equal(y, held)
+    del graph
