@@ -76,6 +76,7 @@ int rx_aw_step(const AwStep* a, int bits, int bf16, int stream_past, void* strea
 // grid: workgroups, one partial sum each; stream_past: all gradients together are larger than the last-level cache
 int rx_norm_part(const NormArgs* a, int grid, int stream_past, void* stream);
 int rx_norm_scale(const ScaleArgs* a, int grid, int stream_past, void* stream);
+// stream_past: codes and values take much of the last-level cache
 int rx_aw_decode(const uint8_t* m, const uint8_t* v, const uint8_t* sc, void* mo, void* vo, long long n, int bf16,
-                 void* stream);
+                 int stream_past, void* stream);
 }

@@ -496,7 +496,7 @@ __global__ __launch_bounds__(256) void norm_scale_kernel(ScaleArgs a) {
 // of them in flight. Bound by memory: 35.4 M to bf16 in 37 us (5.7 TB/s)
 constexpr int kDecUnroll = 4;
 
-template <bool BF16>
+template <bool BF16, bool NT>
 __device__ __forceinline__ void aw_decode_store(uint32_t mc, uint32_t vc, uint32_t s, void* mo, void* vo, long long i,
                                                 int left) {
   const int sm = s & 0xFF, sv = s >> 8;
@@ -506,15 +506,15 @@ __device__ __forceinline__ void aw_decode_store(uint32_t mc, uint32_t vc, uint32
   if (sm == 255) m = (f32x4){nan, nan, nan, nan};
   if (sv == 255) v = (f32x4){nan, nan, nan, nan};
   if constexpr (BF16) {
-    aw_store4h((u16*)mo + i, rx_f2bf2(m[0], m[1]), rx_f2bf2(m[2], m[3]), left);
-    aw_store4h((u16*)vo + i, rx_f2bf2(v[0], v[1]), rx_f2bf2(v[2], v[3]), left);
+    aw_store4h<NT>((u16*)mo + i, rx_f2bf2(m[0], m[1]), rx_f2bf2(m[2], m[3]), left);
+    aw_store4h<NT>((u16*)vo + i, rx_f2bf2(v[0], v[1]), rx_f2bf2(v[2], v[3]), left);
   } else {
-    aw_store4((float*)mo + i, m, left);
-    aw_store4((float*)vo + i, v, left);
+    aw_store4<NT>((float*)mo + i, m, left);
+    aw_store4<NT>((float*)vo + i, v, left);
   }
 }
 
-template <bool BF16>
+template <bool BF16, bool NT>
 __global__ __launch_bounds__(256) void aw_decode_kernel(const uint8_t* __restrict__ m, const uint8_t* __restrict__ v,
                                                         const uint8_t* __restrict__ sc, void* __restrict__ mo,
                                                         void* __restrict__ vo, long long n) {
@@ -525,18 +525,18 @@ __global__ __launch_bounds__(256) void aw_decode_kernel(const uint8_t* __restric
 #pragma unroll
     for (int u = 0; u < kDecUnroll; ++u) {
       s[u] = *(const u16*)(sc + (blk + u) * 2);
-      mc[u] = *(const uint32_t*)(m + (blk + u) * kBlk + lane * 4);
-      vc[u] = *(const uint32_t*)(v + (blk + u) * kBlk + lane * 4);
+      mc[u] = aw_get<NT>((const uint32_t*)(m + (blk + u) * kBlk + lane * 4));
+      vc[u] = aw_get<NT>((const uint32_t*)(v + (blk + u) * kBlk + lane * 4));
     }
 #pragma unroll
     for (int u = 0; u < kDecUnroll; ++u)
-      aw_decode_store<BF16>(mc[u], vc[u], s[u], mo, vo, (blk + u) * kBlk + lane * 4, 4);
+      aw_decode_store<BF16, NT>(mc[u], vc[u], s[u], mo, vo, (blk + u) * kBlk + lane * 4, 4);
     return;
   }
   for (long long b = blk; b < blk + kDecUnroll && b * kBlk < n; ++b) {
     const long long i = b * kBlk + lane * 4;
     const int left = n - i >= 4 ? 4 : n - i > 0 ? (int)(n - i) : 0;
-    aw_decode_store<BF16>(aw_load4c(m + i, left), aw_load4c(v + i, left), *(const u16*)(sc + b * 2), mo, vo, i, left);
+    aw_decode_store<BF16, NT>(aw_load4c(m + i, left), aw_load4c(v + i, left), *(const u16*)(sc + b * 2), mo, vo, i, left);
   }
 }
 
@@ -587,15 +587,18 @@ int rx_norm_scale(const ScaleArgs* a, int grid, int stream_past, void* on) {
 }
 
 int rx_aw_decode(const uint8_t* m, const uint8_t* v, const uint8_t* sc, void* mo, void* vo, long long n, int bf16,
-                 void* on) {
+                 int stream_past, void* on) {
   hipStream_t stream = static_cast<hipStream_t>(on);
   if (n <= 0) return 0;
   const long long grid = (n + 4 * kDecUnroll * kBlk - 1) / (4 * kDecUnroll * kBlk);
   if (grid > 0x7FFFFFFFll) return -1;
-  if (bf16)
-    hipLaunchKernelGGL((aw_decode_kernel<true>), dim3((unsigned)grid), dim3(256), 0, stream, m, v, sc, mo, vo, n);
-  else
-    hipLaunchKernelGGL((aw_decode_kernel<false>), dim3((unsigned)grid), dim3(256), 0, stream, m, v, sc, mo, vo, n);
+#define RX_DECODE(BF16, NT) \
+  hipLaunchKernelGGL((aw_decode_kernel<BF16, NT>), dim3((unsigned)grid), dim3(256), 0, stream, m, v, sc, mo, vo, n)
+  if (bf16 && stream_past) RX_DECODE(true, true);
+  else if (bf16) RX_DECODE(true, false);
+  else if (stream_past) RX_DECODE(false, true);
+  else RX_DECODE(false, false);
+#undef RX_DECODE
   return (int)hipGetLastError();
 }
 
