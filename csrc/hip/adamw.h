@@ -5,11 +5,12 @@
 enum {
   kAwMax = 64,         // tensors in one step launch (kernel arguments under 4 KiB)
   kAwPrepMax = 256,    // tensors in one preparation launch (one thread each)
-  kNormMax = 128,      // tensors in one norm / scale launch
+  kNormMax = 256,      // tensors in one norm / scale launch (kernel arguments under 4 KiB)
   kAwBlock = 256,      // elements that share a scale: 4 per lane of one wave
   kAwChunk = 2048,     // elements of a step workgroup: 4 waves, 2 scale blocks in flight in each
   kNormChunk = 8192,   // elements that a norm workgroup has in flight
-  kNormGrid = 1024     // workgroups, and so partial sums, of a norm launch at most
+  kNormGrid = 1024,    // workgroups, and so partial sums, of a norm launch at most
+  kNormBf16 = 0x8000   // in NormArgs::last: the tensor is bf16
 };
 
 struct AwHead {        // one per launch group of a step
@@ -57,10 +58,11 @@ struct NormArgs {
   double* part;                      // one partial sum per workgroup
   unsigned chunks, pad_;
   const void* g[kNormMax];
-  long long len[kNormMax];
-  unsigned start[kNormMax + 1];
-  unsigned char bf16[kNormMax];
+  unsigned start[kNormMax + 1];      // first chunk of each tensor
+  uint16_t last[kNormMax];           // elements of its last chunk, and kNormBf16
 };
+
+static_assert(kNormChunk < kNormBf16, "a chunk's elements and the type share 16 bits");
 
 struct ScaleArgs {
   NormArgs t;                        // t.part: the partial sums to finish

@@ -429,6 +429,11 @@ __device__ __forceinline__ double aw_squares(const void* g, long long i, long lo
   return s;
 }
 
+// elements of chunk c, which is one of tensor t's
+__device__ __forceinline__ int norm_count(const NormArgs& a, int t, unsigned c) {
+  return c + 1 < a.start[t + 1] ? (int)kNormChunk : (int)(a.last[t] & ~kNormBf16);
+}
+
 // a workgroup takes consecutive chunks, so that it looks for its tensor once and then walks on
 template <bool NT>
 __global__ __launch_bounds__(256) void norm_part_kernel(NormArgs a) {
@@ -440,9 +445,9 @@ __global__ __launch_bounds__(256) void norm_part_kernel(NormArgs a) {
   for (unsigned c = first; c < last; ++c) {
     while (c >= a.start[t + 1]) ++t;
     const void* g = a.g[t];
-    const long long i = (long long)(c - a.start[t]) * kNormChunk, n = a.len[t];
-    const bool full = i + kNormChunk <= n;
-    if (a.bf16[t]) s += full ? aw_squares<true, true, NT>(g, i, n) : aw_squares<true, false, NT>(g, i, n);
+    const long long i = (long long)(c - a.start[t]) * kNormChunk, n = i + norm_count(a, t, c);
+    const bool full = n == i + kNormChunk;
+    if (a.last[t] & kNormBf16) s += full ? aw_squares<true, true, NT>(g, i, n) : aw_squares<true, false, NT>(g, i, n);
     else s += full ? aw_squares<false, true, NT>(g, i, n) : aw_squares<false, false, NT>(g, i, n);
   }
   s = aw_blocksum(s, lds);
@@ -485,9 +490,9 @@ __global__ __launch_bounds__(256) void norm_scale_kernel(ScaleArgs a) {
   for (unsigned c = first; c < last; ++c) {
     while (c >= a.t.start[t + 1]) ++t;
     void* g = const_cast<void*>(a.t.g[t]);
-    const long long i = (long long)(c - a.t.start[t]) * kNormChunk, n = a.t.len[t];
-    const bool full = i + kNormChunk <= n;
-    if (a.t.bf16[t]) full ? aw_scale_chunk<true, true, NT>(g, i, n, f) : aw_scale_chunk<true, false, NT>(g, i, n, f);
+    const long long i = (long long)(c - a.t.start[t]) * kNormChunk, n = i + norm_count(a.t, t, c);
+    const bool full = n == i + kNormChunk;
+    if (a.t.last[t] & kNormBf16) full ? aw_scale_chunk<true, true, NT>(g, i, n, f) : aw_scale_chunk<true, false, NT>(g, i, n, f);
     else full ? aw_scale_chunk<false, true, NT>(g, i, n, f) : aw_scale_chunk<false, false, NT>(g, i, n, f);
   }
 }

@@ -113,8 +113,7 @@ NormPlan norm_plan(const std::vector<Tensor>& grads) {
     for (int j = 0; j < a.n; ++j) {
       const Tensor& g = grads[k + j];
       a.g[j] = g.data_ptr();
-      a.len[j] = g.numel();
-      a.bf16[j] = bf16(g);
+      a.last[j] = (uint16_t)((g.numel() - 1) % kNormChunk + 1 + (bf16(g) ? kNormBf16 : 0));
       plan.bytes += g.numel() * g.element_size();
       a.start[j] = (unsigned)at;
       at += (g.numel() + kNormChunk - 1) / kNormChunk;

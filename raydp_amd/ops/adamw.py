@@ -7,7 +7,7 @@
   that a fused Linear tower reads get their bf16 image in the same pass; bf16 parameters have no master copy and are
   rounded stochastically. Step counts live on the device, so a step can be captured into a HIP graph once an eager step
   has made the state.
-* :func:`clip_grad_norm_` -- ``torch.nn.utils.clip_grad_norm_`` (2-norm) in two launches per 128 tensors, without a host
+* :func:`clip_grad_norm_` -- ``torch.nn.utils.clip_grad_norm_`` (2-norm) in two launches per 256 tensors, without a host
   read. ``FusedAdamW(max_grad_norm=...)`` applies the same factor inside the step instead, without the pass that
   rewrites the gradients.
 * :func:`decode_moments` -- the values that 8-bit moments stand for.

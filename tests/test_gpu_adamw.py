@@ -559,3 +559,25 @@ def test_neighbours_in_one_buffer_are_not_shared():
     p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
     FusedAdamW([p, q]).step()
     assert bool((flat < 1).all())
+
+
+@pytest.mark.parametrize("count", [255, 256, 257, 600])
+def test_clip_over_several_launches(count, last_level):
+    """Lengths around a chunk (8192) and of one element, types in turn."""
+    gen = torch.Generator().manual_seed(count)
+    params = []
+    for i in range(count):
+        n = (1, 8191, 8192, 8193, 37, 16384, 300)[i % 7]
+        p = nn.Parameter(torch.empty(n, dtype=torch.bfloat16 if i % 3 == 1 else torch.float32, device="cuda"))
+        p.grad = torch.randn(n, generator=gen).to(p.dtype).cuda()
+        params.append(p)
+    before = [p.grad.double() for p in params]
+    want = math.sqrt(sum(float(b.square().sum()) for b in before))
+    norm = clip_grad_norm_(params, want / 3)
+    # 64-bit sums of 32-bit squares: what is seen is the last rounding, to 32 bits
+    assert abs(float(norm) - want) <= (2 ** -24 + 2 ** -40) * want
+    f = want / 3 / (want + 1e-6)
+    for p, b in zip(params, before):
+        eps = 2 ** -8 if p.dtype == torch.bfloat16 else 2 ** -24
+        # the factor's rounding, the product's, and for bf16 the last one
+        assert ((p.grad.double() - b * f).abs() <= (eps + 2 * 2 ** -24) * (b * f).abs()).all()
