@@ -397,7 +397,7 @@ __global__ __launch_bounds__(256) void aw_prep_kernel(AwPrep a) {
 // Sums of squares in 64 bits: the norm then does not depend on the order of the sum in any of its 32 bits but by chance.
 // Bound by memory (a conversion and a 64-bit multiply-add an element fit beside it): 8192 elements are loaded before the
 // first is squared, 1024 workgroups give 16 waves a CU. 50 M fp32 in 36 us (5.6 TB/s; 4096 elements: 38, 512 workgroups: 52),
-// bf16 in 18; 67 M fp32 in 256 tensors, streamed, 48 us for both launches.
+// bf16 in 20; 67 M fp32 in 256 tensors, streamed, 46 us for both launches (55 with 128 tensors a launch).
 // 4 x 4 (bf16: 2 x 8) elements of a lane, in flight together
 template <bool BF16, bool FULL, bool NT>
 __device__ __forceinline__ double aw_squares(const void* g, long long i, long long n) {
