@@ -442,6 +442,10 @@ class DataParallelTrainer:
                         pass
                 raise conv_error
             if error is not None:
+                # a peer past its last collective may be handing over the checkpoint to resume
+                # from; one that waits for the lost rank is given up after this
+                if pending:
+                    runtime.wait(pending, num_returns=len(pending), timeout=1.0)
                 raise _WorkerFailure(error)
             for r, reports in enumerate(outs):
                 for metrics, ckpt in reports:

@@ -166,3 +166,29 @@ def test_rank_dying_after_the_final_report_resumes_from_the_last_epoch_checkpoin
     assert os.path.exists(os.path.join(res.restored_from[0], "meta.json"))
     finals = [m for m in res.metrics_history if m.get("final")]
     assert finals and finals[-1]["start"] == 3, res.metrics_history
+
+
+def _loop_dies_while_a_peer_reports(config):
+    import json
+    import time
+    from raydp_amd.train import Checkpoint, session
+    rank, ck = session.get_world_rank(), session.get_checkpoint()
+    if rank == 1 and not os.path.exists(config["flag"]):
+        open(config["flag"], "w").close()
+        os._exit(1)
+    if rank == 0 and ck is None:
+        time.sleep(0.3)                     # still busy with the epoch that its peer has left
+    d = session.staging_dir()
+    with open(os.path.join(d, "meta.json"), "w") as f:
+        json.dump({"epoch": 0}, f)
+    session.report({"resumed": ck is not None}, checkpoint=Checkpoint(d, movable=True) if rank == 0 else None)
+
+
+def test_a_peer_about_to_report_is_heard_before_the_group_is_restarted(runtime_local, tmp_path):
+    from raydp_amd.train import FailureConfig, RunConfig, ScalingConfig, TorchTrainer
+    tr = TorchTrainer(_loop_dies_while_a_peer_reports, train_loop_config={"flag": str(tmp_path / "died")},
+                      scaling_config=ScalingConfig(num_workers=2, use_gpu=False),
+                      run_config=RunConfig(storage_path=str(tmp_path / "runs"),
+                                           failure_config=FailureConfig(max_failures=1)))
+    res = tr.fit()
+    assert len(res.restored_from) == 1 and res.metrics["resumed"]
