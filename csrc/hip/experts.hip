@@ -80,7 +80,7 @@ struct Vec {
 //                  struck out by its index.
 // The order-preserving bits are the sign and magnitude as a number, shifted so that the magnitudes past infinity (NaN, of
 // either sign) wrap to the bottom: the least key of a chosen logit is the first above minus infinity's, and -0 equals 0.
-// The loop keeps winners as keys in LDS; what they stand for is worked out afterwards, a winner per lane.
+// A winner stays in its lane as the key; what it stands for is worked out afterwards.
 typedef short rx_s16x2 __attribute__((ext_vector_type(2)));
 
 template <int DT> struct Order;
@@ -128,12 +128,17 @@ __device__ __forceinline__ void wave_sync() {
 
 // lane ^ d within groups of L lanes
 __device__ __forceinline__ uint32_t lane_xor(uint32_t v, int d) { return (uint32_t)__shfl_xor((int)v, d); }
+// (every lane has its partner: saying that none is read as anything else lets the move become part of the maximum)
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true));
+}
 template <int L>
 __device__ __forceinline__ uint32_t group_max(uint32_t v) {
-  if constexpr (L >= 2) v = max(v, rx_dppu<RX_DPP_XOR1>(v));
-  if constexpr (L >= 4) v = max(v, rx_dppu<RX_DPP_XOR2>(v));
-  if constexpr (L >= 8) v = max(v, rx_dppu<RX_DPP_HALF_MIRROR>(v));
-  if constexpr (L >= 16) v = max(v, rx_dppu<RX_DPP_MIRROR>(v));
+  if constexpr (L >= 2) v = dpp_max<RX_DPP_XOR1>(v);
+  if constexpr (L >= 4) v = dpp_max<RX_DPP_XOR2>(v);
+  if constexpr (L >= 8) v = dpp_max<RX_DPP_HALF_MIRROR>(v);
+  if constexpr (L >= 16) v = dpp_max<RX_DPP_MIRROR>(v);
   if constexpr (L >= 32) v = max(v, lane_xor(v, 16));
   if constexpr (L >= 64) v = max(v, lane_xor(v, 32));
   return v;
@@ -186,7 +191,6 @@ template <int DT, int L, int V>
 __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>::type* __restrict__ z, long long ldz,
                                                         long long T, int E, int k, int renorm, float* __restrict__ w,
                                                         int* __restrict__ ids, float* __restrict__ norm) {
-  extern __shared__ uint2 taken[];          // [rows of the workgroup][k]: order, 0xFFFF - index
   constexpr int N = Elem<DT>::kVec;
   const int lane = threadIdx.x % L, first = lane * V;
   const long long t = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
@@ -203,8 +207,10 @@ __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>:
         if (at + q >= E) x[c].e[q] = Elem<DT>::put(-__builtin_huge_valf());
     }
   }
-  uint2* mine = taken + (threadIdx.x / L) * k;
-  uint32_t least = 0xFFFFFFFFu;             // a NaN's order is below minus infinity's
+  // lane j % L keeps winner j: no more than kSlots of them
+  constexpr int kSlots = V < kRouteMaxK / L ? V : L < kRouteMaxK ? kRouteMaxK / L : 1;
+  uint32_t won[kSlots], at[kSlots];         // order, 0xFFFF - index (16 bits: both in won)
+  uint32_t least = 0xFFFFFFFFu, top;        // a NaN's order is below minus infinity's; of the first winner
   if constexpr (DT == 0) {
     uint32_t hi[V], lo[V];
     const uint32_t low0 = 0xFFFFu - (uint32_t)first;
@@ -215,49 +221,75 @@ __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>:
       hi[i] = o >> 2;
       lo[i] = (o << 30) | (low0 - i);
     }
-    for (int j = 0; j < k; ++j) {
+    const auto largest = [&] {
       double best = as_key(hi[0], lo[0]);
 #pragma unroll
       for (int i = 1; i < V - 1; ++i) best = key_max<false>(best, as_key(hi[i], lo[i]));
-      best = group_max<L>(key_max<true>(best, as_key(hi[V - 1], lo[V - 1])));
-      const unsigned long long b = (unsigned long long)__double_as_longlong(best);
-      const uint32_t low = (uint32_t)b & 0xFFFFu;
-      if (lane == 0) mine[j] = make_uint2((uint32_t)(b >> 30), low);
-      // a winner loses its high word: what is left stands for less than minus infinity
-      const uint32_t at = low0 - low;
+      return (unsigned long long)__double_as_longlong(group_max<L>(key_max<true>(best, as_key(hi[V - 1], lo[V - 1]))));
+    };
+    unsigned long long last = largest();
+    top = (uint32_t)(last >> 30);
+    int j = 0;
 #pragma unroll
-      for (int i = 0; i < V; ++i) hi[i] = at == (uint32_t)i ? 0u : hi[i];
+    for (int r = 0; r < kSlots; ++r) {
+      won[r] = at[r] = 0;
+      for (int l = 0; l < L && j < k; ++l) {
+        const uint32_t o = (uint32_t)(last >> 30), low = (uint32_t)last & 0xFFFFu;
+        won[r] = lane == l ? o : won[r];
+        at[r] = lane == l ? low : at[r];
+        if (++j == k) break;
+        // a winner loses its high word: what is left stands for less than minus infinity
+        const uint32_t mine = low0 - low;
+#pragma unroll
+        for (int i = 0; i < V; ++i) hi[i] = mine == (uint32_t)i ? 0u : hi[i];
+        last = largest();
+      }
     }
   } else {
     uint32_t key[V];
-    const uint32_t low0 = 0xFFFFu - (uint32_t)first;
+    uint32_t low = 0xFFFFu - (uint32_t)first;
+    low |= (low - 1) << 16;
 #pragma unroll
     for (int i = 0; i < V; i += 2) {
-      const uint32_t o = order_pair<DT>(x[i / N].w[(i % N) / 2]);
-      key[i] = (o << 16) | (low0 - i);
-      key[i + 1] = (o & 0xFFFF0000u) | (low0 - i - 1);
+      const uint32_t o = order_pair<DT>(x[i / N].w[(i % N) / 2]), lows = low - i * 0x10001u;
+      key[i] = __builtin_amdgcn_perm(o, lows, 0x05040100u);        // (lower half of o, lower half of lows)
+      key[i + 1] = __builtin_amdgcn_perm(o, lows, 0x07060302u);    // (the upper halves)
       least = min(least, min(o << 16, o & 0xFFFF0000u));
     }
     least >>= 16;
-    uint32_t last = 0;
-    for (int j = 0; j < k; ++j) {
-      uint32_t best = key[0] - last;
+    uint32_t last = key[0];
 #pragma unroll
-      for (int i = 1; i < V; ++i) best = max(best, key[i] - last);
-      last += group_max<L>(best);
-      if (lane == 0) mine[j] = make_uint2(last >> 16, last & 0xFFFFu);
+    for (int i = 1; i < V; ++i) last = max(last, key[i]);
+    last = group_max<L>(last);
+    top = last >> 16;
+    int j = 0;
+#pragma unroll
+    for (int r = 0; r < kSlots; ++r) {
+      won[r] = 0;
+      for (int l = 0; l < L && j < k; ++l) {
+        won[r] = lane == l ? last : won[r];
+        if (++j == k) break;
+        uint32_t best = key[0] - last;
+#pragma unroll
+        for (int i = 1; i < V; ++i) best = max(best, key[i] - last);
+        last += group_max<L>(best);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kSlots; ++r) {
+      at[r] = won[r] & 0xFFFFu;
+      won[r] >>= 16;
     }
   }
-  wave_sync();                             // (a row's lanes are one wave's)
-  const uint32_t top = mine[0].x;
   const float peak = top > Order<DT>::kLowest ? order_back<DT>(top) : 0.f;
-  float total = 0.f;
-  if (renorm) {
-    for (int j = lane; j < k; j += L) {
-      const uint32_t o = mine[j].x;
-      if (o > Order<DT>::kLowest) total += exp_neg(order_back<DT>(o) - peak);
-    }
-  } else {
+  float part[kSlots], total = 0.f;
+#pragma unroll
+  for (int r = 0; r < kSlots; ++r) {
+    part[r] = won[r] > Order<DT>::kLowest ? exp_neg(order_back<DT>(won[r]) - peak) : 0.f;     // (no winner: 0)
+    total += part[r];
+  }
+  if (!renorm) {
+    total = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) total += exp_neg(Elem<DT>::get(x[i / N].e[i % N]) - peak);
   }
@@ -267,11 +299,12 @@ __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>:
   const int shift = (threadIdx.x & 63) / L * L;
   const bool any = ((rows >> shift) & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1)) != 0;
   const float inv = any ? __uint_as_float(0x7FC00000u) : total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-  for (int j = lane; j < k; j += L) {
-    const uint2 e = mine[j];
-    const bool there = e.x > Order<DT>::kLowest;
-    w[t * k + j] = (there ? exp_neg(order_back<DT>(e.x) - peak) : 0.f) * inv;
-    ids[t * k + j] = there ? (int)(0xFFFFu - e.y) : -1;
+#pragma unroll
+  for (int r = 0; r < kSlots; ++r) {
+    const int j = r * L + lane;
+    if (j >= k) break;
+    w[t * k + j] = part[r] * inv;
+    ids[t * k + j] = won[r] > Order<DT>::kLowest ? (int)(0xFFFFu - at[r]) : -1;
   }
   if (norm != nullptr && lane == 0) {
     norm[2 * t] = peak;
@@ -614,8 +647,8 @@ int route_launch(int bwd, const void* z, long long ldz, const float* norm, float
     hipLaunchKernelGGL((route_bwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), 0, stream, (const S*)z, ldz, norm,
                        w, ids, dw, T, E, k, (S*)dz);
   else
-    hipLaunchKernelGGL((route_fwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), sizeof(uint2) * (256 / L) * k,
-                       stream, (const S*)z, ldz, T, E, k, renorm, w, ids, norm_out);
+    hipLaunchKernelGGL((route_fwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), 0, stream, (const S*)z, ldz, T, E, k,
+                       renorm, w, ids, norm_out);
   return (int)hipGetLastError();
 }
 
