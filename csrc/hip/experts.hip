@@ -126,8 +126,7 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// lane ^ d within groups of L lanes
-__device__ __forceinline__ uint32_t lane_xor(uint32_t v, int d) { return (uint32_t)__shfl_xor((int)v, d); }
+// Maxima and sums over groups of L lanes.
 // (every lane has its partner: saying that none is read as anything else lets the move become part of the maximum)
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
@@ -139,8 +138,10 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
   if constexpr (L >= 4) v = dpp_max<RX_DPP_XOR2>(v);
   if constexpr (L >= 8) v = dpp_max<RX_DPP_HALF_MIRROR>(v);
   if constexpr (L >= 16) v = dpp_max<RX_DPP_MIRROR>(v);
-  if constexpr (L >= 32) v = max(v, lane_xor(v, 16));
-  if constexpr (L >= 64) v = max(v, lane_xor(v, 32));
+  if constexpr (L >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(p[0], p[1]);
+  }
   return v;
 }
 template <int L>
@@ -158,7 +159,7 @@ __device__ __forceinline__ double as_key(uint32_t hi, uint32_t lo) {
   return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
 }
 // No key is a NaN, which fmax() has to allow for with a second instruction an operand (65536 x 256, k = 8: 29 us with it, 25
-// without). LAST: the result is moved across lanes next, which needs two wait states that the compiler does not see here.
+// without it). LAST: the result is moved across lanes next, which needs two wait states that the compiler does not see here.
 template <bool LAST>
 __device__ __forceinline__ double key_max(double a, double b) {
   double r;
@@ -177,16 +178,20 @@ __device__ __forceinline__ double group_max(double v) {
   if constexpr (L >= 4) v = key_max<true>(v, dpp_key<RX_DPP_XOR2>(v));
   if constexpr (L >= 8) v = key_max<true>(v, dpp_key<RX_DPP_HALF_MIRROR>(v));
   if constexpr (L >= 16) v = key_max<true>(v, dpp_key<RX_DPP_MIRROR>(v));
-  if constexpr (L >= 32) v = key_max<true>(v, __shfl_xor(v, 16));
-  if constexpr (L >= 64) v = key_max<true>(v, __shfl_xor(v, 32));
+  if constexpr (L >= 32) {
+    const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+    const auto h = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+    const auto l = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+    v = key_max<true>(as_key(h[0], l[0]), as_key(h[1], l[1]));
+  }
   return v;
 }
 
 // e^x for x <= 0: relative error |x| 2^-24 and one ulp
 __device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 
-// Bound by instruction issue where k is large (65536 x 256, k = 8: 18 us in bf16, 25 in fp32, where reading takes 7 and 13),
-// by memory where it is small (262144 x 64, k = 2: 11 us in bf16, 15 in fp32; reading takes 7 and 13).
+// Bound by instruction issue where k is large (65536 x 256, k = 8: 14 us in bf16, 22 in fp32, where reading takes 7 and 13),
+// by memory where it is small (262144 x 64, k = 2: 9 us in bf16, 13 in fp32; reading takes 7 and 13).
 template <int DT, int L, int V>
 __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>::type* __restrict__ z, long long ldz,
                                                         long long T, int E, int k, int renorm, float* __restrict__ w,
@@ -195,16 +200,21 @@ __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>:
   const int lane = threadIdx.x % L, first = lane * V;
   const long long t = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
   if (t >= T) return;
-  // places past the row are minus infinity with indexes past the row's: k <= E, so they are never taken
   Vec<DT> x[V / N];
+  if (E == L * V) {                         // (a power of two of them: nothing to look at per lane)
 #pragma unroll
-  for (int c = 0; c < V / N; ++c) {
-    const int at = first + c * N;
-    x[c].load(z + t * ldz + (at < E ? at : 0), E - at);
-    if (at + N > E) {
+    for (int c = 0; c < V / N; ++c) x[c].load(z + t * ldz + first + c * N, N);
+  } else {
+    // places past the row are minus infinity with indexes past the row's: k <= E, so they are never taken
 #pragma unroll
-      for (int q = 0; q < N; ++q)
-        if (at + q >= E) x[c].e[q] = Elem<DT>::put(-__builtin_huge_valf());
+    for (int c = 0; c < V / N; ++c) {
+      const int at = first + c * N;
+      x[c].load(z + t * ldz + (at < E ? at : 0), E - at);
+      if (at + N > E) {
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+          if (at + q >= E) x[c].e[q] = Elem<DT>::put(-__builtin_huge_valf());
+      }
     }
   }
   // lane j % L keeps winner j: no more than kSlots of them
@@ -254,7 +264,7 @@ __global__ __launch_bounds__(256) void route_fwd_kernel(const typename Elem<DT>:
       const uint32_t o = order_pair<DT>(x[i / N].w[(i % N) / 2]), lows = low - i * 0x10001u;
       key[i] = __builtin_amdgcn_perm(o, lows, 0x05040100u);        // (lower half of o, lower half of lows)
       key[i + 1] = __builtin_amdgcn_perm(o, lows, 0x07060302u);    // (the upper halves)
-      least = min(least, min(o << 16, o & 0xFFFF0000u));
+      least = min(least, min(key[i], key[i + 1]));
     }
     least >>= 16;
     uint32_t last = key[0];
@@ -638,27 +648,46 @@ __global__ __launch_bounds__(256) void rows_gather_kernel(RowArgs a) {
 }
 
 template <int DT, int L, int V>
-int route_launch(int bwd, const void* z, long long ldz, const float* norm, float* w, int* ids, const float* dw,
-                 long long T, int E, int k, int renorm, float* norm_out, void* dz, hipStream_t stream) {
-  typedef typename Elem<DT>::type S;
+int route_fwd_launch(const void* z, long long ldz, long long T, int E, int k, int renorm, float* w, int* ids, float* norm,
+                     hipStream_t stream) {
   const long long grid = (T + 256 / L - 1) / (256 / L);
   if (grid > 0x7FFFFFFFll) return -1;
-  if (bwd)
-    hipLaunchKernelGGL((route_bwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), 0, stream, (const S*)z, ldz, norm,
-                       w, ids, dw, T, E, k, (S*)dz);
-  else
-    hipLaunchKernelGGL((route_fwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), 0, stream, (const S*)z, ldz, T, E, k,
-                       renorm, w, ids, norm_out);
+  hipLaunchKernelGGL((route_fwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), 0, stream,
+                     (const typename Elem<DT>::type*)z, ldz, T, E, k, renorm, w, ids, norm);
+  return (int)hipGetLastError();
+}
+template <int DT, int L, int V>
+int route_bwd_launch(const void* z, long long ldz, const float* norm, const float* w, const int* ids, const float* dw,
+                     long long T, int E, int k, void* dz, hipStream_t stream) {
+  const long long grid = (T + 256 / L - 1) / (256 / L);
+  if (grid > 0x7FFFFFFFll) return -1;
+  hipLaunchKernelGGL((route_bwd_kernel<DT, L, V>), dim3((unsigned)grid), dim3(256), 0, stream,
+                     (const typename Elem<DT>::type*)z, ldz, norm, w, ids, dw, T, E, k, (typename Elem<DT>::type*)dz);
   return (int)hipGetLastError();
 }
 
 // Lanes and logits per lane: the fewest lanes that hold a row in at most 16 logits each, since what crosses lanes is paid
-// per row and a wave then has 64 / L rows to overlap; a lane's logits are whole 16-byte loads.
+// per row and a wave then has 64 / L rows to overlap; a lane's logits are whole 16-byte loads. A forward of more than 256
+// takes 32 a lane (65536 rows, k = 8, 16 a lane and 32: 512 bf16 24 and 22 us, fp32 47 and 44; 1024 bf16 46 and 39, fp32 84 and
+// 79; 256 bf16 13.7 and 13.3, not worth the registers). A backward's rows in LDS would then leave room for too few.
 template <int DT>
-int route_pick(int bwd, const void* z, long long ldz, const float* norm, float* w, int* ids, const float* dw, long long T,
-               int E, int k, int renorm, float* norm_out, void* dz, hipStream_t stream) {
-#define RX_ROUTE(L, V) \
-  return route_launch<DT, L, V>(bwd, z, ldz, norm, w, ids, dw, T, E, k, renorm, norm_out, dz, stream)
+int route_fwd_pick(const void* z, long long ldz, long long T, int E, int k, int renorm, float* w, int* ids, float* norm,
+                   hipStream_t stream) {
+#define RX_ROUTE(L, V) return route_fwd_launch<DT, L, V>(z, ldz, T, E, k, renorm, w, ids, norm, stream)
+  if (E <= 8) RX_ROUTE(1, 8);
+  if (E <= 16) RX_ROUTE(2, 8);
+  if (E <= 32) RX_ROUTE(4, 8);
+  if (E <= 64) RX_ROUTE(4, 16);
+  if (E <= 128) RX_ROUTE(8, 16);
+  if (E <= 256) RX_ROUTE(16, 16);
+  if (E <= 512) RX_ROUTE(16, 32);
+  RX_ROUTE(32, 32);
+#undef RX_ROUTE
+}
+template <int DT>
+int route_bwd_pick(const void* z, long long ldz, const float* norm, const float* w, const int* ids, const float* dw,
+                   long long T, int E, int k, void* dz, hipStream_t stream) {
+#define RX_ROUTE(L, V) return route_bwd_launch<DT, L, V>(z, ldz, norm, w, ids, dw, T, E, k, dz, stream)
   if (E <= 8) RX_ROUTE(1, 8);
   if (E <= 16) RX_ROUTE(2, 8);
   if (E <= 32) RX_ROUTE(4, 8);
@@ -679,9 +708,9 @@ int rx_route_fwd(const void* z, long long ldz, int dtype, long long T, int E, in
   hipStream_t stream = static_cast<hipStream_t>(on);
   if (T < 0 || E <= 0 || E > kMaxExperts || k <= 0 || k > kRouteMaxK || k > E) return -1;
   if (T == 0) return 0;
-  if (dtype == 0) return route_pick<0>(0, z, ldz, nullptr, w, ids, nullptr, T, E, k, renorm, norm, nullptr, stream);
-  if (dtype == 1) return route_pick<1>(0, z, ldz, nullptr, w, ids, nullptr, T, E, k, renorm, norm, nullptr, stream);
-  if (dtype == 2) return route_pick<2>(0, z, ldz, nullptr, w, ids, nullptr, T, E, k, renorm, norm, nullptr, stream);
+  if (dtype == 0) return route_fwd_pick<0>(z, ldz, T, E, k, renorm, w, ids, norm, stream);
+  if (dtype == 1) return route_fwd_pick<1>(z, ldz, T, E, k, renorm, w, ids, norm, stream);
+  if (dtype == 2) return route_fwd_pick<2>(z, ldz, T, E, k, renorm, w, ids, norm, stream);
   return -1;
 }
 
@@ -690,11 +719,9 @@ int rx_route_bwd(const void* z, long long ldz, int dtype, const float* norm, con
   hipStream_t stream = static_cast<hipStream_t>(on);
   if (T < 0 || E <= 0 || E > kMaxExperts || k <= 0 || k > kRouteMaxK || k > E) return -1;
   if (T == 0) return 0;
-  float* wm = const_cast<float*>(w);
-  int* im = const_cast<int*>(ids);
-  if (dtype == 0) return route_pick<0>(1, z, ldz, norm, wm, im, dw, T, E, k, 0, nullptr, dz, stream);
-  if (dtype == 1) return route_pick<1>(1, z, ldz, norm, wm, im, dw, T, E, k, 0, nullptr, dz, stream);
-  if (dtype == 2) return route_pick<2>(1, z, ldz, norm, wm, im, dw, T, E, k, 0, nullptr, dz, stream);
+  if (dtype == 0) return route_bwd_pick<0>(z, ldz, norm, w, ids, dw, T, E, k, dz, stream);
+  if (dtype == 1) return route_bwd_pick<1>(z, ldz, norm, w, ids, dw, T, E, k, dz, stream);
+  if (dtype == 2) return route_bwd_pick<2>(z, ldz, norm, w, ids, dw, T, E, k, dz, stream);
   return -1;
 }
 
