@@ -453,3 +453,11 @@ def test_capturing_what_an_eager_call_made_is_refused(what):
         torch.cuda.synchronize()
         assert torch.equal(z.grad, torch.full_like(z, 2.0)) and torch.equal(y, held)
     del graph
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("E", [2, 4, 8, 9, 16, 32, 63, 64, 128, 256, 257, 511, 512, 513, 1024])
+@pytest.mark.parametrize("most", [True, False])
+def test_route_at_every_number_of_lanes(E, most, dtype):
+    """Rows that fill their lanes and rows that do not, as many winners as there may be and fewer."""
+    test_route_and_its_gradient(21, E, min(E, 32) if most else min(E, 5), not most, dtype)
