@@ -461,3 +461,75 @@ def test_capturing_what_an_eager_call_made_is_refused(what):
 def test_route_at_every_number_of_lanes(E, most, dtype):
     """Rows that fill their lanes and rows that do not, as many winners as there may be and fewer."""
     test_route_and_its_gradient(21, E, min(E, 32) if most else min(E, 5), not most, dtype)
+
+
+class _PlainRouted(nn.Module):
+    def __init__(self, capacity):
+        super().__init__()
+        self.router, self.out = nn.Linear(12, 4), nn.Linear(12, 1)
+        self.experts = nn.ModuleList(nn.Linear(12, 12) for _ in range(4))
+        self.capacity = capacity
+
+    def forward(self, x):
+        w, ids = route(self.router(x), 2)
+        p = expert_plan(ids, 4, self.capacity)
+        rows = dispatch(x, p).view(4, self.capacity, 12)
+        h = torch.cat([torch.relu(e(rows[i])) for i, e in enumerate(self.experts)])
+        return self.out(x + combine(h, p, w)).reshape(-1)
+
+
+def test_a_routed_model_in_the_graphed_training_loop(monkeypatch):
+    """TorchLoopEngine with the 8-bit optimizer: captured steps and eager ones end at the same bits."""
+    from raydp_amd.ops.fused_optim import FusedAdamW
+    from raydp_amd.torch.engine import TorchLoopEngine, _ShardTensors
+    from raydp_amd.torch.metrics import TorchMetric
+    from raydp_amd.train import session
+
+    class Shard(_ShardTensors):
+        def __init__(self, feats, labels):
+            self.feats, self.labels, self.n, self.multi = [feats], labels, labels.shape[0], False
+    g = torch.Generator().manual_seed(1)
+    x, y = torch.randn(32 * 12 + 5, 12, generator=g).cuda(), torch.randn(32 * 12 + 5, generator=g).cuda()
+
+    def trained(graphed):
+        monkeypatch.setenv("RAYDP_TORCH_GRAPHS", "1" if graphed else "0")
+        torch.manual_seed(0)
+        model = _PlainRouted(48).cuda()
+        opt = FusedAdamW(model.parameters(), lr=1e-2, max_grad_norm=1.0)
+        session._set_session(session._Session(session.TrainContext(), {}, lambda *a: None, "/tmp"))
+        try:
+            e = TorchLoopEngine(model, opt, nn.MSELoss(), TorchMetric(["MeanAbsoluteError"]), torch.device("cuda:0"),
+                                {"batch_size": 32, "shuffle": False, "drop_last": False}, None)
+            e.train = e.eval = Shard(x, y)
+            for _ in range(3):
+                e.train_epoch()
+        finally:
+            session._set_session(None)
+        assert (e.graphed is not None and e.graphed.failed is None and bool(e.graphed.graphs)) == graphed, e.graph_status
+        return model
+    a, b = trained(True), trained(False)
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert torch.equal(p, q)
+
+
+def test_a_routed_model_graphed_by_shape():
+    """graph_model holds the forward and the backward in a graph; the losses that the loop keeps do not matter to it."""
+    import copy
+    from raydp_amd.train.gpu_policy import graph_model
+    torch.manual_seed(0)
+    ref = _PlainRouted(48).cuda()
+    mine = copy.deepcopy(ref)
+    graph_model(mine)
+    g = torch.Generator().manual_seed(3)
+    for i in range(8):
+        x, y = torch.randn(32, 12, generator=g).cuda(), torch.randn(32, generator=g).cuda()
+        kept = [nn.functional.mse_loss(m(x), y) for m in (ref, mine)]
+        for loss, m in zip(kept, (ref, mine)):
+            m.zero_grad()
+            loss.backward()
+        assert float(kept[0]) == float(kept[1])
+        for p, q in zip(ref.parameters(), mine.parameters()):
+            assert torch.equal(p.grad, q.grad), i
+            with torch.no_grad():
+                p -= 0.1 * p.grad
+                q -= 0.1 * q.grad
