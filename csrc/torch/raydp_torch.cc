@@ -60,14 +60,17 @@ variable_list once(variable_list out) {
   return named;
 }
 
+bool capturing(c10::DeviceIndex device) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  check((int)hipStreamIsCapturing(c10::hip::getCurrentHIPStream(device).stream(), &status), "hipStreamIsCapturing");
+  return status != hipStreamCaptureStatusNone;
+}
+
 // Called by a backward of ours. A node of an eager call runs on that call's stream, and a leaf's gradient node is one of them
 // as long as anything holds the call's graph. The default stream can have no part in a capture: trying to ends the process.
 // What the pass would reach of that kind is found here first, and the call refused.
 void check_capturable(const Tensor& t) {
-  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  const auto on = c10::hip::getCurrentHIPStream(t.get_device());
-  check((int)hipStreamIsCapturing(on.stream(), &status), "hipStreamIsCapturing");
-  if (status == hipStreamCaptureStatusNone) return;
+  if (!capturing(t.get_device())) return;
   using torch::autograd::Node;
   const auto self = torch::autograd::get_current_node();
   if (!self) return;
@@ -238,10 +241,15 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
     const py::object lr = o["lr"];
     if (THPVariable_Check(lr.ptr())) {
       const Tensor l = THPVariable_Unpack(lr.ptr());
-      if (!l.is_cuda()) grp.lr = l.item<double>();
-      else if (l.scalar_type() != at::kFloat || l.device() != params[0].device())
+      if (!l.is_cuda()) {
+        if (capturing(params[0].get_device()))
+          throw std::runtime_error("FusedAdamW: a tensor lr on the host cannot be captured into a graph, whose replays would "
+                                   "keep its value: put it on the parameters' device");
+        grp.lr = l.item<double>();
+      } else if (l.scalar_type() != at::kFloat || l.device() != params[0].device())
         throw py::type_error("FusedAdamW: a tensor lr must be fp32 on the parameters' device");
-      else grp.lr_dev = ptr<float>(l);
+      else
+        grp.lr_dev = ptr<float>(l);
     } else {
       grp.lr = lr.cast<double>();
     }

@@ -177,7 +177,8 @@ class FusedAdamW(torch.optim.Optimizer):
                         is ``self.grad_norm``, on the device). A step whose norm is not finite is left out: parameters,
                         moments and step counts stay as they are. None: no clipping, nothing is left out.
     ``lr``              a number, or a 0-dim fp32 tensor on the parameters' device (read by the kernel: a captured step
-                        sees what a scheduler fills in).
+                        sees what a scheduler fills in). A tensor on the host is read at every step and cannot be captured;
+                        ``load_state_dict`` moves one to the parameters' device.
 
     State per parameter: ``step`` (0-dim fp32 on the parameter's device), ``exp_avg``, ``exp_avg_sq`` (uint8 codes or
     fp32) and, for 8 bits, ``scales`` (uint8 ``[ceil(n / 256), 2]``); :func:`decode_moments` gives their values.
@@ -236,6 +237,9 @@ class FusedAdamW(torch.optim.Optimizer):
         saved = state_dict["state"]
         super().load_state_dict(state_dict)
         self._fill_groups()
+        for g in self.param_groups:      # a checkpoint's rate is read where the step is: a captured one sees what is filled in
+            if isinstance(g["lr"], torch.Tensor) and not g["lr"].is_cuda and g["params"] and g["params"][0].is_cuda:
+                g["lr"] = g["lr"].detach().to(g["params"][0].device, torch.float32)
         # torch casts floating state to the parameter's type and codes with it: put the saved bits back
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [(g, p) for g in self.param_groups for p in g["params"]]

@@ -15,7 +15,8 @@ Rules that keep it exact:
   library workspaces), as graph capture requires;
 * Adam/AdamW switch to ``capturable=True`` (device-side step counters; ``FusedAdamW`` always keeps
   them there); with an LR scheduler the learning rate becomes a device tensor that the scheduler
-  ``fill_``s, and chunk = 1 so every step sees its own LR;
+  ``fill_``s, and chunk = 1 so every step sees its own LR; a rate that is a tensor on the host (one
+  read from a checkpoint) is moved to the device;
 * metric state is zeroed in place between epochs (``TorchMetric.zero_``) so the captured
   accumulation keeps pointing at live storage;
 * list indices in user models (``x[:, [1, 7, 8]]`` as in the reference tutorial's NET_Model) are
@@ -108,7 +109,10 @@ class GraphedTrainLoop:
             for g in opt.param_groups:
                 if not isinstance(opt, FusedAdamW):
                     g["capturable"] = True   # (the fused kernel ignores it but step() checks it)
-                if self.e.scheduler is not None and not isinstance(g["lr"], torch.Tensor):
+                if isinstance(g["lr"], torch.Tensor):
+                    if g["lr"].device != dev:    # (a checkpoint's, or the user's own: a replay does not read the host)
+                        g["lr"] = g["lr"].detach().to(device=dev, dtype=torch.float32)
+                elif self.e.scheduler is not None:
                     g["lr"] = torch.tensor(float(g["lr"]), dtype=torch.float32, device=dev)
             for st in opt.state.values():
                 if "step" in st and isinstance(st["step"], torch.Tensor):

@@ -1,0 +1,115 @@
+"""FusedAdamW on the GPU where a step's arithmetic, its rate's place or its tensors' sizes are at a border."""
+import io
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+from raydp_amd.ops.fused_optim import FusedAdamW, clip_grad_norm_, decode_moments
+
+from adamw_oracle import Oracle
+
+pytestmark = pytest.mark.gpu
+
+
+def _nan(dtype, word):
+    if dtype == torch.bfloat16:
+        return torch.tensor([word - (1 << 16) if word >> 15 else word], dtype=torch.int16).view(dtype).cuda()
+    return torch.tensor([word - (1 << 32) if word >> 31 else word], dtype=torch.int32).view(dtype).cuda()
+
+
+def test_a_rate_on_the_host_is_not_captured():
+    """A replay would go on with the rate that the capture saw."""
+    p = torch.ones(300, device="cuda", requires_grad=True)
+    p.grad = torch.ones(300, device="cuda")
+    opt = FusedAdamW([p], lr=torch.tensor(1e-3))
+    opt.step()
+    keep = p.detach().clone()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="lr"):
+            opt.step()
+    torch.cuda.synchronize()
+    assert torch.equal(p.detach(), keep)
+    opt.param_groups[0]["lr"] = opt.param_groups[0]["lr"].cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for lr in (0.0, 0.25):
+        opt.param_groups[0]["lr"].fill_(lr)
+        keep = p.detach().clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(p.detach(), keep) == (lr == 0.0)
+
+
+def _train(make, schedule, graphed, monkeypatch, resume):
+    """Epochs of the torch-loop engine on a small MLP; with ``resume`` on a model, optimizer and scheduler that take over
+    what a first engine left after one epoch, read back onto the host as a worker that restarts does."""
+    from raydp_amd.torch.engine import TorchLoopEngine, _ShardTensors
+    from raydp_amd.torch.metrics import TorchMetric
+    from raydp_amd.train import session
+
+    class Shard(_ShardTensors):
+        def __init__(self, feats, labels):
+            self.feats, self.labels, self.n, self.multi = [feats], labels, labels.shape[0], False
+    monkeypatch.setenv("RAYDP_TORCH_GRAPHS", "1" if graphed else "0")
+    session._set_session(session._Session(session.TrainContext(), {}, lambda *a: None, "/tmp"))
+    dev, saved = torch.device("cuda:0"), None
+    try:
+        for part in range(1 + resume):
+            torch.manual_seed(0)
+            model = nn.Sequential(nn.Linear(12, 64), nn.ReLU(), nn.Linear(64, 1))
+            if saved is not None:
+                model.load_state_dict(saved[0])
+            model.to(dev)
+            opt = make(model.parameters())
+            sch = schedule(opt)
+            if saved is not None:
+                opt.load_state_dict(torch.load(io.BytesIO(saved[1]), map_location="cpu", weights_only=True))
+                sch.load_state_dict(torch.load(io.BytesIO(saved[2]), weights_only=True))
+            e = TorchLoopEngine(model, opt, nn.MSELoss(), TorchMetric(["MeanAbsoluteError"]), dev,
+                                {"batch_size": 32, "shuffle": True, "drop_last": False}, sch)
+            g = torch.Generator().manual_seed(1)
+            e.train = Shard(torch.randn(32 * 9 + 5, 12, generator=g).to(dev), torch.randn(32 * 9 + 5, 1, generator=g).to(dev))
+            for _ in range(1 if resume and part == 0 else 2):
+                e.train_epoch()
+            torch.cuda.synchronize()
+            files = io.BytesIO(), io.BytesIO()
+            torch.save(e.optimizer_state_dict(), files[0])
+            torch.save(sch.state_dict(), files[1])
+            saved = ({k: v.detach().cpu().clone() for k, v in e.state_dict().items()}, *(f.getvalue() for f in files))
+            graphs, lr = e.graphed, opt.param_groups[0]["lr"]
+            e.close()
+        return saved[0], graphs, lr
+    finally:
+        session._set_session(None)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_resumed_graphed_loop_follows_the_schedule(bits, monkeypatch):
+    """(The graphed loop holds the rate in fp32: so does the eager one here.)"""
+    a, graphs, lr = _train(lambda ps: FusedAdamW(ps, lr=1e-2, state_bits=bits), _halving, True, monkeypatch, True)
+    assert graphs.failed is None and lr.is_cuda
+    b, _, want = _train(lambda ps: FusedAdamW(ps, lr=torch.tensor(1e-2), state_bits=bits), _halving, False, monkeypatch, True)
+    assert float(lr) == float(want)
+    for k in b:
+        assert torch.equal(a[k], b[k]), k
+
+
+def _halving(opt):
+    return torch.optim.lr_scheduler.StepLR(opt, step_size=3, gamma=0.5)
+
+
+@pytest.mark.parametrize("cls", [torch.optim.AdamW, FusedAdamW])
+def test_a_host_rate_under_a_schedule_is_moved_to_the_device(cls, monkeypatch):
+    """torch's AdamW takes a rate of its own tensor only in its capturable form, which the graphed loop asks for."""
+    kw = {} if cls is FusedAdamW else {"capturable": True}
+    _, graphs, lr = _train(lambda ps: cls(ps, lr=torch.tensor(1e-2), **kw), _halving, True, monkeypatch, False)
+    assert graphs.failed is None and graphs.graphs is not None and lr.is_cuda
+    assert float(lr) == pytest.approx(1e-2 * 0.5 ** (20 // 3))
+
+
+# lengths around a wave's two scale blocks (512 elements), a step's workgroups (2048) and a norm's (8192)
+EDGES = [511, 512, 513, 767, 768, 769, 1024, 1535, 1536, 1537, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 8192, 8193, 16384, 16385]
