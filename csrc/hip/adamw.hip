@@ -205,7 +205,7 @@ struct AwPlace {       // where a launch's workgroup works (wave-uniform)
 };
 
 // One lane's share of a scale block: 4 elements. FULL: the block lies inside the tensor and the vectors are aligned, so
-// loads and stores are whole and nothing branches; otherwise element by element under the tensor's end.
+// loads and stores are whole and no lane branches; otherwise element by element under the tensor's end.
 template <bool BITS8, bool BF16, bool NT, bool FULL>
 struct AwLane {
   f32x4 p, g, m, v;
@@ -240,6 +240,7 @@ struct AwLane {
     uint32_t mtop = 0, vtop = 0;
     uint32_t x = 0;
     if constexpr (BITS8 || BF16) x = (uint32_t)i * kPhi + (uint32_t)((unsigned long long)i >> 32) * kSq2 + k.key;
+    float root[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       {
@@ -248,8 +249,20 @@ struct AwLane {
         m[q] = b1 * m[q] + c.omb1 * gq;
         v[q] = b2 * v[q] + c.omb2 * (gq * gq);
       }
+      root[q] = __builtin_amdgcn_sqrtf(v[q]);
+    }
+    // The instruction takes subnormals, whose roots are under 2^-63, for 0: nothing in a denominator with eps of 2^38 times
+    // that (under half a step of it), an infinite update with eps = 0. (One branch for the launch's eps: 48 M bf16 with 8 bits
+    // 101 -> 102 us; scaling every root 108, a second kernel path for such an eps 104.)
+    if (__builtin_expect(c.eps < k.rs_bc2 * 0x1p-38f, 0)) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (v[q] < 0x1p-126f) root[q] = ldexpf(__builtin_amdgcn_sqrtf(ldexpf(v[q], 32)), -16);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
       // square root and quotient to 1 ulp each: the update is about 1e-3 of p
-      const float den = fmaf(__builtin_amdgcn_sqrtf(v[q]), k.rs_bc2, c.eps);
+      const float den = fmaf(root[q], k.rs_bc2, c.eps);
       p[q] = fmaf(k.nlr_bc1, m[q] * __builtin_amdgcn_rcpf(den), p[q] * k.decay);
       if (FULL || q < left) {
         mtop = max(mtop, __float_as_uint(m[q]) & 0x7FFFFFFFu);

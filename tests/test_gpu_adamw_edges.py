@@ -19,6 +19,20 @@ def _nan(dtype, word):
     return torch.tensor([word - (1 << 32) if word >> 31 else word], dtype=torch.int32).view(dtype).cuda()
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("power", [-60, -62, -63, -64, -66, -70, -73, -74])
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -64, 2.0 ** -39, 2.0 ** -38, 1e-8])
+def test_second_moments_under_the_normal_range(power, bits, eps):
+    """A gradient of 2^power: its square is exact, subnormal from 2^-64 on. With both betas 0 the update is
+    lr / (1 + eps / |g|). Half steps of 2^-24: the root 2, quotient 2, two constants and three products and sums 5: under
+    10 with their products."""
+    p = torch.zeros(600, device="cuda", requires_grad=True)
+    p.grad = torch.full((600,), 2.0 ** power, device="cuda")
+    FusedAdamW([p], lr=0.5, betas=(0.0, 0.0), eps=eps, weight_decay=0.0, state_bits=bits).step()
+    want = 0.5 / (1.0 + eps / 2.0 ** power)
+    assert ((p.detach().double() + want).abs() <= want * 10 * 2.0 ** -24).all(), p[0]
+
+
 def test_a_rate_on_the_host_is_not_captured():
     """A replay would go on with the rate that the capture saw."""
     p = torch.ones(300, device="cuda", requires_grad=True)
