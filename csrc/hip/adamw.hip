@@ -56,7 +56,7 @@ __device__ __forceinline__ uint32_t aw_wavemax(uint32_t v) {
   return max(q[0], q[1]);
 }
 
-// biased scale exponent of a block from the largest magnitude's bits (NaN and infinity: 255 or more)
+// biased scale exponent of a block from the largest magnitude's bits without a sign (NaN and infinity: 255 or more)
 __device__ __forceinline__ int aw_scale(uint32_t top) { return (int)((top + 0xFFFFFu) >> 23); }
 __device__ __forceinline__ int aw_exp(int s) { return (s > 0 ? s : 1) - 127; }
 
@@ -266,13 +266,13 @@ struct AwLane {
       p[q] = fmaf(k.nlr_bc1, m[q] * __builtin_amdgcn_rcpf(den), p[q] * k.decay);
       if (FULL || q < left) {
         mtop = max(mtop, __float_as_uint(m[q]) & 0x7FFFFFFFu);
-        vtop = max(vtop, __float_as_uint(v[q]));       // (not negative, or NaN)
+        vtop = max(vtop, __float_as_uint(v[q]));       // (a NaN's sign: the largest of all)
       }
       // (a lane's 4 indexes do not cross 2^32)
       if constexpr (BITS8 || BF16) h[q] = aw_mix(x + q * kPhi);
     }
     if constexpr (BITS8) {
-      const int sm1 = aw_scale(aw_wavemax(mtop)), sv1 = aw_scale(aw_wavemax(vtop));
+      const int sm1 = aw_scale(aw_wavemax(mtop)), sv1 = aw_scale(aw_wavemax(vtop) & 0x7FFFFFFFu);
       const int em = aw_exp(sm1), ev = aw_exp(sv1);
       uint32_t me[4], ve[4];
 #pragma unroll

@@ -59,8 +59,9 @@ def _blocks(x):
 
 
 def _encode(x, rnd16, emin):
-    """(codes, biased scale exponents) of blocks of non-negative fp32 values: 3 mantissa bits, normal from 2^emin."""
-    s = (x.view(torch.int32).long().amax(1) + 0xFFFFF) >> 23
+    """(codes, biased scale exponents) of blocks of non-negative fp32 values: 3 mantissa bits, normal from 2^emin. A scale of
+    255 marks a block with a NaN (of any sign and payload) or an infinity."""
+    s = (((x.view(torch.int32) & 0x7FFFFFFF).long().amax(1) + 0xFFFFF) >> 23).clamp(max=255)
     y = x.double() * _pow2(127 - s.clamp(min=1))[:, None]
     f = ((y.view(torch.int64) >> 52) - 1023).clamp(min=emin)
     code = ((torch.round(y * _pow2(3 - f) * 2.0 ** 20).long() + rnd16 * 16 + 8) >> 20) + 8 * (f - emin)

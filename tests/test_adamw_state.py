@@ -1,0 +1,52 @@
+"""FusedAdamW's coded state where values are not numbers, the states it loads, its options, and its norm (no GPU needed)."""
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+from raydp_amd.ops.fused_optim import FusedAdamW, decode_moments
+
+# quiet NaNs of either sign: the plain ones, all bits set, and what a bf16 NaN of all bits widens to
+NANS = [0x7FC00000, 0xFFC00000, 0x7FFFFFFF, 0xFFFFFFFF, 0x7FFF0000, 0xFFFF0000]
+
+
+def _bits(word):
+    return torch.tensor([word - (1 << 32) if word >> 31 else word], dtype=torch.int32).view(torch.float32)
+
+
+@pytest.mark.parametrize("word", NANS, ids=hex)
+def test_any_nan_in_a_gradient_shows_in_both_moments_of_its_block(word):
+    p = torch.ones(600, requires_grad=True)
+    p.grad = torch.full((600,), 0.1)
+    opt = FusedAdamW([p])
+    opt.step()
+    p.grad[300:301] = _bits(word)
+    assert torch.isnan(p.grad[300])
+    opt.step()
+    st = opt.state[p]
+    for t in decode_moments(st["exp_avg"], st["exp_avg_sq"], st["scales"]):
+        assert torch.isnan(t[256:512]).all() and torch.isfinite(t[:256]).all() and torch.isfinite(t[512:]).all()
+
+
+@pytest.mark.parametrize("word", NANS, ids=hex)
+def test_a_loaded_state_with_a_nan_in_either_moment(word):
+    for name, which in (("exp_avg", 0), ("exp_avg_sq", 1)):
+        p, q = (torch.ones(600, requires_grad=True) for _ in range(2))
+        p.grad = torch.full((600,), 0.1)
+        src, dst = torch.optim.AdamW([p]), FusedAdamW([q])
+        src.step()
+        src.state[p][name][300:301] = _bits(word)
+        dst.load_state_dict(src.state_dict())
+        st = dst.state[q]
+        got = decode_moments(st["exp_avg"], st["exp_avg_sq"], st["scales"])
+        assert torch.isnan(got[which][256:512]).all() and torch.isfinite(got[which][:256]).all()
+        assert torch.isfinite(got[1 - which]).all()
+
+
+def _state(cls, **kw):
+    p = torch.ones(300, requires_grad=True)
+    p.grad = torch.full((300,), 0.1)
+    opt = cls([p], **kw)
+    opt.step()
+    return opt.state_dict()

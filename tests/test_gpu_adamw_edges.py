@@ -19,6 +19,24 @@ def _nan(dtype, word):
     return torch.tensor([word - (1 << 32) if word >> 31 else word], dtype=torch.int32).view(dtype).cuda()
 
 
+@pytest.mark.parametrize("dtype,word", [(torch.float32, w) for w in (0x7FC00000, 0xFFC00000, 0x7FFFFFFF, 0xFFFFFFFF)] +
+                         [(torch.bfloat16, w) for w in (0x7FC0, 0xFFC0, 0x7FFF, 0xFFFF)], ids=str)
+def test_any_nan_in_a_gradient_shows_in_both_moments_of_its_block(dtype, word):
+    n = 2600                                     # whole blocks of a wave, and what is left behind them
+    p = torch.ones(n, dtype=dtype, device="cuda", requires_grad=True)
+    p.grad = torch.full((n,), 0.1, dtype=dtype, device="cuda")
+    opt = FusedAdamW([p])
+    opt.step()
+    for at in (300, n - 1):
+        p.grad[at:at + 1] = _nan(dtype, word)
+    opt.step()
+    st = opt.state[p]
+    bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+    bad[256:512] = bad[2560:] = True
+    for t in decode_moments(st["exp_avg"], st["exp_avg_sq"], st["scales"]):
+        assert torch.equal(torch.isnan(t), bad)
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 @pytest.mark.parametrize("power", [-60, -62, -63, -64, -66, -70, -73, -74])
 @pytest.mark.parametrize("eps", [0.0, 2.0 ** -64, 2.0 ** -39, 2.0 ** -38, 1e-8])
