@@ -16,7 +16,8 @@ Rules that keep it exact:
 * Adam/AdamW switch to ``capturable=True`` (device-side step counters; ``FusedAdamW`` always keeps
   them there); with an LR scheduler the learning rate becomes a device tensor that the scheduler
   ``fill_``s, and chunk = 1 so every step sees its own LR; a rate that is a tensor on the host (one
-  read from a checkpoint) is moved to the device;
+  read from a checkpoint) is moved to the device. Anything else that a scheduler changes (the betas,
+  under OneCycleLR) is a constant of a captured step: the loop goes on eagerly once one has changed;
 * metric state is zeroed in place between epochs (``TorchMetric.zero_``) so the captured
   accumulation keeps pointing at live storage;
 * list indices in user models (``x[:, [1, 7, 8]]`` as in the reference tutorial's NET_Model) are
@@ -99,6 +100,7 @@ class GraphedTrainLoop:
         self.warm = 0
         self.failed = None
         self.index_cache = {}
+        self.options = None        # of the optimizer, as captured (under a scheduler)
         self.total = torch.zeros((), dtype=torch.float64, device=engine.device)
         self._prepare_optimizer()
 
@@ -117,6 +119,11 @@ class GraphedTrainLoop:
             for st in opt.state.values():
                 if "step" in st and isinstance(st["step"], torch.Tensor):
                     st["step"] = st["step"].to(device=dev, dtype=torch.float32)
+
+    def _options(self):
+        """The optimizer's options that a captured step holds as constants."""
+        return [{k: v for k, v in g.items() if k != "params" and not isinstance(v, torch.Tensor)}
+                for g in self.e.optimizer.param_groups]
 
     # ------------------------------------------------------------------ step bodies
     def _forward_step(self, feats, lab):
@@ -160,27 +167,36 @@ class GraphedTrainLoop:
         if self.pool is None:
             self.pool = g.pool()
         self.graphs[steps] = (g, win)
+        if self.e.scheduler is not None and self.options is None:
+            self.options = self._options()
         return g, win
 
     def _replay(self, steps: int, sel):
         ent = self.graphs.get(steps)
+        if ent is not None and self.options is not None and self._options() != self.options:
+            names = {k for a, b in zip(self._options(), self.options) for k in a if a[k] != b.get(k)}
+            return self._give_up(f"the scheduler changed {', '.join(sorted(names))}", steps, sel)
         if ent is None:
             try:
                 ent = self._capture(steps)
             except Exception as exc:   # capture is best effort: fall back to eager for good
-                self.failed = f"{type(exc).__name__}: {exc}\n" + "".join(traceback.format_tb(exc.__traceback__)[-4:])
-                self.graphs.clear()
-                torch.cuda.synchronize(self.e.device)
-                self.e.zero_grad()
-                b = self.e.batch
-                for j in range(steps):
-                    self._eager(sel[j * b:(j + 1) * b])
-                return
+                return self._give_up(f"{type(exc).__name__}: {exc}\n" + "".join(traceback.format_tb(exc.__traceback__)[-4:]),
+                                     steps, sel)
         g, win = ent
         win.copy_(sel)
         g.replay()
         if self.e.scheduler is not None:
             self.e.scheduler.step()
+
+    def _give_up(self, why, steps, sel):
+        """Run these batches, and all after them, eagerly."""
+        self.failed = why
+        torch.cuda.synchronize(self.e.device)
+        self.graphs.clear()
+        self.e.zero_grad()
+        b = self.e.batch
+        for j in range(steps):
+            self._eager(sel[j * b:(j + 1) * b])
 
     def close(self):
         """Destroy the captured graphs and their pool (no capture may be running)."""

@@ -143,5 +143,17 @@ def test_a_host_rate_under_a_schedule_is_moved_to_the_device(cls, monkeypatch):
     assert float(lr) == pytest.approx(1e-2 * 0.5 ** (20 // 3))
 
 
+def test_a_schedule_that_moves_the_betas(monkeypatch):
+    """OneCycleLR changes betas too, which a captured step has as constants."""
+    def cycle(opt):
+        return torch.optim.lr_scheduler.OneCycleLR(opt, max_lr=1e-2, total_steps=30)
+    a, b = (_train(lambda ps: FusedAdamW(ps, lr=torch.tensor(1e-3), state_bits=32), cycle, graphed, monkeypatch, False)[0]
+            for graphed in (True, False))
+    for k in b:
+        assert torch.equal(a[k], b[k]), k
+    _, graphs, _ = _train(lambda ps: torch.optim.AdamW(ps, lr=1e-3), cycle, True, monkeypatch, False)
+    assert "betas" in graphs.failed
+
+
 # lengths around a wave's two scale blocks (512 elements), a step's workgroups (2048) and a norm's (8192)
 EDGES = [511, 512, 513, 767, 768, 769, 1024, 1535, 1536, 1537, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 8192, 8193, 16384, 16385]
