@@ -183,7 +183,8 @@ class FusedAdamW(torch.optim.Optimizer):
 
     State per parameter: ``step`` (0-dim fp32 on the parameter's device), ``exp_avg``, ``exp_avg_sq`` (uint8 codes or
     fp32) and, for 8 bits, ``scales`` (uint8 ``[ceil(n / 256), 2]``); :func:`decode_moments` gives their values.
-    ``load_state_dict`` also takes the state of a ``torch.optim.AdamW`` and codes its moments.
+    ``load_state_dict`` also takes the state of a ``torch.optim.AdamW`` and codes its moments; one with ``amsgrad``, or of a
+    ``torch.optim.Adam`` whose ``weight_decay`` meant another thing, raises before anything is changed.
 
     Parameters are contiguous fp32 or bf16; gradients are dense and of the parameter's type. Sparse gradients, parameters
     that share memory, a first step inside a graph capture raise."""
@@ -236,30 +237,33 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         saved = state_dict["state"]
+        # torch casts floating state to the parameter's type and codes with it: the saved bits are put back below
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        mine = [p for g in self.param_groups for p in g["params"]]
+        for k, (i, p) in enumerate(zip(ids, mine)):
+            if saved.get(i):
+                self._check_saved(saved[i], k, p)
+        for g in state_dict["param_groups"]:
+            if g.get("amsgrad"):
+                raise ValueError("FusedAdamW: the state is of an amsgrad optimizer, whose largest second moments it does not keep")
+            if g.get("weight_decay") and g.get("decoupled_weight_decay") is False:
+                raise ValueError("FusedAdamW: the state is of an Adam whose weight_decay was added to the gradients; here "
+                                 "it shrinks the parameters (for that, set decoupled_weight_decay in the state's group)")
         super().load_state_dict(state_dict)
         self._fill_groups()
         for g in self.param_groups:      # a checkpoint's rate is read where the step is: a captured one sees what is filled in
             if isinstance(g["lr"], torch.Tensor) and not g["lr"].is_cuda and g["params"] and g["params"][0].is_cuda:
                 g["lr"] = g["lr"].detach().to(g["params"][0].device, torch.float32)
-        # torch casts floating state to the parameter's type and codes with it: put the saved bits back
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [(g, p) for g in self.param_groups for p in g["params"]]
-        for k, (i, (g, p)) in enumerate(zip(ids, params)):
+        for i, (g, p) in zip(ids, params):
             src = saved.get(i)
             if not src:
                 continue
-            if any(n not in src for n in ("step", "exp_avg", "exp_avg_sq")):
-                raise ValueError(f"FusedAdamW: state of parameter {k} lacks step, exp_avg or exp_avg_sq")
-            step = src["step"]
-            st = {"step": torch.as_tensor(step, dtype=torch.float32).detach().clone().to(p.device)}
+            st = {"step": torch.as_tensor(src["step"], dtype=torch.float32).detach().clone().to(p.device)}
             m, v = (src[n].detach().to(p.device) for n in ("exp_avg", "exp_avg_sq"))
-            if m.shape != p.shape or v.shape != p.shape:
-                raise ValueError(f"FusedAdamW: moments of parameter {k} are {tuple(m.shape)}, the parameter is {tuple(p.shape)}")
             coded = m.dtype == torch.uint8
             if coded:
                 sc = src["scales"].detach().to(p.device, copy=True).contiguous()
-                if v.dtype != torch.uint8 or sc.dtype != torch.uint8 or sc.numel() != 2 * _scale_rows(p.numel()):
-                    raise ValueError(f"FusedAdamW: 8-bit state of parameter {k} is incomplete")
             m, v = (t.clone(memory_format=torch.contiguous_format) for t in (m, v))
             if g["state_bits"] == 8:
                 if not coded:
@@ -270,6 +274,18 @@ class FusedAdamW(torch.optim.Optimizer):
                 m, v = decode_moments(m, v, sc) if coded else (m.float(), v.float())
                 st.update(exp_avg=m, exp_avg_sq=v)
             self.state[p] = st
+
+    @staticmethod
+    def _check_saved(src, k, p):
+        if any(n not in src for n in ("step", "exp_avg", "exp_avg_sq")):
+            raise ValueError(f"FusedAdamW: state of parameter {k} lacks step, exp_avg or exp_avg_sq")
+        m, v = src["exp_avg"], src["exp_avg_sq"]
+        if m.shape != p.shape or v.shape != p.shape:
+            raise ValueError(f"FusedAdamW: moments of parameter {k} are {tuple(m.shape)}, the parameter is {tuple(p.shape)}")
+        if torch.uint8 in (m.dtype, v.dtype):
+            sc = src.get("scales")
+            if sc is None or m.dtype != v.dtype or sc.dtype != torch.uint8 or sc.numel() != 2 * _scale_rows(p.numel()):
+                raise ValueError(f"FusedAdamW: 8-bit state of parameter {k} is incomplete")
 
     def _new_state(self, p, bits):
         """The parameter's state, made with its first gradient."""

@@ -50,3 +50,34 @@ def _state(cls, **kw):
     opt = cls([p], **kw)
     opt.step()
     return opt.state_dict()
+
+
+@pytest.mark.parametrize("make,match", [
+    (lambda: _state(torch.optim.AdamW, amsgrad=True), "amsgrad"),
+    (lambda: _state(torch.optim.Adam, amsgrad=True), "amsgrad"),
+    (lambda: _state(torch.optim.Adam, weight_decay=0.1), "weight_decay")])
+def test_a_state_that_means_something_else_is_refused_and_changes_nothing(make, match):
+    q = torch.ones(300, requires_grad=True)
+    q.grad = torch.full((300,), 0.1)
+    opt = FusedAdamW([q], lr=0.25)
+    opt.step()
+    before = {n: t.clone() for n, t in opt.state[q].items()}
+    with pytest.raises(ValueError, match=match):
+        opt.load_state_dict(make())
+    assert opt.param_groups[0]["lr"] == 0.25 and all(torch.equal(opt.state[q][n], t) for n, t in before.items())
+
+
+def test_an_adam_state_without_decay_is_taken():
+    opt = FusedAdamW([torch.ones(300, requires_grad=True)], state_bits=32)
+    want = _state(torch.optim.Adam, lr=0.5)
+    opt.load_state_dict(want)
+    (st,) = opt.state.values()
+    assert opt.param_groups[0]["lr"] == 0.5 and torch.equal(st["exp_avg"], want["state"][0]["exp_avg"])
+
+
+def test_an_incomplete_coded_state_is_refused():
+    for name in ("scales", "step", "exp_avg", "exp_avg_sq"):
+        sd = _state(FusedAdamW)
+        del sd["state"][0][name]
+        with pytest.raises(ValueError, match="FusedAdamW"):
+            FusedAdamW([torch.ones(300, requires_grad=True)]).load_state_dict(sd)
