@@ -332,11 +332,13 @@ class FusedAdamW(torch.optim.Optimizer):
             states = [state[p] or self._new_state(p, bits) for p in params]
             steps.append((params, grads, states, places, images, group))
         if not steps:
+            if self.param_groups[0]["max_grad_norm"] is not None:
+                self.grad_norm = torch.zeros((), device=self.param_groups[0]["params"][0].device)
             return loss
         if steps[0][0][0].is_cuda:
             norm = _ext().adamw_step(steps, -1.0 if clip is None else clip, seed)
-            if clip is not None:
-                self.grad_norm = norm
+            if clip is not None:          # (None: nothing but empty tensors)
+                self.grad_norm = norm if norm is not None else torch.zeros((), device=steps[0][0][0].device)
             for tower, li in owners:
                 tower.image_updated(li)
         else:

@@ -81,3 +81,14 @@ def test_an_incomplete_coded_state_is_refused():
         del sd["state"][0][name]
         with pytest.raises(ValueError, match="FusedAdamW"):
             FusedAdamW([torch.ones(300, requires_grad=True)]).load_state_dict(sd)
+
+
+def test_the_norm_of_a_step_without_gradients_is_not_the_last_ones():
+    p = torch.ones(3, requires_grad=True)
+    opt = FusedAdamW([p], max_grad_norm=1.0)
+    p.grad = torch.ones(3)
+    opt.step()
+    assert float(opt.grad_norm) == pytest.approx(math.sqrt(3.0), rel=2 ** -23)
+    p.grad = None
+    opt.step()
+    assert float(opt.grad_norm) == 0.0

@@ -155,5 +155,21 @@ def test_a_schedule_that_moves_the_betas(monkeypatch):
     assert "betas" in graphs.failed
 
 
+def test_the_norm_of_a_step_without_gradients():
+    p, e = torch.ones(3, device="cuda", requires_grad=True), torch.ones(0, device="cuda", requires_grad=True)
+    opt = FusedAdamW([p, e], max_grad_norm=1.0)
+    p.grad = torch.ones(3, device="cuda")
+    opt.step()
+    assert float(opt.grad_norm) > 1.0
+    p.grad, e.grad = None, torch.ones(0, device="cuda")
+    opt.step()
+    assert float(opt.grad_norm) == 0.0 and opt.grad_norm.is_cuda
+    p.grad = torch.ones(3, device="cuda")
+    opt.step()
+    p.grad = e.grad = None
+    opt.step()
+    assert float(opt.grad_norm) == 0.0
+
+
 # lengths around a wave's two scale blocks (512 elements), a step's workgroups (2048) and a norm's (8192)
 EDGES = [511, 512, 513, 767, 768, 769, 1024, 1535, 1536, 1537, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 8192, 8193, 16384, 16385]
