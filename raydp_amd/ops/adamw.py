@@ -333,7 +333,7 @@ class FusedAdamW(torch.optim.Optimizer):
             steps.append((params, grads, states, places, images, group))
         if not steps:
             if self.param_groups[0]["max_grad_norm"] is not None:
-                self.grad_norm = torch.zeros((), device=self.param_groups[0]["params"][0].device)
+                self.grad_norm = torch.zeros((), device=next(p for g in self.param_groups for p in g["params"]).device)
             return loss
         if steps[0][0][0].is_cuda:
             norm = _ext().adamw_step(steps, -1.0 if clip is None else clip, seed)

@@ -85,10 +85,14 @@ def test_an_incomplete_coded_state_is_refused():
 
 def test_the_norm_of_a_step_without_gradients_is_not_the_last_ones():
     p = torch.ones(3, requires_grad=True)
-    opt = FusedAdamW([p], max_grad_norm=1.0)
+    opt = FusedAdamW([dict(params=[]), dict(params=[p])], max_grad_norm=1.0)
     p.grad = torch.ones(3)
     opt.step()
     assert float(opt.grad_norm) == pytest.approx(math.sqrt(3.0), rel=2 ** -23)
     p.grad = None
     opt.step()
     assert float(opt.grad_norm) == 0.0
+
+
+BAD = [dict(lr=-1.0), dict(lr=torch.ones(2)), dict(eps=-1.0), dict(eps=1e-40), dict(betas=(1.0, 0.9)), dict(betas=(0.9,)),
+       dict(weight_decay=-1.0), dict(state_bits=16), dict(max_grad_norm=-1.0), dict(seed=-1)]
