@@ -186,33 +186,39 @@ class FusedAdamW(torch.optim.Optimizer):
     ``load_state_dict`` also takes the state of a ``torch.optim.AdamW`` and codes its moments; one with ``amsgrad``, or of a
     ``torch.optim.Adam`` whose ``weight_decay`` meant another thing, raises before anything is changed.
 
-    Parameters are contiguous fp32 or bf16; gradients are dense and of the parameter's type. Sparse gradients, parameters
-    that share memory, a first step inside a graph capture raise."""
+    ``eps`` is 0 or at least 2^-126. Parameters are contiguous fp32 or bf16; gradients are dense and of the parameter's
+    type. Sparse gradients, parameters that share memory, a first step inside a graph capture raise."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                  state_bits: int = 8, max_grad_norm: Optional[float] = None, maximize: bool = False, seed: int = 0):
-        if isinstance(lr, torch.Tensor):
-            if lr.numel() != 1:
-                raise ValueError("FusedAdamW: a tensor lr must have one element")
-        elif not 0.0 <= lr:
-            raise ValueError(f"FusedAdamW: invalid learning rate {lr}")
-        if not eps >= 0.0:
-            raise ValueError(f"FusedAdamW: invalid eps {eps}")
-        if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
-            raise ValueError(f"FusedAdamW: invalid betas {betas}")
-        if not weight_decay >= 0.0:
-            raise ValueError(f"FusedAdamW: invalid weight_decay {weight_decay}")
-        if state_bits not in (8, 32):
-            raise ValueError(f"FusedAdamW: state_bits is 8 or 32, got {state_bits}")
-        if max_grad_norm is not None and not max_grad_norm >= 0.0:
-            raise ValueError(f"FusedAdamW: invalid max_grad_norm {max_grad_norm}")
-        if not 0 <= int(seed) <= _MASK:
-            raise ValueError(f"FusedAdamW: seed must fit 32 bits, got {seed}")
+        self._check_options(dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                 max_grad_norm=max_grad_norm, seed=seed))
         super().__init__(params, dict(lr=lr, betas=tuple(float(b) for b in betas), eps=float(eps),
                                       weight_decay=float(weight_decay), state_bits=int(state_bits),
                                       max_grad_norm=None if max_grad_norm is None else float(max_grad_norm),
                                       maximize=bool(maximize), seed=int(seed)))
         self.grad_norm: Optional[torch.Tensor] = None
+
+    @staticmethod
+    def _check_options(o):
+        lr, eps, betas, clip = o["lr"], o["eps"], o["betas"], o["max_grad_norm"]
+        if isinstance(lr, torch.Tensor):
+            if lr.numel() != 1:
+                raise ValueError("FusedAdamW: a tensor lr must have one element")
+        elif not 0.0 <= lr:
+            raise ValueError(f"FusedAdamW: invalid learning rate {lr}")
+        if eps != 0.0 and not eps >= 2.0 ** -126:
+            raise ValueError(f"FusedAdamW: eps must be 0 or a normal fp32 number (at least 2^-126), got {eps}")
+        if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"FusedAdamW: invalid betas {betas}")
+        if not o["weight_decay"] >= 0.0:
+            raise ValueError(f"FusedAdamW: invalid weight_decay {o['weight_decay']}")
+        if o["state_bits"] not in (8, 32):
+            raise ValueError(f"FusedAdamW: state_bits is 8 or 32, got {o['state_bits']}")
+        if clip is not None and not clip >= 0.0:
+            raise ValueError(f"FusedAdamW: invalid max_grad_norm {clip}")
+        if not 0 <= int(o["seed"]) <= _MASK:
+            raise ValueError(f"FusedAdamW: seed must fit 32 bits, got {o['seed']}")
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -227,13 +233,16 @@ class FusedAdamW(torch.optim.Optimizer):
     def add_param_group(self, group):
         super().add_param_group(group)
         params = self.param_groups[-1]["params"]
-        for p in params:
-            if p.dtype not in (torch.float32, torch.bfloat16):
-                self.param_groups.pop()
-                raise TypeError(f"FusedAdamW: parameter dtype {p.dtype} (fp32 or bf16)")
-        if len({id(p) for p in params}) < len(params):
+        try:
+            self._check_options(self.param_groups[-1])
+            for p in params:
+                if p.dtype not in (torch.float32, torch.bfloat16):
+                    raise TypeError(f"FusedAdamW: parameter dtype {p.dtype} (fp32 or bf16)")
+            if len({id(p) for p in params}) < len(params):
+                raise ValueError("FusedAdamW: a parameter is listed twice")
+        except (TypeError, ValueError):
             self.param_groups.pop()
-            raise ValueError("FusedAdamW: a parameter is listed twice")
+            raise
 
     def load_state_dict(self, state_dict):
         saved = state_dict["state"]
@@ -244,6 +253,7 @@ class FusedAdamW(torch.optim.Optimizer):
             if saved.get(i):
                 self._check_saved(saved[i], k, p)
         for g in state_dict["param_groups"]:
+            self._check_options({**self.defaults, **g})
             if g.get("amsgrad"):
                 raise ValueError("FusedAdamW: the state is of an amsgrad optimizer, whose largest second moments it does not keep")
             if g.get("weight_decay") and g.get("decoupled_weight_decay") is False:
@@ -329,6 +339,8 @@ class FusedAdamW(torch.optim.Optimizer):
             elif group["max_grad_norm"] != clip or group["seed"] != seed:
                 raise ValueError("FusedAdamW: max_grad_norm and seed are the optimizer's, not a group's")
             bits = group["state_bits"]
+            if bits not in (8, 32):
+                raise ValueError(f"FusedAdamW: state_bits is 8 or 32, got {bits}")
             states = [state[p] or self._new_state(p, bits) for p in params]
             steps.append((params, grads, states, places, images, group))
         if not steps:

@@ -55,7 +55,7 @@ def _state(cls, **kw):
 @pytest.mark.parametrize("make,match", [
     (lambda: _state(torch.optim.AdamW, amsgrad=True), "amsgrad"),
     (lambda: _state(torch.optim.Adam, amsgrad=True), "amsgrad"),
-    (lambda: _state(torch.optim.Adam, weight_decay=0.1), "weight_decay")])
+    (lambda: _state(torch.optim.Adam, weight_decay=0.1), "weight_decay"), (lambda: _state(torch.optim.AdamW, eps=1e-40), "eps")])
 def test_a_state_that_means_something_else_is_refused_and_changes_nothing(make, match):
     q = torch.ones(300, requires_grad=True)
     q.grad = torch.full((300,), 0.1)
@@ -96,3 +96,27 @@ def test_the_norm_of_a_step_without_gradients_is_not_the_last_ones():
 
 BAD = [dict(lr=-1.0), dict(lr=torch.ones(2)), dict(eps=-1.0), dict(eps=1e-40), dict(betas=(1.0, 0.9)), dict(betas=(0.9,)),
        dict(weight_decay=-1.0), dict(state_bits=16), dict(max_grad_norm=-1.0), dict(seed=-1)]
+
+
+@pytest.mark.parametrize("bad", BAD, ids=lambda d: next(iter(d)))
+def test_a_groups_own_options_are_checked_like_the_optimizers(bad):
+    """(A denominator under 2^-126 has no quotient on the GPU: with eps = 1e-40 a gradient of 0 would give 0 * inf.)"""
+    a, b = (torch.ones(4, requires_grad=True) for _ in range(2))
+    with pytest.raises(ValueError, match="FusedAdamW"):
+        FusedAdamW([a], **bad)
+    with pytest.raises(ValueError, match="FusedAdamW"):
+        FusedAdamW([dict(params=[a], **bad)])
+    opt = FusedAdamW([a])
+    with pytest.raises(ValueError, match="FusedAdamW"):
+        opt.add_param_group(dict(params=[b], **bad))
+    assert len(opt.param_groups) == 1
+
+
+def test_state_bits_set_to_nothing_there_is():
+    p = torch.ones(4, requires_grad=True)
+    p.grad = torch.ones(4)
+    opt = FusedAdamW([p])
+    opt.param_groups[0]["state_bits"] = 16
+    with pytest.raises(ValueError, match="state_bits"):
+        opt.step()
+    assert not opt.state[p] and (p == 1).all()
