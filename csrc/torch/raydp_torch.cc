@@ -47,6 +47,12 @@ void written(const Tensor& t) {
 
 bool bf16(const Tensor& t) { return t.scalar_type() == at::kBFloat16; }
 
+// A launch computes no tangent: the result would have none, without a word.
+void check_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what,
+                              ": forward-mode derivatives are not implemented on the GPU");
+}
+
 // A backward of ours is not differentiable itself: under create_graph its results carry a node that says so.
 variable_list once(variable_list out) {
   if (!at::GradMode::is_enabled()) return out;
@@ -150,6 +156,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& all, double max_norm) {
   const auto dev = all.at(0).device();
   std::vector<std::pair<uintptr_t, uintptr_t>> spans;
   for (const Tensor& g : all) {
+    check_tangent(g, "clip_grad_norm_");
     if (g.layout() != at::kStrided) throw py::value_error("clip_grad_norm_: sparse gradients are not supported");
     if (g.device() != dev)
       throw py::value_error("clip_grad_norm_: gradients on " + dev.str() + " and " + g.device().str());
@@ -261,6 +268,7 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
       s.img = nullptr;
       if (s.g.layout() != at::kStrided) throw std::runtime_error("FusedAdamW does not support sparse gradients");
       if (s.p.numel() == 0) continue;
+      check_tangent(s.g, "FusedAdamW");
       if (!dev) dev = s.p.device();
       if (s.p.device() != *dev || s.g.device() != *dev)
         throw py::value_error("FusedAdamW: parameters with gradients on " + dev->str() + " and " +
@@ -444,6 +452,7 @@ struct Route : torch::autograd::Function<Route> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Variable(), Variable(), Variable()};
+    check_tangent(grads[0], "route");
     check_capturable(grads[0]);
     const auto saved = ctx->get_saved_variables();
     const Tensor &w = saved[0], &ids = saved[1], dw = grads[0].contiguous();
@@ -460,6 +469,7 @@ struct Route : torch::autograd::Function<Route> {
 };
 
 std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, bool renorm) {
+  check_tangent(logits, "route");
   variable_list out = logits.requires_grad() && at::GradMode::is_enabled() ? Route::apply(logits, k, renorm)
                                                                            : route_forward(rows_of(logits), k, renorm, false);
   return {out[0], out[1]};
@@ -564,6 +574,7 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
     return scatter(position, source, x, Tensor(), Tensor()).first;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_tangent(grads[0], "dispatch");
     check_capturable(grads[0]);
     const auto saved = ctx->get_saved_variables();
     return once({gather(saved[0], saved[1], grads[0].contiguous(), Tensor()), Variable(), Variable()});
@@ -579,6 +590,7 @@ struct Combine : torch::autograd::Function<Combine> {
     return gather(position, source, rows, w);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_tangent(grads[0], "combine");
     check_capturable(grads[0]);
     const auto saved = ctx->get_saved_variables();
     auto [drows, dw] = scatter(saved[0], saved[1], grads[0], saved[2], saved[3]);
@@ -587,11 +599,14 @@ struct Combine : torch::autograd::Function<Combine> {
 };
 
 Tensor dispatch(const Tensor& x, const Tensor& position, const Tensor& source) {
+  check_tangent(x, "dispatch");
   if (x.requires_grad() && at::GradMode::is_enabled()) return Dispatch::apply(x, position, source);
   return scatter(position, source, x, Tensor(), Tensor()).first;
 }
 
 Tensor combine(const Tensor& rows_, const c10::optional<Tensor>& weights, const Tensor& position, const Tensor& source) {
+  check_tangent(rows_, "combine");
+  if (weights) check_tangent(*weights, "combine");
   const Tensor rows = rows_.contiguous();
   c10::optional<Tensor> w;
   if (weights) w = weights->to(at::kFloat).contiguous();
@@ -603,6 +618,13 @@ Tensor combine(const Tensor& rows_, const c10::optional<Tensor>& weights, const 
 }  // namespace
 
 PYBIND11_MODULE(raydp_torch, m) {
+  py::register_local_exception_translator([](std::exception_ptr error) {
+    try {
+      if (error) std::rethrow_exception(error);
+    } catch (const c10::NotImplementedError& e) {
+      PyErr_SetString(PyExc_NotImplementedError, e.what_without_backtrace());
+    }
+  });
   m.def("clip_grad_norm", &clip_grad_norm);
   m.def("adamw_step", &adamw_step);
   m.def("decode_moments", &decode_moments);

@@ -8,9 +8,9 @@
 Nothing is read back to the host, so a step with them can be captured into a HIP graph; with a ``capacity`` every expert's
 rows are a slice of fixed size (``rows.view(num_experts, capacity, D)``) that a ``FusedLinearTower`` takes as it is.
 
-``route``, ``dispatch`` and ``combine`` are differentiable (once). Capturing a backward pass through them is refused when it
-would reach what an eager call on the default stream made: intermediate results, or leaves that something the call returned
-still holds.
+``route``, ``dispatch`` and ``combine`` are differentiable (once, in reverse; a forward-mode tangent raises on the GPU).
+Capturing a backward pass through them is refused when it would reach what an eager call on the default stream made:
+intermediate results, or leaves that something the call returned still holds.
 
 On the GPU all run on the HIP kernels (through ``csrc/torch/raydp_torch.cc``) and fail loudly if these are missing; on the
 CPU they are the equivalent PyTorch expressions (any floating type, for tests and CPU-only hosts).
