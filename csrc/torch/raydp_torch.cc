@@ -5,10 +5,12 @@
 // and a node's backward runs without the interpreter. What the callers documented and checked holds here: tensors are on one
 // GPU, launches go to its current stream, and every failure is a C++ exception that becomes the Python error it names.
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/engine.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -46,6 +48,12 @@ void written(const Tensor& t) {
 }
 
 bool bf16(const Tensor& t) { return t.scalar_type() == at::kBFloat16; }
+
+// A trace keeps torch's operators: of a call here it would keep the allocation of the results and not what fills them.
+void check_trace(const char* what) {
+  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
+    throw std::runtime_error(std::string(what) + " cannot be traced on the GPU: the trace would miss the kernel's launch");
+}
 
 // A launch computes no tangent: the result would have none, without a word.
 void check_tangent(const Tensor& t, const char* what) {
@@ -152,6 +160,7 @@ void check_overlap(std::vector<std::pair<uintptr_t, uintptr_t>>& spans, const ch
 
 // grads: checked here, dense in any order of dimensions; returns the norm
 Tensor clip_grad_norm(const std::vector<Tensor>& all, double max_norm) {
+  check_trace("clip_grad_norm_");
   std::vector<Tensor> grads;
   const auto dev = all.at(0).device();
   std::vector<std::pair<uintptr_t, uintptr_t>> spans;
@@ -222,6 +231,7 @@ Tensor state_tensor(py::dict& st, const char* name, const Tensor& p) {
 // groups: [(parameters, gradients, states, places, images, options)]; images: {index: bf16 tensor}. max_norm < 0: no
 // clipping. Returns the norm, or None without clipping.
 c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_t seed) {
+  check_trace("FusedAdamW.step");
   std::vector<Group> all;
   std::vector<Tensor> grads;
   c10::optional<c10::Device> dev;
@@ -399,6 +409,7 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
 }
 
 std::vector<Tensor> decode_moments(const Tensor& m, const Tensor& v, const Tensor& sc, bool to_bf16) {
+  check_trace("decode_moments");
   const auto kind = to_bf16 ? at::kBFloat16 : at::kFloat;
   Tensor mo = at::empty(m.sizes(), m.options().dtype(kind)), vo = at::empty(m.sizes(), m.options().dtype(kind));
   if (m.numel()) {
@@ -469,6 +480,7 @@ struct Route : torch::autograd::Function<Route> {
 };
 
 std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, bool renorm) {
+  check_trace("route");
   check_tangent(logits, "route");
   variable_list out = logits.requires_grad() && at::GradMode::is_enabled() ? Route::apply(logits, k, renorm)
                                                                            : route_forward(rows_of(logits), k, renorm, false);
@@ -486,6 +498,7 @@ std::pair<int64_t, int64_t> plan_grid(int64_t n) {
 
 // (position, source, load, offsets); capacity 0: unlimited
 std::vector<Tensor> expert_plan(const Tensor& experts, int64_t E, int64_t capacity) {
+  check_trace("expert_plan");
   const Tensor ids = experts.contiguous();
   const int64_t T = ids.size(0), k = ids.size(1), n = T * k, rows = capacity ? E * capacity : n;
   const auto [chunk, blocks] = plan_grid(n);
@@ -599,12 +612,14 @@ struct Combine : torch::autograd::Function<Combine> {
 };
 
 Tensor dispatch(const Tensor& x, const Tensor& position, const Tensor& source) {
+  check_trace("dispatch");
   check_tangent(x, "dispatch");
   if (x.requires_grad() && at::GradMode::is_enabled()) return Dispatch::apply(x, position, source);
   return scatter(position, source, x, Tensor(), Tensor()).first;
 }
 
 Tensor combine(const Tensor& rows_, const c10::optional<Tensor>& weights, const Tensor& position, const Tensor& source) {
+  check_trace("combine");
   check_tangent(rows_, "combine");
   if (weights) check_tangent(*weights, "combine");
   const Tensor rows = rows_.contiguous();

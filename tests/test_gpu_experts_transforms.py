@@ -75,3 +75,16 @@ def _traced():
         "clip": (lambda t: clip_grad_norm_([p], 1.0) + t, x),
         "step": (lambda t: (opt.step(), t + 1)[1], x),
     }
+
+
+@pytest.mark.parametrize("name", ["route", "plan", "dispatch", "combine", "decode", "clip", "step"])
+@pytest.mark.parametrize("how", ["jit", "fx"])
+def test_a_trace_that_would_miss_the_launch_is_refused(how, name):
+    f, t = _traced()[name]
+    with pytest.raises(RuntimeError, match="trace"):
+        if how == "jit":
+            torch.jit.trace(f, (t,), check_trace=False)
+        else:
+            from torch.fx.experimental.proxy_tensor import make_fx
+            make_fx(f)(t)
+    f(t)
