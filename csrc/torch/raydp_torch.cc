@@ -55,6 +55,17 @@ void check_trace(const char* what) {
     throw std::runtime_error(std::string(what) + " cannot be traced on the GPU: the trace would miss the kernel's launch");
 }
 
+// Wrappers say that they are on the GPU and have no memory there, or not the values that stand in it.
+void check_memory(const Tensor& t, const char* what) {
+  using c10::DispatchKey;
+  static const c10::DispatchKeySet odd({DispatchKey::Python, DispatchKey::Functionalize, DispatchKey::FuncTorchBatched,
+                                        DispatchKey::FuncTorchGradWrapper, DispatchKey::Batched, DispatchKey::ZeroTensor,
+                                        DispatchKey::Negative, DispatchKey::Conjugate});
+  if (t.defined() && t.key_set().has_any(odd))
+    throw py::type_error(std::string(what) + ": a kernel cannot read a wrapped tensor (a fake or functional one, a transform's, "
+                         "a subclass that dispatches, a lazy negation)");
+}
+
 // A launch computes no tangent: the result would have none, without a word.
 void check_tangent(const Tensor& t, const char* what) {
   TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what,
@@ -165,6 +176,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& all, double max_norm) {
   const auto dev = all.at(0).device();
   std::vector<std::pair<uintptr_t, uintptr_t>> spans;
   for (const Tensor& g : all) {
+    check_memory(g, "clip_grad_norm_");
     check_tangent(g, "clip_grad_norm_");
     if (g.layout() != at::kStrided) throw py::value_error("clip_grad_norm_: sparse gradients are not supported");
     if (g.device() != dev)
@@ -220,6 +232,7 @@ Tensor state_tensor(py::dict& st, const char* name, const Tensor& p) {
   if (o == nullptr || !THPVariable_Check(o))
     throw py::value_error(std::string("FusedAdamW: a parameter's state lacks ") + name);
   Tensor t = THPVariable_Unpack(o);
+  check_memory(t, "FusedAdamW");
   if (t.device() != p.device()) {      // state that was loaded before the model was moved
     t = t.to(p.device());
     st[name] = t;
@@ -258,6 +271,7 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
     const py::object lr = o["lr"];
     if (THPVariable_Check(lr.ptr())) {
       const Tensor l = THPVariable_Unpack(lr.ptr());
+      check_memory(l, "FusedAdamW");
       if (!l.is_cuda()) {
         if (capturing(params[0].get_device()))
           throw std::runtime_error("FusedAdamW: a tensor lr on the host cannot be captured into a graph, whose replays would "
@@ -278,6 +292,8 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
       s.img = nullptr;
       if (s.g.layout() != at::kStrided) throw std::runtime_error("FusedAdamW does not support sparse gradients");
       if (s.p.numel() == 0) continue;
+      check_memory(s.p, "FusedAdamW");
+      check_memory(s.g, "FusedAdamW");
       check_tangent(s.g, "FusedAdamW");
       if (!dev) dev = s.p.device();
       if (s.p.device() != *dev || s.g.device() != *dev)
@@ -312,6 +328,7 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
       }
       if (with_images && !bf16(s.p) && images.contains(py::int_(i))) {   // (a bf16 parameter is its own image)
         const Tensor img = images[py::int_(i)].cast<Tensor>();
+        check_memory(img, "FusedAdamW");
         if (!bf16(img) || !img.is_contiguous() || img.numel() != s.p.numel() || img.device() != *dev)
           throw py::value_error("FusedAdamW: a weight's image must be contiguous bf16 of its size");
         s.img = ptr<uint16_t>(img);
@@ -410,6 +427,7 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
 
 std::vector<Tensor> decode_moments(const Tensor& m, const Tensor& v, const Tensor& sc, bool to_bf16) {
   check_trace("decode_moments");
+  for (const Tensor& t : {m, v, sc}) check_memory(t, "decode_moments");
   const auto kind = to_bf16 ? at::kBFloat16 : at::kFloat;
   Tensor mo = at::empty(m.sizes(), m.options().dtype(kind)), vo = at::empty(m.sizes(), m.options().dtype(kind));
   if (m.numel()) {
@@ -463,6 +481,7 @@ struct Route : torch::autograd::Function<Route> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Variable(), Variable(), Variable()};
+    check_memory(grads[0], "route");
     check_tangent(grads[0], "route");
     check_capturable(grads[0]);
     const auto saved = ctx->get_saved_variables();
@@ -481,6 +500,7 @@ struct Route : torch::autograd::Function<Route> {
 
 std::tuple<Tensor, Tensor> route(const Tensor& logits, int64_t k, bool renorm) {
   check_trace("route");
+  check_memory(logits, "route");
   check_tangent(logits, "route");
   variable_list out = logits.requires_grad() && at::GradMode::is_enabled() ? Route::apply(logits, k, renorm)
                                                                            : route_forward(rows_of(logits), k, renorm, false);
@@ -499,6 +519,7 @@ std::pair<int64_t, int64_t> plan_grid(int64_t n) {
 // (position, source, load, offsets); capacity 0: unlimited
 std::vector<Tensor> expert_plan(const Tensor& experts, int64_t E, int64_t capacity) {
   check_trace("expert_plan");
+  check_memory(experts, "expert_plan");
   const Tensor ids = experts.contiguous();
   const int64_t T = ids.size(0), k = ids.size(1), n = T * k, rows = capacity ? E * capacity : n;
   const auto [chunk, blocks] = plan_grid(n);
@@ -587,6 +608,7 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
     return scatter(position, source, x, Tensor(), Tensor()).first;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_memory(grads[0], "dispatch");
     check_tangent(grads[0], "dispatch");
     check_capturable(grads[0]);
     const auto saved = ctx->get_saved_variables();
@@ -603,6 +625,7 @@ struct Combine : torch::autograd::Function<Combine> {
     return gather(position, source, rows, w);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_memory(grads[0], "combine");
     check_tangent(grads[0], "combine");
     check_capturable(grads[0]);
     const auto saved = ctx->get_saved_variables();
@@ -613,6 +636,7 @@ struct Combine : torch::autograd::Function<Combine> {
 
 Tensor dispatch(const Tensor& x, const Tensor& position, const Tensor& source) {
   check_trace("dispatch");
+  for (const Tensor& t : {x, position, source}) check_memory(t, "dispatch");
   check_tangent(x, "dispatch");
   if (x.requires_grad() && at::GradMode::is_enabled()) return Dispatch::apply(x, position, source);
   return scatter(position, source, x, Tensor(), Tensor()).first;
@@ -620,6 +644,7 @@ Tensor dispatch(const Tensor& x, const Tensor& position, const Tensor& source) {
 
 Tensor combine(const Tensor& rows_, const c10::optional<Tensor>& weights, const Tensor& position, const Tensor& source) {
   check_trace("combine");
+  for (const Tensor& t : {rows_, weights ? *weights : Tensor(), position, source}) check_memory(t, "combine");
   check_tangent(rows_, "combine");
   if (weights) check_tangent(*weights, "combine");
   const Tensor rows = rows_.contiguous();

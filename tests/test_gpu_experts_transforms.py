@@ -88,3 +88,28 @@ def test_a_trace_that_would_miss_the_launch_is_refused(how, name):
             from torch.fx.experimental.proxy_tensor import make_fx
             make_fx(f)(t)
     f(t)
+
+
+def test_transforms_and_wrapped_tensors_are_refused():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    z, x, w, ids, plan, rows = _inputs()
+    with pytest.raises(TypeError, match="wrapped"):
+        torch.func.vmap(lambda t: route(t, 2)[0])(torch.stack([z, z]))
+    with pytest.raises(TypeError, match="wrapped"):
+        torch.func.grad(lambda t: dispatch(t, plan).sum())(x)
+    with pytest.raises(TypeError, match="wrapped"):
+        combine(torch._neg_view(rows), plan, w)
+    leaf = rows.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="wrapped"):          # (what a backward throws arrives as this)
+        torch.autograd.grad(combine(leaf, plan, w), leaf, torch.ones(3, 6, 5, device="cuda"), is_grads_batched=True)
+    with FakeTensorMode():
+        p = nn.Parameter(torch.ones(300, device="cuda"))
+        p.grad = torch.ones(300, device="cuda")
+        with pytest.raises(TypeError, match="wrapped"):
+            FusedAdamW([p]).step()
+    p = nn.Parameter(torch.ones(300, device="cuda"))
+    p.grad = torch._neg_view(torch.ones(300, device="cuda"))
+    for call in (lambda: FusedAdamW([p]).step(), lambda: clip_grad_norm_([p], 1.0)):
+        with pytest.raises(TypeError, match="wrapped"):
+            call()
+    route(z, 2)
