@@ -46,7 +46,7 @@ def route(logits: torch.Tensor, k: int, renormalize: bool = True) -> Tuple[torch
 
     An expert whose logit is ``-inf`` is never chosen; a sample with fewer than ``k`` others gets expert -1 with weight 0
     in the places that are left (all of them, for a padding row of ``-inf``). A NaN is not chosen and makes the weights of
-    its row NaN."""
+    its row, and what reaches its logits from them, NaN."""
     if logits.dim() != 2 or not logits.is_floating_point():
         raise ValueError(f"route: logits must be floating [T, E], got {logits.dtype} {tuple(logits.shape)}")
     T, E = logits.shape
@@ -72,7 +72,7 @@ def _route_cpu(logits, k, renormalize):
     part = torch.where(there, torch.exp(z.gather(1, ids).masked_fill(~there, 0.0) - peak), 0.0)
     total = part.sum(1, keepdim=True) if renormalize else torch.exp(z - peak).sum(1, keepdim=True)
     w = part / torch.where(total == 0, 1.0, total)
-    w = torch.where(bad.any(1, keepdim=True), torch.nan, w)
+    w = w * torch.where(bad.any(1, keepdim=True), torch.nan, 1.0)      # (a product: the gradient shows the NaN too)
     return (w.float() if z.dtype == torch.float32 else w), torch.where(there, ids, -1).int()
 
 
