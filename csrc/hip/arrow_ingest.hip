@@ -19,6 +19,7 @@
 //     the fused trainer expects.
 // The epoch shuffle is not materialised here: rx_feistel_perm draws a permutation on the device
 // and the training kernels gather rows through it (fused into their row loads).
+#include "common/logging.h"
 #include "rx_common.h"
 
 #include <algorithm>
@@ -418,7 +419,8 @@ int rx_arrow_ingest(const IngestArgs* a, void* out, hipStream_t stream) {
 
 // Pin [addr, addr + len) of the arena [base, base + cap) (chunk-granular, idempotent). A system
 // that refuses to register existing memory is asked once: rx_ingest_dma then bounces the range
-// through pinned memory of its own. Returns 0, or -1 for a range outside the arena.
+// through pinned memory of its own. Returns 0, -1 for a range outside the arena, or the HIP error
+// of a registration that failed for another reason (the next call asks again).
 int rx_pin_range(unsigned long long base, unsigned long long cap, unsigned long long addr,
                  unsigned long long len, unsigned long long chunk) {
   if (len == 0) return 0;
@@ -447,7 +449,11 @@ int rx_pin_range(unsigned long long base, unsigned long long cap, unsigned long 
     const hipError_t rc = hipHostRegister(reinterpret_cast<void*>(s), n, hipHostRegisterDefault);
     if (rc != hipSuccess && rc != hipErrorHostMemoryAlreadyRegistered) {
       (void)hipGetLastError();
+      // the range is part of a mapped arena and nothing was ever registered: it is the system that does not take it
+      if ((rc != hipErrorInvalidValue && rc != hipErrorNotSupported) || g_pin_calls != 0) return (int)rc;
       g_pin_refused = true;
+      rx_log::msg("ingest", "the system does not register existing memory (HIP error %d): store blocks go through a pinned "
+                  "buffer", (int)rc);
       return 0;
     }
     for (size_t k = c; k <= e; ++k) pa->run[k] = (int64_t)c;

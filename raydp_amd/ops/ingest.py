@@ -218,7 +218,7 @@ def _pin(regions) -> None:
             continue
         rc = lib.rx_pin_range(u64(ar[0]), u64(ar[1]), u64(s), u64(n), u64(PIN_CHUNK))
         if rc != 0:
-            raise RuntimeError(f"pinning outside the object-store arena (error {rc})")
+            raise RuntimeError(f"hipHostRegister of the object-store arena failed (HIP error {rc}; -1: a range outside it)")
 
 
 def _reap_inflight():
