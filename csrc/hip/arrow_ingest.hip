@@ -365,6 +365,13 @@ int rx_bounce_copy(uint8_t* dst, uintptr_t host, size_t bytes, hipStream_t copy,
   return 0;
 }
 
+// Memory that was to be pinned: other memory stays pageable. Caller holds g_mu.
+bool rx_in_arena(uintptr_t host) {
+  for (const auto& a : g_arenas)
+    if (host >= a.base && host < a.base + a.cap) return true;
+  return false;
+}
+
 // Largest n <= want such that [host, host + n) lies inside one registration run (or `want`
 // when the address is in no registered arena). Caller holds g_mu.
 size_t rx_contig_pinned(uintptr_t host, size_t want) {
@@ -426,7 +433,6 @@ int rx_pin_range(unsigned long long base, unsigned long long cap, unsigned long 
   if (len == 0) return 0;
   if (addr < base || addr + len > base + cap || chunk == 0) return -1;
   std::lock_guard<std::mutex> g(g_mu);
-  if (g_pin_refused) return 0;
   PinnedArena* pa = nullptr;
   for (auto& a : g_arenas)
     if (a.base == base && a.cap == cap) pa = &a;
@@ -435,6 +441,7 @@ int rx_pin_range(unsigned long long base, unsigned long long cap, unsigned long 
                                    std::vector<int64_t>((cap + chunk - 1) / chunk, -1)});
     pa = &g_arenas.back();
   }
+  if (g_pin_refused) return 0;
   const size_t c0 = (addr - base) / pa->chunk, c1 = (addr + len - 1 - base) / pa->chunk;
   size_t c = c0;
   while (c <= c1) {
@@ -535,7 +542,7 @@ int rx_ingest_dma(const RxDmaChunk* chunks, int nchunks, const RxDmaRegion* regi
       const bool pin = hipPointerGetAttributes(&at, reinterpret_cast<void*>(rg.host)) == hipSuccess &&
                        at.type == hipMemoryTypeHost;
       (void)hipGetLastError();
-      if (!pin && g_pin_refused) {
+      if (!pin && g_pin_refused && rx_in_arena((uintptr_t)rg.host)) {
         const int rc = rx_bounce_copy(ring + s + rg.off, (uintptr_t)rg.host, (size_t)rg.bytes, copy, &ncopies);
         if (rc) return rc;
         pinned += rg.bytes;

@@ -2,24 +2,25 @@
 
 GPU path (``csrc/hip/arrow_ingest.hip``, ``rx_ingest_dma``):
 
-* the host never copies column bytes. For every block it computes which byte ranges of the
+* the host does not convert column bytes. For every block it computes which byte ranges of the
   block's buffers the requested columns need (values + validity, sliced to the array window)
   and hands the list to native code: ranges that are dense in the Arrow IPC body are merged
   into one DMA per block, sparse ones go buffer by buffer;
 * ranges inside a store arena are pinned with ``hipHostRegister`` in 2 MiB chunks, lazily, once
   per process (``rx_pin_range``), so the copies are true DMAs out of the shared mapping; on a
-  system that refuses to register existing memory they go through a pinned buffer of our own
+  system that refuses to register existing memory the host copies them through a pinned buffer
   (two 4 MiB halves, one filling while the other is copied out);
 * ``hipMemcpyAsync`` runs on a dedicated copy stream into a ring of device staging memory;
   each chunk's decode kernel waits on an event on the compute stream, so chunk k+1's DMA
   overlaps chunk k's decode (column decode, validity -> fill value, dtype cast, transpose to the
   row-major [N, stride] matrix the trainers read, 16-B loads and stores).
 
-Counters (``ingest_stats()``): ``host_copy_bytes`` (bytes the host itself copied or converted:
-casts of dictionary / timestamp / string columns, the CPU path), ``dma_pinned_bytes``,
-``dma_pageable_bytes`` (sources outside any pinned arena: HIP stages those itself), ``dma_copies``,
-``chunks``, ``dma_bounced_bytes`` (those of the pinned ones that the pinned buffer carried), plus
-the native pinning counters.
+Counters (``ingest_stats()``): ``host_copy_bytes`` (columns that the host converted before the
+transfer: casts of dictionary / timestamp / string columns, the CPU path), ``dma_pinned_bytes`` (DMAs
+out of pinned memory: the store's, or the pinned buffer), ``dma_bounced_bytes`` (those of them that
+the host first copied into the pinned buffer: all where the system refuses to register memory, else
+none), ``dma_pageable_bytes`` (sources outside any store arena: HIP stages those itself),
+``dma_copies``, ``chunks``, plus the native pinning counters.
 
 Reference hot site: ``python/raydp/torch/estimator.py:226-241`` (Ray Data ``to_torch`` per
 batch on the CPU).
