@@ -323,23 +323,32 @@ struct Bounce {
 };
 Bounce g_bounce;
 
-// Close the half that is being filled: its copies are all enqueued on `copy`.
+// Close the half that is being filled: its copies are all enqueued on `copy`. (Where the event
+// fails, they are waited for: nothing fills a half again that is still read.)
 int rx_bounce_close(hipStream_t copy) {
   Bounce& b = g_bounce;
   if (b.fill == 0) return 0;
-  RX_CHECK(hipEventRecord(b.drained[b.half], copy));
-  b.busy[b.half] = true;
+  const hipError_t rc = hipEventRecord(b.drained[b.half], copy);
+  if (rc != hipSuccess) (void)hipStreamSynchronize(copy);
+  b.busy[b.half] = rc == hipSuccess;
   b.half ^= 1;
   b.fill = 0;
-  return 0;
+  return (int)rc;
 }
+
+// On every way out of a call, so that no half stays open for the next one's stream.
+struct BounceCall {
+  hipStream_t copy;
+  ~BounceCall() { (void)rx_bounce_close(copy); }
+};
 
 // dst <- [host, host + bytes) through the bounce buffer, in order on `copy`. Caller holds g_mu.
 int rx_bounce_copy(uint8_t* dst, uintptr_t host, size_t bytes, hipStream_t copy, long long* ncopies) {
   Bounce& b = g_bounce;
   if (b.mem == nullptr) {
+    for (auto& e : b.drained)
+      if (e == nullptr) RX_CHECK(hipEventCreateWithFlags(&e, hipEventDisableTiming));
     RX_CHECK(hipHostMalloc(reinterpret_cast<void**>(&b.mem), 2 * Bounce::kHalf, hipHostMallocPortable));
-    for (auto& e : b.drained) RX_CHECK(hipEventCreateWithFlags(&e, hipEventDisableTiming));
     ++g_pin_calls;
     g_pin_bytes += (long long)(2 * Bounce::kHalf);
   }
@@ -516,6 +525,7 @@ int rx_ingest_dma(const RxDmaChunk* chunks, int nchunks, const RxDmaRegion* regi
     size_t ev;
   };
   std::deque<Busy> busy;
+  const BounceCall call{copy};
   long long pos = 0;
   long long pinned = 0, pageable = 0, ncopies = 0, bounced = 0;
   for (int k = 0; k < nchunks; ++k) {

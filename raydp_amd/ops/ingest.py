@@ -314,8 +314,10 @@ def ingest_columns(tables: Sequence[pa.Table], cols: List[str], device, out_bf16
         rc = lib.rx_ingest_dma(chunks, len(chunk_l), regs, dcols, len(cols), stride, 2 if out_i64 else int(out_bf16),
                                ctypes.c_void_p(out.data_ptr()), ctypes.c_void_p(stage.data_ptr()), ring,
                                ctypes.c_void_p(compute.cuda_stream), ctypes.c_void_p(cs.cuda_stream), st)
+        stage.record_stream(cs)            # (also where the call failed: earlier chunks may be on their way)
+        if rc != 0:
+            cs.synchronize()
         _hip.check(rc, "rx_ingest_dma")
-        stage.record_stream(cs)
         for key, v in zip(("dma_pinned_bytes", "dma_pageable_bytes", "dma_copies", "chunks", "dma_bounced_bytes"), st):
             _stats[key] += int(v)
         ev = torch.cuda.Event()

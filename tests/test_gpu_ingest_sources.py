@@ -49,3 +49,29 @@ def test_ordinary_memory_is_pageable_also_after_a_store_was_read(store):
     inside, outside = _stored(store, _table(n, 3)), _table(3 * n, 4)
     st = _ingest([inside, outside, inside])
     assert st["dma_pinned_bytes"] >= 16 * n and st["dma_pageable_bytes"] >= 24 * n
+
+
+def test_a_call_that_fails_midway_leaves_the_next_one_right(store, monkeypatch):
+    """The second chunk claims more staging memory than there is, which the native code finds after the first is on its way."""
+    from raydp_amd.ops import _hip
+    n = 60_000
+    blocks = [_stored(store, _table(n, s)) for s in (5, 6)]
+    lib = _hip.lib()
+
+    class Claims:
+        def __getattr__(self, name):
+            return getattr(lib, name)
+
+        def rx_ingest_dma(self, chunks, count, *rest):
+            real, chunks[1].bytes = chunks[1].bytes, 1 << 40
+            try:
+                return lib.rx_ingest_dma(chunks, count, *rest)
+            finally:
+                chunks[1].bytes = real
+    with monkeypatch.context() as m:
+        m.setattr(_hip, "lib", Claims)
+        with pytest.raises(RuntimeError, match="rx_ingest_dma"):
+            _ingest(blocks)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        _ingest(blocks[::-1])
+    _ingest([_stored(store, _table(2_000_000, 7))])            # 16 MB: both halves, several times
