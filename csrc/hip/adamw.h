@@ -2,6 +2,14 @@
 #pragma once
 #include <stdint.h>
 
+// One number for a list of sizes: both sides of the C interface compare what they were built with.
+template <class... N>
+constexpr unsigned long long rx_layout(N... sizes) {
+  unsigned long long h = 1469598103934665603ull;      // FNV-1a
+  for (const unsigned long long v : {(unsigned long long)sizes...}) h = (h ^ v) * 1099511628211ull;
+  return h;
+}
+
 enum {
   kAwMax = 64,         // tensors in one step launch (kernel arguments under 4 KiB)
   kAwPrepMax = 256,    // tensors in one preparation launch (one thread each)
@@ -71,7 +79,12 @@ struct ScaleArgs {
   float* norm;
 };
 
+constexpr unsigned long long kAwLayout =
+    rx_layout(sizeof(AwHead), sizeof(AwTensor), sizeof(AwPrep), sizeof(AwStep), sizeof(NormArgs), sizeof(ScaleArgs), kAwMax,
+              kAwPrepMax, kNormMax, kAwBlock, kAwChunk, kNormChunk, kNormGrid, kNormBf16);
+
 extern "C" {
+unsigned long long rx_aw_layout();
 int rx_aw_prep(const AwPrep* a, void* stream);
 // stream_past: the step's working set is larger than the last-level cache
 int rx_aw_step(const AwStep* a, int bits, int bf16, int stream_past, void* stream);

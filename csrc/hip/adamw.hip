@@ -562,6 +562,8 @@ __global__ __launch_bounds__(256) void aw_decode_kernel(const uint8_t* __restric
 
 extern "C" {
 
+unsigned long long rx_aw_layout() { return kAwLayout; }
+
 int rx_aw_prep(const AwPrep* a, void* on) {
   hipStream_t stream = static_cast<hipStream_t>(on);
   if (a->n < 0 || a->n > kAwPrepMax) return -1;

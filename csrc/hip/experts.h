@@ -1,5 +1,6 @@
 // Arguments of csrc/hip/experts.hip's entry points (shared with their callers in csrc/torch).
 #pragma once
+#include "hip/adamw.h"   // rx_layout
 
 enum {
   kMaxExperts = 1024,
@@ -29,8 +30,12 @@ struct RowArgs {
   float* dw;                  // scatter with h: [T][k]
 };
 
+constexpr unsigned long long kExpertLayout =
+    rx_layout(sizeof(PlanArgs), sizeof(RowArgs), kMaxExperts, kRouteMaxK, kPlanThreads);
+
 // dtype: 0 fp32, 1 bf16, 2 fp16
 extern "C" {
+unsigned long long rx_expert_layout();
 // norm: [T][2] peak and 1 / sum, written when not null
 int rx_route_fwd(const void* z, long long ldz, int dtype, long long T, int E, int k, int renorm, float* w, int* ids,
                  float* norm, void* stream);

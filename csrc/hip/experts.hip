@@ -703,6 +703,8 @@ int route_bwd_pick(const void* z, long long ldz, const float* norm, const float*
 
 extern "C" {
 
+unsigned long long rx_expert_layout() { return kExpertLayout; }
+
 int rx_route_fwd(const void* z, long long ldz, int dtype, long long T, int E, int k, int renorm, float* w, int* ids,
                  float* norm, void* on) {
   hipStream_t stream = static_cast<hipStream_t>(on);

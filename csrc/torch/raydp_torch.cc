@@ -658,6 +658,9 @@ Tensor combine(const Tensor& rows_, const c10::optional<Tensor>& weights, const 
 }  // namespace
 
 PYBIND11_MODULE(raydp_torch, m) {
+  // its arguments are read by their layout in a library that is built by itself
+  if (rx_aw_layout() != kAwLayout || rx_expert_layout() != kExpertLayout)
+    throw py::import_error("raydp_torch.so and libhipkernels.so were built from different sources: build both again");
   py::register_local_exception_translator([](std::exception_ptr error) {
     try {
       if (error) std::rethrow_exception(error);
@@ -674,6 +677,7 @@ PYBIND11_MODULE(raydp_torch, m) {
   m.def("dispatch", &dispatch);
   m.def("combine", &combine);
   m.def("set_last_level", [](int64_t bytes) { std::swap(g_last_level, bytes); return bytes; });   // (tests: returns the old)
+  m.attr("layouts") = py::make_tuple(kAwLayout, kExpertLayout);
   m.attr("max_experts") = (int)kMaxExperts;
   m.attr("max_topk") = (int)kRouteMaxK;
   m.attr("block") = (int)kAwBlock;
