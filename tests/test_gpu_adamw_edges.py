@@ -173,3 +173,52 @@ def test_the_norm_of_a_step_without_gradients():
 
 # lengths around a wave's two scale blocks (512 elements), a step's workgroups (2048) and a norm's (8192)
 EDGES = [511, 512, 513, 767, 768, 769, 1024, 1535, 1536, 1537, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 8192, 8193, 16384, 16385]
+
+
+@pytest.mark.parametrize("clip", [None, 0.5])
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_steps_at_the_borders_of_the_kernels_pieces(dtype, bits, clip):
+    g = torch.Generator().manual_seed(11)
+    cfg = dict(lr=1e-2, weight_decay=0.1, max_grad_norm=clip, seed=6)
+    ps = [(torch.randn(n, generator=g) * 0.1).to(dtype).cuda().requires_grad_() for n in EDGES]
+    qs = [p.detach().cpu().clone().requires_grad_() for p in ps]
+    a, b = FusedAdamW(ps, state_bits=bits, **cfg), FusedAdamW(qs, state_bits=bits, **cfg)
+    for step in range(3):
+        oracle = Oracle.of(a, ps, bits)
+        before = [p.detach().double().cpu() for p in ps]
+        gs = [(torch.randn(n, generator=g) * torch.exp(2 * torch.randn(n, generator=g))).to(dtype) for n in EDGES]
+        for p, q, x in zip(ps, qs, gs):
+            p.grad, q.grad = x.cuda(), x.clone()
+        a.step()
+        b.step()
+        oracle.step([x.double() for x in gs], **cfg)
+        if clip is not None:        # both round the 64-bit norm once; their sums' orders differ by far less
+            assert abs(float(a.grad_norm) - oracle.norm) <= 2 ** -24 * oracle.norm
+        for i, (p, q) in enumerate(zip(ps, qs)):
+            for n, t in b.state[q].items():
+                assert torch.equal(a.state[p][n].cpu(), t), (EDGES[i], step, n)
+            got, want = p.detach().double().cpu(), oracle.p[i]
+            if dtype == torch.float32:      # three roundings of p, 21.5 of the update before anything cancels in it
+                tol = 3 * 2 ** -24 * (want.abs() + before[i].abs()) + 2 ** -19 * oracle.upd_terms[i]
+                assert ((got - want).abs() <= tol).all(), (EDGES[i], step)
+            else:       # one of two neighbours of a value that is off by as much: where p and the update cancel, 1e-2 leaves
+                        # 1e-8 with an error of 1e-9, and a neighbour is 2^-7 of the value away
+                off = 3 * 2 ** -24 * (want.abs() + before[i].abs()) + 2 ** -19 * oracle.upd_terms[i]
+                assert ((got - want).abs() <= off + 2 ** -7 * (want.abs() + off)).all(), (EDGES[i], step)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_clipping_at_the_borders_of_the_kernels_pieces(dtype):
+    g = torch.Generator().manual_seed(12)
+    ps = [nn.Parameter(torch.zeros(n, dtype=dtype, device="cuda")) for n in EDGES]
+    for p in ps:
+        p.grad = torch.randn(p.shape, generator=g).to(dtype).cuda()
+    before = [p.grad.double().cpu() for p in ps]
+    want = math.sqrt(sum(float(x.square().sum()) for x in before))
+    norm = clip_grad_norm_(ps, 0.25)
+    assert abs(float(norm) - want) <= 2 ** -24 * want
+    f = 0.25 / (want + 1e-6)
+    eps = 2 ** -8 if dtype == torch.bfloat16 else 2 ** -24
+    for p, x in zip(ps, before):      # the factor's rounding, the product's, and for bf16 the last one
+        assert ((p.grad.double().cpu() - x * f).abs() <= (eps + 2 * 2 ** -24) * (x * f).abs()).all(), len(x)
