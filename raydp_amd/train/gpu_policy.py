@@ -174,9 +174,9 @@ def graph_model(module):
     def _capture(args):
         bufs = [(b, b.detach().clone()) for b in module.buffers()]
         # the worker's native-BatchNorm policy (cudnn switched off around each BatchNorm call)
-        # is lifted while the graph is captured: a capture of that path's backward crashed at
-        # capture end on the GPU box (scripts/dev/hvd_graph_repro.py); the replay then runs the
-        # default BatchNorm kernels, which is what a replay's launch cost no longer cares about
+        # is lifted while the graph is captured: a capture of that path's backward ended the
+        # process at capture end; the replay then runs the default BatchNorm kernels, which is
+        # what a replay's launch cost no longer cares about
         from torch.nn.modules.batchnorm import _BatchNorm
         patched = _BatchNorm.forward
         plain = getattr(patched, "__wrapped__", None)
@@ -186,8 +186,8 @@ def graph_model(module):
             # The capture differentiates w.r.t. ALIASES of the parameters (fresh leaves on the
             # same storage), not the parameters: a parameter's gradient accumulator from an
             # earlier step is still alive while the caller holds that step's loss, and the
-            # capture's backward then synchronises with the default stream it was made on -- a
-            # crash at capture end on this stack (scripts/dev/graph_bisect.py: gm vs gm_delloss).
+            # capture's backward then synchronises with the default stream it was made on, which
+            # ends the process at capture end on this stack (not where the loss was dropped first).
             # A replay gets the real parameters (same storage: nothing copied), so autograd
             # accumulates their gradients as an eager backward would.
             samples = tuple(a.detach().clone() for a in args) + tuple(
