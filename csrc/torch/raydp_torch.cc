@@ -9,6 +9,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/engine.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
@@ -58,13 +59,16 @@ void check_trace(const char* what) {
 // Wrappers say that they are on the GPU and have no memory there, or not the values that stand in it.
 void check_memory(const Tensor& t, const char* what) {
   using c10::DispatchKey;
-  static const c10::DispatchKeySet odd({DispatchKey::Python, DispatchKey::Functionalize, DispatchKey::FuncTorchBatched,
-                                        DispatchKey::FuncTorchGradWrapper, DispatchKey::Batched, DispatchKey::ZeroTensor,
-                                        DispatchKey::Negative, DispatchKey::Conjugate});
+  constexpr c10::DispatchKeySet odd({DispatchKey::Python, DispatchKey::Functionalize, DispatchKey::FuncTorchBatched,
+                                     DispatchKey::FuncTorchGradWrapper, DispatchKey::Batched, DispatchKey::ZeroTensor,
+                                     DispatchKey::Negative, DispatchKey::Conjugate});
   if (t.defined() && t.key_set().has_any(odd))
     throw py::type_error(std::string(what) + ": a kernel cannot read a wrapped tensor (a fake or functional one, a transform's, "
                          "a subclass that dispatches, a lazy negation)");
 }
+
+// Is anything differentiated in forward mode at all? (Asked once for a list: a tensor's own answer costs 20 ns.)
+bool tangents() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 
 // A launch computes no tangent: the result would have none, without a word.
 void check_tangent(const Tensor& t, const char* what) {
@@ -172,12 +176,13 @@ void check_overlap(std::vector<std::pair<uintptr_t, uintptr_t>>& spans, const ch
 // grads: checked here, dense in any order of dimensions; returns the norm
 Tensor clip_grad_norm(const std::vector<Tensor>& all, double max_norm) {
   check_trace("clip_grad_norm_");
+  const bool forward = tangents();
   std::vector<Tensor> grads;
   const auto dev = all.at(0).device();
   std::vector<std::pair<uintptr_t, uintptr_t>> spans;
   for (const Tensor& g : all) {
     check_memory(g, "clip_grad_norm_");
-    check_tangent(g, "clip_grad_norm_");
+    if (forward) check_tangent(g, "clip_grad_norm_");
     if (g.layout() != at::kStrided) throw py::value_error("clip_grad_norm_: sparse gradients are not supported");
     if (g.device() != dev)
       throw py::value_error("clip_grad_norm_: gradients on " + dev.str() + " and " + g.device().str());
@@ -232,7 +237,6 @@ Tensor state_tensor(py::dict& st, const char* name, const Tensor& p) {
   if (o == nullptr || !THPVariable_Check(o))
     throw py::value_error(std::string("FusedAdamW: a parameter's state lacks ") + name);
   Tensor t = THPVariable_Unpack(o);
-  check_memory(t, "FusedAdamW");
   if (t.device() != p.device()) {      // state that was loaded before the model was moved
     t = t.to(p.device());
     st[name] = t;
@@ -245,6 +249,7 @@ Tensor state_tensor(py::dict& st, const char* name, const Tensor& p) {
 // clipping. Returns the norm, or None without clipping.
 c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_t seed) {
   check_trace("FusedAdamW.step");
+  const bool forward = tangents();
   std::vector<Group> all;
   std::vector<Tensor> grads;
   c10::optional<c10::Device> dev;
@@ -294,7 +299,7 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
       if (s.p.numel() == 0) continue;
       check_memory(s.p, "FusedAdamW");
       check_memory(s.g, "FusedAdamW");
-      check_tangent(s.g, "FusedAdamW");
+      if (forward) check_tangent(s.g, "FusedAdamW");
       if (!dev) dev = s.p.device();
       if (s.p.device() != *dev || s.g.device() != *dev)
         throw py::value_error("FusedAdamW: parameters with gradients on " + dev->str() + " and " +
@@ -328,7 +333,6 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
       }
       if (with_images && !bf16(s.p) && images.contains(py::int_(i))) {   // (a bf16 parameter is its own image)
         const Tensor img = images[py::int_(i)].cast<Tensor>();
-        check_memory(img, "FusedAdamW");
         if (!bf16(img) || !img.is_contiguous() || img.numel() != s.p.numel() || img.device() != *dev)
           throw py::value_error("FusedAdamW: a weight's image must be contiguous bf16 of its size");
         s.img = ptr<uint16_t>(img);
