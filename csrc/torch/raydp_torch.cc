@@ -282,8 +282,8 @@ c10::optional<Tensor> adamw_step(const py::list& groups, double max_norm, int64_
           throw std::runtime_error("FusedAdamW: a tensor lr on the host cannot be captured into a graph, whose replays would "
                                    "keep its value: put it on the parameters' device");
         grp.lr = l.item<double>();
-      } else if (l.scalar_type() != at::kFloat || l.device() != params[0].device())
-        throw py::type_error("FusedAdamW: a tensor lr must be fp32 on the parameters' device");
+      } else if (l.scalar_type() != at::kFloat || l.device() != params[0].device() || l.numel() != 1)
+        throw py::type_error("FusedAdamW: a tensor lr must be one fp32 value on the parameters' device");
       else
         grp.lr_dev = ptr<float>(l);
     } else {

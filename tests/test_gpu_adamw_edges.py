@@ -222,3 +222,14 @@ def test_clipping_at_the_borders_of_the_kernels_pieces(dtype):
     eps = 2 ** -8 if dtype == torch.bfloat16 else 2 ** -24
     for p, x in zip(ps, before):      # the factor's rounding, the product's, and for bf16 the last one
         assert ((p.grad.double().cpu() - x * f).abs() <= (eps + 2 * 2 ** -24) * (x * f).abs()).all(), len(x)
+
+
+def test_a_rate_of_no_or_many_elements_is_refused():
+    p = torch.ones(4, device="cuda", requires_grad=True)
+    p.grad = torch.ones(4, device="cuda")
+    opt = FusedAdamW([p], lr=torch.tensor(1e-3, device="cuda"))
+    for n in (0, 2):
+        opt.param_groups[0]["lr"] = torch.ones(n, device="cuda")
+        with pytest.raises(TypeError, match="lr"):
+            opt.step()
+    assert (p == 1).all()
