@@ -606,6 +606,16 @@ Tensor gather(const Tensor& position, const Tensor& source, const Tensor& h, con
   return out;
 }
 
+// What the row kernels take from a plan's tensors by address: a plan can be put together, or changed, by hand.
+void check_plan(const Tensor& position, const Tensor& source, const Tensor& rows, bool samples, const char* what) {
+  for (const Tensor& t : {position, source})
+    if (t.scalar_type() != at::kInt || !t.is_contiguous() || t.device() != rows.device())
+      throw py::value_error(std::string(what) + ": a plan's position and source must be contiguous int32 on the rows' device");
+  if (position.dim() != 2 || position.size(1) < 1 || source.dim() != 1 || rows.size(0) != (samples ? position : source).size(0))
+    throw py::value_error(std::string(what) + ": the plan's position must be [T, k] and its source [rows], with " +
+                          (samples ? "T samples" : "that many expert rows") + " given");
+}
+
 struct Dispatch : torch::autograd::Function<Dispatch> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& position, const Tensor& source) {
     ctx->save_for_backward({position, source});
@@ -641,6 +651,7 @@ struct Combine : torch::autograd::Function<Combine> {
 Tensor dispatch(const Tensor& x, const Tensor& position, const Tensor& source) {
   check_trace("dispatch");
   for (const Tensor& t : {x, position, source}) check_memory(t, "dispatch");
+  check_plan(position, source, x, true, "dispatch");
   check_tangent(x, "dispatch");
   if (x.requires_grad() && at::GradMode::is_enabled()) return Dispatch::apply(x, position, source);
   return scatter(position, source, x, Tensor(), Tensor()).first;
@@ -649,6 +660,8 @@ Tensor dispatch(const Tensor& x, const Tensor& position, const Tensor& source) {
 Tensor combine(const Tensor& rows_, const c10::optional<Tensor>& weights, const Tensor& position, const Tensor& source) {
   check_trace("combine");
   for (const Tensor& t : {rows_, weights ? *weights : Tensor(), position, source}) check_memory(t, "combine");
+  check_plan(position, source, rows_, false, "combine");
+  if (weights && weights->sizes() != position.sizes()) throw py::value_error("combine: one weight for each place in the plan");
   check_tangent(rows_, "combine");
   if (weights) check_tangent(*weights, "combine");
   const Tensor rows = rows_.contiguous();
