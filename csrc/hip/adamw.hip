@@ -93,8 +93,8 @@ __device__ __forceinline__ uint32_t aw_dither_bf16x2(float x, float y, uint32_t 
   return __builtin_amdgcn_perm(b, a, 0x07060302u);
 }
 
-// Loads and stores of 4 consecutive elements from any address of the type's; n: how many there are (<= 4). Parameters are
-// aligned, but gradients may be slices of a bucket: gfx950 takes vectors at any element. NT: streamed past the caches. A step
+// Loads and stores of 4 consecutive elements from any address of the type's; n: how many there are (<= 4). Parameters and
+// gradients may be slices of a larger buffer: gfx950 takes vectors at any element. NT: streamed past the caches. A step
 // that touches more than the 256 MB of the last-level cache gains by that (24 M fp32 with 32-bit moments, 384 MB:
 // 128 -> 112 us; 48 M with 8 bits: 148 -> 133), one that fits loses (16 M, 256 MB: 68 -> 76), so the host goes by the bytes.
 typedef f32x4 __attribute__((aligned(4))) f32x4_u;
@@ -204,8 +204,8 @@ struct AwPlace {       // where a launch's workgroup works (wave-uniform)
   long long n;
 };
 
-// One lane's share of a scale block: 4 elements. FULL: the block lies inside the tensor and the vectors are aligned, so
-// loads and stores are whole and no lane branches; otherwise element by element under the tensor's end.
+// One lane's share of a scale block: 4 elements. FULL: the block lies inside the tensor, so loads and stores are
+// whole and no lane branches; otherwise element by element under the tensor's end.
 template <bool BITS8, bool BF16, bool NT, bool FULL>
 struct AwLane {
   f32x4 p, g, m, v;
@@ -309,7 +309,8 @@ struct AwLane {
 // before the first is worked on (bf16: 104 -> 99 us for 48 M; four give nothing more). Coding, dither and update are about 65
 // issue slots an element, of the 76 that bf16 leaves per element at 5 TB/s: they had to come down from 90 (bytes packed
 // by v_perm, m's code decoded by one sign-extending shift, square root and reciprocal to 1 ulp). 35.4 M fp32 in 17 tensors:
-// 95 us with 8 bits (6.0 TB/s), 160 us with 32 (6.2); 16.8 M bf16 in 64 tensors with 8 bits: 35 us (4.8).
+// 92 us with 8 bits (6.1 TB/s), 161 us with 32 (6.1); bf16: 16.8 M in 64 tensors with 8 bits 36 us (4.6), 50.3 M in 3 with 32
+// bits 178 us (6.2).
 template <bool BITS8, bool BF16, bool NT>
 __global__ __launch_bounds__(256) void aw_step_kernel(AwStep c) {
   const AwHead head = *c.head;
@@ -410,7 +411,8 @@ __global__ __launch_bounds__(256) void aw_prep_kernel(AwPrep a) {
 // Sums of squares in 64 bits: the norm then does not depend on the order of the sum in any of its 32 bits but by chance.
 // Bound by memory (a conversion and a 64-bit multiply-add an element fit beside it): 8192 elements are loaded before the
 // first is squared, 1024 workgroups give 16 waves a CU. 50 M fp32 in 36 us (5.6 TB/s; 4096 elements: 38, 512 workgroups: 52),
-// bf16 in 20; 67 M fp32 in 256 tensors, streamed, 46 us for both launches (55 with 128 tensors a launch).
+// bf16 in 20; 67 M fp32 in 256 tensors, streamed, 43 us, and 3.8 for a scaling that finds a factor of 1
+// (with 128 tensors a launch: 55 in all).
 // 4 x 4 (bf16: 2 x 8) elements of a lane, in flight together
 template <bool BF16, bool FULL, bool NT>
 __device__ __forceinline__ double aw_squares(const void* g, long long i, long long n) {

@@ -31,8 +31,7 @@
 #include <type_traits>
 
 // No implicit multiply-add contraction in the training kernels: whether the compiler fuses an
-// a * b + c depends on the inlining context (and on what the SLP vectorizer pairs into v_pk_*
-// ops), so the same expression could round differently in the launch-per-step kernel and in
+// a * b + c depends on the inlining context, so the same expression could round differently in the launch-per-step kernel and in
 // the persistent epoch kernel. Fused multiply-adds are written out (fmaf) where they pay.
 #pragma clang fp contract(off)
 
@@ -604,7 +603,7 @@ __device__ __forceinline__ f32x4 rx_rowmask(f32x4 v, int mt, int lg, int nvalid)
   return v;
 }
 
-// Sum of the MT x 4 (row-masked) values of one lane: a tree over packed-fp32 adds (depth
+// Sum of the MT x 4 (row-masked) values of one lane: a tree over 4-vector adds (depth
 // log2(MT) + 2) instead of a serial chain of MT * 4 dependent adds.
 template <int MT, bool FULL>
 __device__ __forceinline__ float rx_lane_sum(const f32x4* a, int lg, int nvalid) {
@@ -1218,7 +1217,7 @@ __device__ __forceinline__ void layer_forward(const D& d, const LY& ly, const NX
         }
       } else {
         // branch-free: every element computes its terms, invalid ones (padded rows / columns)
-        // are selected out; per-lane sums in packed-fp32 vectors
+        // are selected out; per-lane sums in 4-vectors
         const float hb = 0.5f * beta, inv_beta = 1.f / beta, h_inv_beta = 0.5f * inv_beta;
         f32x4 l4 = f32x4{0.f, 0.f, 0.f, 0.f}, a4 = l4, s4 = l4, c4 = l4, g4s = l4;
 #pragma unroll
@@ -1636,7 +1635,7 @@ __device__ __forceinline__ void layer_backward(const D& d, const LY& ly, const P
         sg = bsg[j];
         sgx = bsgx[j];
       } else {
-        // batch sums of dL/dy and dL/dy * x_hat: packed-fp32 trees, then across the lane groups
+        // batch sums of dL/dy and dL/dy * x_hat: trees over 4-vectors, then across the lane groups
         f32x4 a4 = g4[0], b4 = g4[0] * xh4[0];
 #pragma unroll
         for (int mt = 1; mt < MT; ++mt) {

@@ -72,9 +72,9 @@ __device__ __forceinline__ void opt_update_pre(const O& o, float& pv, float& mv,
   }
 }
 
-// Four elements at once: Adam / AdamW in packed-fp32 operations (v_pk_fma_f32 / v_pk_mul_f32 on
-// pairs), the same operations per element as opt_update_pre -- so the same bits; other algorithms
-// and options element by element.
+// Four elements at once: Adam / AdamW on 4-vectors (their instructions interleave), the same
+// operations per element as opt_update_pre -- so the same bits; other algorithms and options
+// element by element.
 template <class O>
 __device__ __forceinline__ void opt_update_pre4(const O& o, f32x4& pv, f32x4& mv, f32x4& vv, f32x4 g, float lr,
                                                 float nlr_bc1, float rs_bc2, int first) {
